@@ -113,6 +113,12 @@ SIGNATURES = {
     "hymt_rows_swiglu": [_vp, _vp, _i, _i, _vp],
     "hymt_rows_swiglu_bf16": [_vp, _vp, _i, _i, _vp],
     "hymt_gemm_swiglu": [_vp, _vp, _vp, _vp, _i, _vp],
+    "hymt_weight_i8": [_vp, _vp],
+    "hymt_weight_i8_data": [_vp, ctypes.POINTER(_vp), ctypes.POINTER(_vp)],
+    "hymt_to_i8": [_vp, _vp, _i, _i, _i, _vp, _vp],
+    "hymt_rows_rmsnorm_i8": [_vp, _vp, _vp, _i, _i, _i, _vp, ctypes.c_float, _vp, _vp],
+    "hymt_gemm_i8": [_vp, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _i, _i],
+    "hymt_gemm_i8_swiglu": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _i],
     "hymt_to_bf16": [_vp, _vp, ctypes.c_size_t, _vp],
     "hymt_model_create": [_vp, _i, _i, _i, _i, ctypes.c_float, ctypes.POINTER(_vp)],
     "hymt_model_set_layer": [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],

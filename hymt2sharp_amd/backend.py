@@ -283,6 +283,44 @@ class HipBackend:
     def to_bf16(self, x_dev, count: int, out_dev):
         N.check(self._lib.hymt_to_bf16(self._h, x_dev, count, out_dev))
 
+    # ---- products and norms in 8-bit integers (device pointers)
+    def weight_i8(self, w):
+        """Give W int8 codes and a scale per row (synchronous)."""
+        N.check(self._lib.hymt_weight_i8(self._h, w))
+
+    def weight_i8_data(self, w) -> tuple[int, int]:
+        """The device addresses of W's codes [rows][cols] and scales [rows]."""
+        q, s = ctypes.c_void_p(), ctypes.c_void_p()
+        N.check(self._lib.hymt_weight_i8_data(w, ctypes.byref(q), ctypes.byref(s)))
+        return q.value, s.value
+
+    def to_i8(self, x_dev, m: int, n: int, out_dev, scale_dev, x_dtype: int = N.F32):
+        """out[m][n], scale[m] = the int8 codes of x's rows (fp32 or bf16):
+        rint(127 v / max|v|) and max|v| / 127."""
+        N.check(self._lib.hymt_to_i8(self._h, x_dev, x_dtype, m, n, out_dev, scale_dev))
+
+    def rows_rmsnorm_i8(self, x_dev, m: int, n: int, norm_w_dev, eps: float, out_dev, scale_dev, add=None,
+                        add_dtype: int = N.BF16):
+        """out, scale = the int8 codes of RMSNorm(x) * norm_w; with add (bf16 or
+        fp32 rows) x becomes x + add first."""
+        N.check(self._lib.hymt_rows_rmsnorm_i8(self._h, x_dev, add, add_dtype, m, n, norm_w_dev, eps, out_dev,
+                                               scale_dev))
+
+    def gemm_i8(self, w_dev, w_scale_dev, n: int, k: int, x_dev, x_scale_dev, m: int, y_dev, ldy: int | None = None,
+                accumulate: bool = False, out_bf16: bool = False):
+        """y[m][n] (+)= w_scale x_scale (x[m][k] . w[n][k]^T) of int8 codes (y fp32
+        or bf16, rows ldy elements apart)."""
+        flags = (N.GEMM_ACCUMULATE if accumulate else 0) | (N.GEMM_OUT_BF16 if out_bf16 else 0)
+        N.check(self._lib.hymt_gemm_i8(self._h, w_dev, w_scale_dev, n, k, x_dev, x_scale_dev, m, y_dev,
+                                       n if ldy is None else ldy, flags))
+
+    def gemm_i8_swiglu(self, gate_dev, gate_scale_dev, up_dev, up_scale_dev, f: int, k: int, x_dev, x_scale_dev,
+                       m: int, act_dev, ld: int | None = None):
+        """act[m][f] = bf16(silu(g) u) of the int8 products with the gate and the
+        up rows."""
+        N.check(self._lib.hymt_gemm_i8_swiglu(self._h, gate_dev, gate_scale_dev, up_dev, up_scale_dev, f, k, x_dev,
+                                              x_scale_dev, m, act_dev, f if ld is None else ld))
+
     def stream(self) -> int:
         s = ctypes.c_void_p()
         N.check(self._lib.hymt_get_stream(self._h, ctypes.byref(s)))

@@ -38,6 +38,8 @@ HIP_SOURCES = {
     "gemm_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     # the same, for the same reason
     "gemm_skinny.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "gemm_i8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "rows_i8.hip": [],
     "ktimer.cpp": [],
 }
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

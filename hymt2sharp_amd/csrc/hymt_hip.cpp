@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "attn_kernels.hpp"
+#include "int8.hpp"
 #include "ktimer.hpp"
 #include "kv_pages.hpp"
 #include "weights.hpp"
@@ -1040,6 +1041,8 @@ struct hymt_weight {
     void *mem = nullptr;
     size_t bytes = 0;
     uint16_t *dense = nullptr;  // bf16 [rows][cols] copy for the prefill GEMMs (hymt_weight_dense)
+    int8_t *i8 = nullptr;       // int8 [rows][cols] codes (hymt_weight_i8) ...
+    float *i8_scale = nullptr;  // ... and their scales [rows], in the same allocation
 };
 
 // A Q4_K, Q6_K or Q8_0 matrix into its tiles, through a device buffer of at
@@ -1129,6 +1132,10 @@ int hymt_weight_free(hymt_ctx *c, hymt_weight *w) {
         const hipError_t e2 = hipFree(w->dense);
         if (e == hipSuccess) e = e2;
     }
+    if (w->i8) {
+        const hipError_t e3 = hipFree(w->i8);
+        if (e == hipSuccess) e = e3;
+    }
     delete w;
     if (e != hipSuccess) return fail(HYMT_E_DEVICE, std::string("hipFree: ") + hipGetErrorString(e));
     return HYMT_OK;
@@ -1139,7 +1146,9 @@ int hymt_weight_info(const hymt_weight *w, int *type, int *rows, int *cols, size
     if (type) *type = w->dev.type;
     if (rows) *rows = w->dev.rows;
     if (cols) *cols = w->dev.cols;
-    if (device_bytes) *device_bytes = w->bytes + (w->dense ? (size_t)w->dev.rows * w->dev.cols * 2 : 0);
+    if (device_bytes)
+        *device_bytes = w->bytes + (w->dense ? (size_t)w->dev.rows * w->dev.cols * 2 : 0) +
+                        (w->i8 ? (size_t)w->dev.rows * (w->dev.cols + 4) : 0);
     return HYMT_OK;
 }
 
@@ -1350,6 +1359,151 @@ int hymt_to_bf16(hymt_ctx *c, const float *x, size_t count, void *out) {
     try {
         HIP_TRY(hipSetDevice(c->device));
         HIP_TRY(hymt::launch_to_bf16(x, count, (uint16_t *)out, c->stream));
+    } catch (const HipError &e) {
+        return map_hip(e);
+    }
+    return HYMT_OK;
+}
+
+// ---- products and norms in 8-bit integers ---------------------------------------
+
+namespace {
+bool misaligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) != 0; }
+
+int check_i8_rows(int m, int n) {
+    if (m < 0) return fail(HYMT_E_ARG, "negative row count");
+    if (n < 4 || n > 8192 || n % 4 != 0)
+        return fail(HYMT_E_UNSUPPORTED, "row length must be a multiple of 4 up to 8192");
+    return HYMT_OK;
+}
+
+// What the two int8 products check alike (up null: no up rows).
+int check_i8_gemm(const I8Gemm &g, size_t y_bytes) {
+    if (g.m < 0) return fail(HYMT_E_ARG, "negative row count");
+    if (g.n < 1 || g.ldy < g.n) return fail(HYMT_E_ARG, "n must be positive and the output's rows at least n apart");
+    if (g.k % kI8StepK || g.k < 2 * kI8StepK || g.k > kI8MaxK)
+        return fail(HYMT_E_UNSUPPORTED, "k must be a multiple of 128, 256 to 65536");
+    if (misaligned(g.w, 16) || misaligned(g.up, 16) || misaligned(g.x, 16))
+        return fail(HYMT_E_ARG, "codes must be 16-byte aligned");
+    if (misaligned(g.ws, 4) || misaligned(g.us, 4) || misaligned(g.xs, 4) || misaligned(g.y, y_bytes))
+        return fail(HYMT_E_ARG, "scales and the output must be aligned to their elements");
+    return HYMT_OK;
+}
+}  // namespace
+
+int hymt_weight_i8(hymt_ctx *c, hymt_weight *w) {
+    if (int r = check_ctx(c, false, true)) return r;
+    if (!w) return fail(HYMT_E_ARG, "null weight");
+    if (int r = refuse_in_capture(c, "hymt_weight_i8")) return r;
+    if (w->i8) return HYMT_OK;
+    const size_t rows = w->dev.rows, cols = w->dev.cols;
+    const int chunk = (int)std::max<size_t>(1, std::min<size_t>(rows, (64u << 20) / (cols * 4)));
+    void *mem = nullptr, *tmp = nullptr;
+    try {
+        HIP_TRY(hipSetDevice(c->device));
+        HIP_TRY(hipMalloc(&mem, rows * (cols + 4)));
+        HIP_TRY(hipMalloc(&tmp, (size_t)chunk * cols * 4));
+        int8_t *codes = (int8_t *)mem;
+        float *scales = (float *)(codes + rows * cols);  // cols is a multiple of 2048
+        for (size_t r0 = 0; r0 < rows; r0 += chunk) {
+            const int n = (int)std::min<size_t>(chunk, rows - r0);
+            HIP_TRY(launch_rows(w->dev, nullptr, (int)r0, n, (float *)tmp, c->stream));
+            HIP_TRY(launch_to_i8(tmp, false, n, (int)cols, codes + r0 * cols, scales + r0, c->stream));
+        }
+        HIP_TRY(hipStreamSynchronize(c->stream));
+        HIP_TRY(hipFree(tmp));
+        w->i8 = codes;
+        w->i8_scale = scales;
+    } catch (const HipError &e) {
+        if (tmp) (void)hipFree(tmp);
+        if (mem) (void)hipFree(mem);
+        return map_hip(e);
+    }
+    return HYMT_OK;
+}
+
+int hymt_weight_i8_data(const hymt_weight *w, const int8_t **codes, const float **scales) {
+    if (!w || !codes || !scales) return fail(HYMT_E_ARG, "null argument");
+    if (!w->i8) return fail(HYMT_E_STATE, "weight has no int8 codes (hymt_weight_i8)");
+    *codes = w->i8;
+    *scales = w->i8_scale;
+    return HYMT_OK;
+}
+
+int hymt_to_i8(hymt_ctx *c, const void *x, int x_dtype, int m, int n, int8_t *out, float *scale) {
+    if (int r = check_ctx(c, false, false)) return r;
+    if (!x || !out || !scale) return fail(HYMT_E_ARG, "null input or output");
+    if (x_dtype != HYMT_F32 && x_dtype != HYMT_BF16) return fail(HYMT_E_UNSUPPORTED, "x must be fp32 or bf16");
+    if (int r = check_i8_rows(m, n)) return r;
+    if (misaligned(x, x_dtype == HYMT_F32 ? 16 : 8) || misaligned(out, 4) || misaligned(scale, 4))
+        return fail(HYMT_E_ARG, "x must be 16-byte aligned (bf16: 8), out and scale 4-byte aligned");
+    if (!c->has_device()) return fail(HYMT_E_NO_DEVICE, "context has no device");
+    TimedCall timed(call_timer(c), "to_i8", m);
+    try {
+        HIP_TRY(hipSetDevice(c->device));
+        HIP_TRY(launch_to_i8(x, x_dtype == HYMT_BF16, m, n, out, scale, c->stream));
+    } catch (const HipError &e) {
+        return map_hip(e);
+    }
+    return HYMT_OK;
+}
+
+int hymt_rows_rmsnorm_i8(hymt_ctx *c, float *x, const void *add, int add_dtype, int m, int n, const float *norm_w,
+                         float eps, int8_t *out, float *scale) {
+    if (int r = check_ctx(c, false, false)) return r;
+    if (!x || !norm_w || !out || !scale) return fail(HYMT_E_ARG, "null input, weight or output");
+    if (add && add_dtype != HYMT_F32 && add_dtype != HYMT_BF16)
+        return fail(HYMT_E_UNSUPPORTED, "add must be fp32 or bf16");
+    if (int r = check_i8_rows(m, n)) return r;
+    if (!(eps >= 0.f)) return fail(HYMT_E_ARG, "eps must not be negative");
+    if (misaligned16(x) || misaligned16(norm_w) || misaligned(add, add_dtype == HYMT_F32 ? 16 : 8) ||
+        misaligned(out, 4) || misaligned(scale, 4))
+        return fail(HYMT_E_ARG, "x, norm_w and an fp32 add must be 16-byte aligned (a bf16 add 8), out and scale 4");
+    if (!c->has_device()) return fail(HYMT_E_NO_DEVICE, "context has no device");
+    TimedCall timed(call_timer(c), "rows_rmsnorm_i8", m);
+    try {
+        HIP_TRY(hipSetDevice(c->device));
+        HIP_TRY(launch_rows_rmsnorm_i8(x, add, add_dtype == HYMT_BF16, m, n, norm_w, eps, out, scale, c->stream));
+    } catch (const HipError &e) {
+        return map_hip(e);
+    }
+    return HYMT_OK;
+}
+
+int hymt_gemm_i8(hymt_ctx *c, const int8_t *w, const float *w_scale, int n, int k, const int8_t *x,
+                 const float *x_scale, int m, void *y, int ldy, int flags) {
+    if (int r = check_ctx(c, false, false)) return r;
+    if (!w || !w_scale || !x || !x_scale || !y) return fail(HYMT_E_ARG, "null matrix or scales");
+    if (flags & ~(HYMT_GEMM_ACCUMULATE | HYMT_GEMM_OUT_BF16)) return fail(HYMT_E_ARG, "unknown gemm flags");
+    if ((flags & HYMT_GEMM_ACCUMULATE) && (flags & HYMT_GEMM_OUT_BF16))
+        return fail(HYMT_E_ARG, "HYMT_GEMM_ACCUMULATE needs an fp32 output");
+    const I8Gemm g{w, w_scale, nullptr, nullptr, x, x_scale, y, n, k, m, ldy};
+    if (int r = check_i8_gemm(g, flags & HYMT_GEMM_OUT_BF16 ? 2 : 4)) return r;
+    if (!c->has_device()) return fail(HYMT_E_NO_DEVICE, "context has no device");
+    TimedCall timed(call_timer(c), "gemm_i8", m);
+    try {
+        HIP_TRY(hipSetDevice(c->device));
+        HIP_TRY(launch_gemm_i8(g, flags & HYMT_GEMM_OUT_BF16 ? kI8Bf16 : flags & HYMT_GEMM_ACCUMULATE ? kI8Acc : kI8F32,
+                               c->stream));
+    } catch (const HipError &e) {
+        return map_hip(e);
+    }
+    return HYMT_OK;
+}
+
+int hymt_gemm_i8_swiglu(hymt_ctx *c, const int8_t *gate, const float *gate_scale, const int8_t *up,
+                        const float *up_scale, int f, int k, const int8_t *x, const float *x_scale, int m, void *act,
+                        int ld) {
+    if (int r = check_ctx(c, false, false)) return r;
+    if (!gate || !gate_scale || !up || !up_scale || !x || !x_scale || !act)
+        return fail(HYMT_E_ARG, "null matrix or scales");
+    const I8Gemm g{gate, gate_scale, up, up_scale, x, x_scale, act, f, k, m, ld};
+    if (int r = check_i8_gemm(g, 2)) return r;
+    if (!c->has_device()) return fail(HYMT_E_NO_DEVICE, "context has no device");
+    TimedCall timed(call_timer(c), "gemm_i8_swiglu", m);
+    try {
+        HIP_TRY(hipSetDevice(c->device));
+        HIP_TRY(launch_gemm_i8_swiglu(g, c->stream));
     } catch (const HipError &e) {
         return map_hip(e);
     }

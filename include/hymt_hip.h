@@ -391,6 +391,60 @@ int hymt_to_bf16(hymt_ctx *ctx, const float *x, size_t count, void *out);
 int hymt_gemm_swiglu(hymt_ctx *ctx, const hymt_weight *gate, const hymt_weight *up, const void *x, int m,
                      void *act);
 
+/* ---- products and norms in 8-bit integers --------------------------------------
+ * The prefill's GEMMs and the row kernels between them over int8 codes: a
+ * weight matrix has one fp32 scale per row (output channel), an activation
+ * matrix one per row (token).  They have no counterpart in the reference's
+ * GPU backends; its CPU path quantizes activations to 8 bits too (Q8K.cs:12-137).
+ *
+ * A row v of n values is coded as q = rint(127 v / a), a = max|v|, ties to
+ * even, with scale = a / 127: the codes are those of exact arithmetic, so they
+ * do not depend on the kernel that made them.  A row of zeros has zeros and
+ * the scale 0; a row that holds a NaN or an infinity has zeros and the scale
+ * NaN, so that what is computed from it is NaN.
+ *
+ * All tensors are device pointers, the calls only enqueue work on the context's
+ * stream, use no workspace and may be recorded.  Inputs and outputs of a call
+ * must not overlap unless stated.  With 0 rows a call does nothing. */
+
+/* Give the weight int8 codes [rows][cols] and a scale per row of its
+ * dequantized values (held until hymt_weight_free; rows * (cols + 4) bytes).
+ * Synchronous; not recordable. */
+int hymt_weight_i8(hymt_ctx *ctx, hymt_weight *w);
+/* The device addresses of those codes and scales; HYMT_E_STATE without. */
+int hymt_weight_i8_data(const hymt_weight *w, const int8_t **codes, const float **scales);
+
+/* out[i][n], scale[i]: the codes of m rows of x, HYMT_F32 or HYMT_BF16 as
+ * x_dtype.  n a multiple of 4 up to 8192; x 16-byte aligned (bf16: 8), out
+ * and scale 4-byte aligned. */
+int hymt_to_i8(hymt_ctx *ctx, const void *x, int x_dtype, int m, int n, int8_t *out, float *scale);
+
+/* The codes of x[i] / sqrt(mean(x[i]^2) + eps) * norm_w for m rows of n
+ * fp32 values (hymt_rows_rmsnorm with an 8-bit output).  With add not NULL,
+ * [m][n] of HYMT_F32 or HYMT_BF16 as add_dtype, x is first replaced by
+ * fp32(x + add), the residual after the addition, and the norm is of that.
+ * The mean is held in fp64.  n a multiple of 4 up to 8192, eps >= 0; x, norm_w
+ * and an fp32 add 16-byte aligned (a bf16 add 8), out and scale 4. */
+int hymt_rows_rmsnorm_i8(hymt_ctx *ctx, float *x, const void *add, int add_dtype, int m, int n,
+                         const float *norm_w, float eps, int8_t *out, float *scale);
+
+/* y[t][f] = w_scale[f] x_scale[t] sum_k x[t][k] w[f][k] for m tokens and n
+ * channels, w [n][k] and x [m][k] int8 (-128 too).  The sum is exact, and fp32
+ * is multiplied by w_scale, then by x_scale, so the result does not depend on the
+ * kernel or on m.  y is fp32, rows ldy >= n elements apart, or as the flags
+ * say: HYMT_GEMM_ACCUMULATE y += in fp32, HYMT_GEMM_OUT_BF16 bf16.  k a
+ * multiple of 128, 256 to 65536; w and x 16-byte aligned, y and the scales by
+ * their elements. */
+int hymt_gemm_i8(hymt_ctx *ctx, const int8_t *w, const float *w_scale, int n, int k, const int8_t *x,
+                 const float *x_scale, int m, void *y, int ldy, int flags);
+
+/* act[t][f] = bf16(silu(g) u), rows ld >= f elements apart, with g and u the
+ * fp32 products of x with the f gate rows and the f up rows (each [f][k]; of
+ * one [gate; up] matrix the up rows start at gate + f k). */
+int hymt_gemm_i8_swiglu(hymt_ctx *ctx, const int8_t *gate, const float *gate_scale, const int8_t *up,
+                        const float *up_scale, int f, int k, const int8_t *x, const float *x_scale, int m,
+                        void *act, int ld);
+
 /* ---- the model's decode step, enqueued natively ---------------------------------
  * IComputeBackend.ForwardStep for one token (IComputeBackend.cs:40-47) in one
  * call: the sequence of HunyuanDenseModel.DecodeBlock
