@@ -1,8 +1,16 @@
 // gemm_i8.hip -- products of int8 codes (gfx950): y[t][f] = ws[f] xs[t] sum_k
-// x[t][k] w[f][k] on v_mfma_i32_16x16x64_i8, the sum exact in int32.
+// x[t][k] w[f][k] on v_mfma_i32_16x16x64_i8, the sum exact in int32, then fp32
+// products with the two scales; fp32, added to fp32, bf16, or (SwiGLU) the bf16
+// silu(g) u of two such products.
+//
+// The sum is exact, so its order is free: every kernel and tile below gives the
+// same bits, and which one runs is a matter of time alone.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <cstdlib>
+#include <cstring>
 
 #include "device_common.hpp"
 #include "int8.hpp"
@@ -15,71 +23,571 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 enum Out { kF32, kAcc, kBf16, kGlu };
 
-// 4 features f .. f + 3 of token t
+constexpr int kBK = kI8StepK;  // k (bytes of a row) per stage
+constexpr int kFrag = 1024;    // bytes of one 16 x 64 operand fragment
+constexpr int kPair = 2048;    // one row block's 16 rows x 128 k of a stage
+constexpr int kGroupF = 4;     // feature tiles walked together (L2 reuse)
+
+struct Args {
+    I8Gemm g;
+    int tiles, tiles_f, tiles_t;
+    int per_xcd;  // workgroups per XCD: ceil(tiles / 8)
+    bool vec;     // the output takes 16-byte stores of whole chunks
+};
+
+// s_waitcnt with vmcnt n (<= 63) alone, with lgkmcnt 0 too, and lgkmcnt 0 alone
+// (gfx9 encoding: vmcnt in bits 3:0 and 15:14, expcnt 6:4, lgkmcnt 11:8)
+template <int N, bool LGKM = false> __device__ __forceinline__ void wait_vm() {
+    static_assert(N >= 0 && N <= 63, "vmcnt");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (LGKM ? 0 : 15 << 8));
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wait_lgkm() {
+    __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));
+    asm volatile("" ::: "memory");
+}
+
+// The one arithmetic of an output: the channel's scale first, then the token's,
+// fused with the addition where there is one.
+__device__ __forceinline__ float scaled(int s, float ws) { return (float)s * ws; }
+__device__ __forceinline__ float glu(int g, int u, float ws, float us, float xs) {
+    return silu_fast(scaled(g, ws) * xs) * (scaled(u, us) * xs);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    return (uint32_t)f32_to_bf16(a) | ((uint32_t)f32_to_bf16(b) << 16);
+}
+
+// Features f .. f + 3 of token t from the sums, where f + e < n.
 template <int OUT>
-__device__ __forceinline__ void store4(const I8Gemm &g, int t, int f, i32x4 acc, i32x4 up) {
-    const float xs = g.xs[t];
+__device__ __forceinline__ void store4(const Args &a, int t, int f, i32x4 s, i32x4 up, const float (&ws)[4],
+                                       const float (&us)[4], float xs) {
+    const I8Gemm &g = a.g;
+    const size_t at = (size_t)t * g.ldy + f;
+    float v[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        if (f + e >= g.n) break;
-        const size_t at = (size_t)t * g.ldy + f + e;
-        const float a = (float)acc[e] * g.ws[f + e], v = a * xs;
-        if constexpr (OUT == kGlu)
-            ((uint16_t *)g.y)[at] = f32_to_bf16(silu_fast(v) * ((float)up[e] * g.us[f + e] * xs));
-        else if constexpr (OUT == kBf16)
-            ((uint16_t *)g.y)[at] = f32_to_bf16(v);
-        else if constexpr (OUT == kAcc)
-            ((float *)g.y)[at] = fmaf(a, xs, ((float *)g.y)[at]);
-        else
-            ((float *)g.y)[at] = v;
+    for (int e = 0; e < 4; e++)
+        v[e] = OUT == kGlu ? glu(s[e], up[e], ws[e], us[e], xs) : OUT == kAcc ? scaled(s[e], ws[e]) : scaled(s[e], ws[e]) * xs;
+    if constexpr (OUT == kGlu || OUT == kBf16) {
+        uint16_t *y = (uint16_t *)g.y + at;
+        if (a.vec && f + 4 <= g.n) {
+            *(uint2 *)y = make_uint2(pack2(v[0], v[1]), pack2(v[2], v[3]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (f + e < g.n) y[e] = f32_to_bf16(v[e]);
+        }
+    } else {
+        float *y = (float *)g.y + at;
+        if (a.vec && f + 4 <= g.n) {
+            if constexpr (OUT == kAcc) {
+                const float4 o = *(const float4 *)y;
+                *(float4 *)y = make_float4(fmaf(v[0], xs, o.x), fmaf(v[1], xs, o.y), fmaf(v[2], xs, o.z), fmaf(v[3], xs, o.w));
+            } else {
+                *(float4 *)y = make_float4(v[0], v[1], v[2], v[3]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (f + e < g.n) y[e] = OUT == kAcc ? fmaf(v[e], xs, y[e]) : v[e];
+        }
     }
 }
 
-// 64 features x 64 tokens by 4 waves of 32 x 32, operands straight from memory
-template <int OUT>
-__global__ __launch_bounds__(256) void simple_kernel(I8Gemm g) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, grp = lane >> 4, c = lane & 15;
-    const int tiles_f = (g.n + 63) / 64;
-    const int f0 = (blockIdx.x % tiles_f) * 64 + 32 * (wave & 1), t0 = (blockIdx.x / tiles_f) * 64 + 32 * (wave >> 1);
-    i32x4 acc[2][2] = {}, up[2][2] = {};
-    size_t wo[2], xo[2];
-    for (int i = 0; i < 2; i++) {
-        wo[i] = (size_t)min(f0 + 16 * i + c, g.n - 1) * g.k + 16 * grp;
-        xo[i] = (size_t)min(t0 + 16 * i + c, g.m - 1) * g.k + 16 * grp;
+// ---- tiles ---------------------------------------------------------------------
+//
+// Workgroup tile: TF = 32 IF features x TT = 32 JT tokens by 2 x WT waves, wave
+// (wf, wt) the tile's feature half wf and token part wt, IF x BJ blocks of 16 x 16.
+//
+// k advances in stages of 128: a stage is (TF + TT) / 16 row blocks of 2 KiB (16
+// rows x 128 k; the W blocks first, then the x blocks), copied from global
+// memory straight into an LDS ring of S stages, each copy instruction 8 whole
+// 128-byte lines; the rows' order and an XOR order of each row's 16-byte pieces
+// leave the operand reads free of bank conflicts.  A step of 64 k is IF x BJ
+// MFMAs per wave, with the operand reads of the next step and a share of a later
+// stage's copies between them.  The bytes moved, the LDS reads and the MFMA cycles
+// of a stage are those of a bf16 stage of 64 k, for twice the k.
+//
+// SwiGLU: the tile holds TF / 2 outputs, of a wave's IF row blocks the first half
+// gate rows and the others the same rows of up, so that g and u of an output
+// meet in one lane's registers.
+//
+// Rows past n or m repeat the last one; their outputs are not written.
+
+// Workgroup b runs on XCD b % 8 (dispatch is round-robin over the 8 XCDs): each
+// XCD takes one contiguous run of tiles.  The order: groups of 4 feature tiles,
+// walked token tile by token tile, so that the workgroups an XCD holds at a
+// time share their W and x rows in that XCD's L2.
+__device__ __forceinline__ bool tile_of(const Args &a, int &tf, int &tt) {
+    const int L = (blockIdx.x & 7) * a.per_xcd + (blockIdx.x >> 3);
+    if (L >= a.tiles) return false;
+    const int per_group = kGroupF * a.tiles_t;
+    const int g = L / per_group, r = L - g * per_group;
+    const int width = min(kGroupF, a.tiles_f - g * kGroupF);
+    tt = r / width;
+    tf = g * kGroupF + (r - tt * width);
+    return true;
+}
+
+// The schedule of a step, row by row: row i's BJ MFMAs, then its reads (W
+// fragment i and the x fragments the row loads).
+template <int IF, int BJ, int I> __device__ __forceinline__ void sched_rows() {
+    if constexpr (I < IF) {
+        __builtin_amdgcn_sched_group_barrier(0x008, BJ, 0);                                   // MFMA
+        __builtin_amdgcn_sched_group_barrier(0x100, 1 + (I + 1) * BJ / IF - I * BJ / IF, 0);  // DS read
+        sched_rows<IF, BJ, I + 1>();
     }
-    for (int k0 = 0; k0 < g.k; k0 += 64)
+}
+
+// One 64-k step of a wave: the MFMAs of the operands in (w, cx), row by row, with
+// the operand reads of the next step (LDS at nsb + noff) interleaved: W fragment
+// i of the next step replaces w[i] once row i's MFMAs have issued, the x
+// fragments go to nx.  after_row(i) runs after row i's reads.
+template <int IF, int BJ, typename F>
+__device__ __forceinline__ void substep(i32x4 (&w)[IF], const i32x4 (&cx)[BJ], const uint8_t *nsb, uint32_t noff,
+                                        int wf, int wt, i32x4 (&nx)[BJ], i32x4 (&acc)[IF][BJ], F &&after_row) {
 #pragma unroll
-        for (int i = 0; i < 2; i++)
+    for (int i = 0; i < IF; i++) {
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const i32x4 x = *(const i32x4 *)(g.x + xo[j] + k0);
-                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4 *)(g.w + wo[i] + k0), x, acc[i][j], 0, 0, 0);
-                if constexpr (OUT == kGlu)
-                    up[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4 *)(g.up + wo[i] + k0), x, up[i][j], 0, 0, 0);
+        for (int j = 0; j < BJ; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], cx[j], acc[i][j], 0, 0, 0);
+        w[i] = *(const i32x4 *)(nsb + noff + (IF * wf + i) * kPair);
+#pragma unroll
+        for (int j = i * BJ / IF; j < (i + 1) * BJ / IF; j++)
+            nx[j] = *(const i32x4 *)(nsb + noff + (2 * IF + BJ * wt + j) * kPair);
+        after_row(i);
+    }
+    sched_rows<IF, BJ, 0>();
+}
+
+// S stages in the ring; LGKM: a stage's slot is refilled at the barrier right
+// after its last operand reads (each wave first waits for its own reads), so
+// S - 1 stages are ahead of the one being read; else one barrier later, with
+// S - 2 ahead and no wait on the reads.
+template <int IF, int JT, int WT, int S, bool LGKM, int OUT>
+__global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
+    constexpr bool GLU = OUT == kGlu;
+    constexpr int TF = 32 * IF, TT = 32 * JT;
+    constexpr int NW = 2 * WT, NT = 64 * NW, BJ = TT / (16 * WT);  // waves, threads, token blocks per wave
+    constexpr int NBF = TF / 16, NB = (TF + TT) / 16;               // row blocks: W, all
+    constexpr int C = 2 * NB / NW;                                   // copy instructions per wave per stage
+    constexpr int kStageBytes = NB * kPair;
+    constexpr int AHEAD = LGKM ? S : S - 1;  // stages issued ahead of the one being read, plus one
+    constexpr int OF = GLU ? TF / 2 : TF;    // output features of the tile
+    constexpr int OI = GLU ? IF / 2 : IF;    // ... and their row blocks per wave
+    static_assert((2 * NB) % NW == 0 && BJ >= 1 && AHEAD >= 2 && C * (AHEAD - 1) <= 63, "tile shape");
+    static_assert(!GLU || IF % 2 == 0, "gate and up row blocks");
+    // after the loop: bf16 rows of the tile (16 bytes of padding a row), the scales
+    constexpr int RS = OF + 8, NS = TF + TT;
+    constexpr int kScaleAt = OUT == kBf16 || GLU ? TT * RS * 2 : 0;
+    constexpr int kLds = S * kStageBytes > kScaleAt + NS * 4 ? S * kStageBytes : kScaleAt + NS * 4;
+    static_assert(kScaleAt % 16 == 0 && kLds <= 160 * 1024, "LDS");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = lane >> 4, c = lane & 15;
+    const I8Gemm &g = a.g;
+    int tf, tt;
+    if (!tile_of(a, tf, tt)) return;
+    const int f0 = tf * OF, t0 = tt * TT, kt = g.k / kBK;
+
+    // The scales of the tile's features (gate, then up) and tokens, one or two a
+    // thread, loaded here and handed over through LDS once the ring is idle.
+    constexpr int PS = (NS + NT - 1) / NT;
+    float sc[PS];
+#pragma unroll
+    for (int p = 0; p < PS; p++) {
+        const int q = tid + NT * p;
+        if (q < OF) sc[p] = g.ws[min(f0 + q, g.n - 1)];
+        else if (GLU && q < TF) sc[p] = g.us[min(f0 + q - OF, g.n - 1)];
+        else sc[p] = g.xs[min(t0 + min(q - TF, TT - 1), g.m - 1)];
+    }
+
+    // Staging: wave w issues loads g = C w + [0, C) of a stage, load g the half
+    // h = g & 1 of row block gb = g >> 1.  The block's 16 slot groups of 128 bytes
+    // hold its rows in the order 0, 8, 1, 9, ..., 7, 15: group ga = 8 h + (l >> 3)
+    // holds row (ga >> 1) + 8 (ga & 1), lane l taking that row's 16-byte piece
+    // (l & 7) ^ (ga >> 1), so that row c (i = c >> 3, r = c & 7) keeps piece p in
+    // slot 16 r + 8 i + (p ^ r).
+    uint32_t voff[C];
+    const int8_t *sbase[C];
+    const int8_t *wt0 = g.w + (size_t)f0 * g.k, *ut0 = GLU ? g.up + (size_t)f0 * g.k : nullptr;
+    const int8_t *xt0 = g.x + (size_t)t0 * g.k;
+#pragma unroll
+    for (int j = 0; j < C; j++) {
+        const int l = wave * C + j, gb = l >> 1, h = l & 1;
+        const int ga = 8 * h + (lane >> 3);
+        const int rl = (ga >> 1) + 8 * (ga & 1);
+        const int piece = (lane & 7) ^ (ga >> 1);
+        const bool isw = gb < NBF;
+        // a wave's blocks: gate and up of the same OI output blocks
+        const int i = gb % IF, ob = GLU ? gb / IF * OI + i % OI : gb;
+        const int row = isw ? min(16 * ob + rl, g.n - 1 - f0) : min(16 * (gb - NBF) + rl, g.m - 1 - t0);
+        voff[j] = (uint32_t)row * (uint32_t)g.k + 16 * piece;
+        sbase[j] = !isw ? xt0 : GLU && i >= OI ? ut0 : wt0;
+    }
+    const uint32_t lds0 = lds_addr(lds) + wave * C * kFrag;
+    // copy j of stage t into its ring slot t % S.  Stages past the last copy the
+    // last stage's rows again: their slots are never read, every iteration issues
+    // C copies, and the waits and the loop have no branch.
+    auto copy = [&](int t, int j) __attribute__((always_inline)) {
+        lds_dma16_sv(sbase[j] + min(t, kt - 1) * kBK, voff[j], lds0 + (t % S) * kStageBytes + j * kFrag);
+    };
+    // A stage's copies are spread over the MFMA rows of two steps: [0, CB) in
+    // the step after the barrier that frees its slot, [CB, C) in the next one
+    // (all in the first with two stages ahead, where the next wait lands them).
+    constexpr int CB = AHEAD > 2 ? (C + 1) / 2 : C;
+    auto first_half = [&](int t) __attribute__((always_inline)) {
+        return [&, t](int i) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = i * CB / IF; j < (i + 1) * CB / IF; j++) copy(t, j);
+        };
+    };
+    auto second_half = [&](int t) __attribute__((always_inline)) {
+        return [&, t](int i) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = CB + i * (C - CB) / IF; j < CB + (i + 1) * (C - CB) / IF; j++) copy(t, j);
+        };
+    };
+    // Operand reads: lane (grp, c) takes row c, k 16 grp + [0, 16) of step ks,
+    // i.e. piece 4 ks + grp, at byte off[ks] of each row block.
+    uint32_t off[2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) {
+        const int i = c >> 3, r = c & 7;
+        off[ks] = 16 * (16 * r + 8 * i + ((4 * ks + grp) ^ r));
+    }
+
+    const int wf = wave & 1, wt = wave >> 1;
+    i32x4 acc[IF][BJ];
+#pragma unroll
+    for (int i = 0; i < IF; i++)
+#pragma unroll
+        for (int j = 0; j < BJ; j++) acc[i][j] = i32x4{0, 0, 0, 0};
+
+    // A wave's copies (C a stage) retire in order, so a wait for at most C n
+    // outstanding copies lands all but the last n stages issued.
+#pragma unroll
+    for (int t = 0; t < AHEAD - 1; t++)
+#pragma unroll
+        for (int j = 0; j < C; j++) copy(t, j);
+#pragma unroll
+    for (int j = 0; j < CB; j++) copy(AHEAD - 1, j);
+    wait_vm<C * (AHEAD - 2) + CB>();
+    asm volatile("s_barrier" ::: "memory");
+    i32x4 w[IF], ax[BJ], bx[BJ];
+#pragma unroll
+    for (int i = 0; i < IF; i++) w[i] = *(const i32x4 *)(lds + off[0] + (IF * wf + i) * kPair);
+#pragma unroll
+    for (int j = 0; j < BJ; j++) ax[j] = *(const i32x4 *)(lds + off[0] + (NBF + BJ * wt + j) * kPair);
+
+    // The last stage is peeled, so that the accumulators meet no branch.
+    for (int s = 0; s < kt - 1; s++) {
+        // step (s, 0): its operands in (w, ax); read step (s, 1) into (w, bx);
+        // the second half of stage s - 1 + AHEAD
+        substep<IF, BJ>(w, ax, lds + (s % S) * kStageBytes, off[1], wf, wt, bx, acc, second_half(s - 1 + AHEAD));
+        // stage s + 1 landed: AHEAD - 2 later ones may stay in flight
+        wait_vm<C * (AHEAD - 2), LGKM>();
+        asm volatile("s_barrier" ::: "memory");
+        // step (s, 1): operands in (w, bx); read step (s + 1, 0) into (w, ax);
+        // the first half of stage s + AHEAD
+        substep<IF, BJ>(w, bx, lds + ((s + 1) % S) * kStageBytes, off[0], wf, wt, ax, acc, first_half(s + AHEAD));
+    }
+    substep<IF, BJ>(w, ax, lds + ((kt - 1) % S) * kStageBytes, off[1], wf, wt, bx, acc, [](int) {});
+#pragma unroll
+    for (int i = 0; i < IF; i++)
+#pragma unroll
+        for (int j = 0; j < BJ; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], bx[j], acc[i][j], 0, 0, 0);
+    wait_vm<0>();     // the copies past the last stage have landed before the ring is reused or freed
+    __syncthreads();  // every wave's operand reads are done
+
+    float *scales = (float *)(lds + kScaleAt);
+#pragma unroll
+    for (int p = 0; p < PS; p++)
+        if (tid + NT * p < NS) scales[tid + NT * p] = sc[p];
+    __syncthreads();
+
+    if constexpr (OUT == kBf16 || GLU) {
+        // restaged through the (idle) ring as [token][feature] rows, then
+        // written as whole 128-byte lines, 16 bytes a lane
+        uint16_t *st = (uint16_t *)lds;
+#pragma unroll
+        for (int j = 0; j < BJ; j++) {
+            const int tl = (TT / WT) * wt + 16 * j + c;
+            const float xs = scales[TF + tl];
+#pragma unroll
+            for (int i = 0; i < OI; i++) {
+                const int fl = (OF / 2) * wf + 16 * i + 4 * grp;
+                const float4 ws = *(const float4 *)(scales + fl);
+                const i32x4 v = acc[i][j];
+                float o[4];
+                if constexpr (GLU) {
+                    const float4 us = *(const float4 *)(scales + OF + fl);
+                    const i32x4 u = acc[i + OI][j];
+                    o[0] = glu(v[0], u[0], ws.x, us.x, xs);
+                    o[1] = glu(v[1], u[1], ws.y, us.y, xs);
+                    o[2] = glu(v[2], u[2], ws.z, us.z, xs);
+                    o[3] = glu(v[3], u[3], ws.w, us.w, xs);
+                } else {
+                    o[0] = scaled(v[0], ws.x) * xs;
+                    o[1] = scaled(v[1], ws.y) * xs;
+                    o[2] = scaled(v[2], ws.z) * xs;
+                    o[3] = scaled(v[3], ws.w) * xs;
+                }
+                *(uint2 *)(st + tl * RS + fl) = make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
             }
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const int t = t0 + 16 * j + c;
-            if (t < g.m) store4<OUT>(g, t, f0 + 16 * i + 4 * grp, acc[i][j], up[i][j]);
         }
+        __syncthreads();
+        constexpr int CPR = OF / 8;  // 16-byte chunks of a token row
+        static_assert((TT * CPR) % NT == 0, "restage");
+#pragma unroll
+        for (int n = 0; n < TT * CPR / NT; n++) {
+            const int q = n * NT + tid, row = q / CPR, col = q - row * CPR;
+            const int t = t0 + row, f = f0 + 8 * col;
+            if (t >= g.m || f >= g.n) continue;
+            uint16_t *y = (uint16_t *)g.y + (size_t)t * g.ldy + f;
+            const uint16_t *s = st + row * RS + 8 * col;
+            if (a.vec && f + 8 <= g.n) {
+                *(uint4 *)y = *(const uint4 *)s;
+            } else {
+                for (int e = 0; e < min(8, g.n - f); e++) y[e] = s[e];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < BJ; j++) {
+            const int tl = (TT / WT) * wt + 16 * j + c;
+            if (t0 + tl >= g.m) continue;
+            const float xs = scales[TF + tl];
+#pragma unroll
+            for (int i = 0; i < IF; i++) {
+                const int fl = (TF / 2) * wf + 16 * i + 4 * grp;
+                const float4 w4 = *(const float4 *)(scales + fl);
+                const float ws[4] = {w4.x, w4.y, w4.z, w4.w};
+                store4<OUT>(a, t0 + tl, f0 + fl, acc[i][j], acc[i][j], ws, ws, xs);
+            }
+        }
+    }
+}
+
+// ---- few tokens ----------------------------------------------------------------
+//
+// A workgroup owns 16 A features x 16 B tokens and its four waves split k: each
+// streams its own quarter of the tile's W and x rows through an LDS ring of its
+// own, so there is no barrier before the end and four load streams run per
+// workgroup.  The four partial tiles meet in LDS.  SwiGLU: the first A / 2 row
+// blocks are gate rows, the others the same rows of up.
+template <int A, int B, int S, int OUT>
+__global__ __launch_bounds__(256) void skinny_kernel(Args a) {
+    constexpr bool GLU = OUT == kGlu;
+    constexpr int C = 2 * (A + B);  // copies (1 KiB each) of a stage
+    constexpr int kStage = C * 1024, kRing = S * kStage;
+    constexpr int AO = GLU ? A / 2 : A;                         // output row blocks
+    constexpr int Q = AO * B * 64, NQ = (Q + 255) / 256;        // 4-feature outputs, per thread
+    static_assert(4 * kRing <= 160 * 1024 && C * (S - 1) <= 63, "ring");
+    static_assert(A * B * 1024 <= kRing, "a wave's partial tile is handed over in its ring");
+    static_assert(!GLU || A % 2 == 0, "gate and up row blocks");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kRing];
+    const I8Gemm &g = a.g;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = lane >> 4, c = lane & 15;
+    // each XCD takes a contiguous run of tiles, the token tiles of one W slab
+    // next to each other: a slab is read from HBM into one L2
+    const int L = (blockIdx.x & 7) * a.per_xcd + (blockIdx.x >> 3);
+    if (L >= a.tiles) return;
+    const int tf = L / a.tiles_t, tt = L - tf * a.tiles_t;
+    const int f0 = tf * 16 * AO, t0 = tt * 16 * B;
+
+    uint32_t voff[C];
+#pragma unroll
+    for (int l = 0; l < C; l++) {
+        const int gb = l >> 1, ga = 8 * (l & 1) + (lane >> 3);
+        const int rl = (ga >> 1) + 8 * (ga & 1), piece = (lane & 7) ^ (ga >> 1);
+        const int row = gb < A ? min(16 * (GLU && gb >= AO ? gb - AO : gb) + rl, g.n - 1 - f0)
+                               : min(16 * (gb - A) + rl, g.m - 1 - t0);
+        voff[l] = (uint32_t)row * (uint32_t)g.k + 16 * piece;
+    }
+    // this wave's stages: a quarter of them, one more or less
+    const int kt = g.k / kBK, s0 = kt * wave / 4, n = kt * (wave + 1) / 4 - s0;
+    const int8_t *wb = g.w + (size_t)f0 * g.k + s0 * kBK;
+    const int8_t *ub = GLU ? g.up + (size_t)f0 * g.k + s0 * kBK : nullptr;
+    const int8_t *xb = g.x + (size_t)t0 * g.k + s0 * kBK;
+    const uint32_t ring = lds_addr(lds) + wave * kRing;
+    auto copy = [&](int t, int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int l = 0; l < C; l++) {
+            const int gb = l >> 1;
+            lds_dma16_sv((gb >= A ? xb : GLU && gb >= AO ? ub : wb) + t * kBK, voff[l], ring + slot * kStage + l * 1024);
+        }
+    };
+    uint32_t off[2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) off[ks] = 16 * (16 * (c & 7) + 8 * (c >> 3) + ((4 * ks + grp) ^ (c & 7)));
+
+    i32x4 acc[A][B];
+#pragma unroll
+    for (int i = 0; i < A; i++)
+#pragma unroll
+        for (int j = 0; j < B; j++) acc[i][j] = i32x4{0, 0, 0, 0};
+    const uint8_t *my = lds + wave * kRing;
+    i32x4 w[2][A], x[2][B];
+    int slot = 0;
+    auto read = [&]() __attribute__((always_inline)) {
+        const uint8_t *p = my + slot * kStage;
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+#pragma unroll
+            for (int i = 0; i < A; i++) w[ks][i] = *(const i32x4 *)(p + off[ks] + i * kPair);
+#pragma unroll
+            for (int j = 0; j < B; j++) x[ks][j] = *(const i32x4 *)(p + off[ks] + (A + j) * kPair);
+        }
+    };
+    auto mma = [&]() __attribute__((always_inline)) {
+        slot = slot + 1 == S ? 0 : slot + 1;
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+            for (int i = 0; i < A; i++)
+#pragma unroll
+                for (int j = 0; j < B; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[ks][i], x[ks][j], acc[i][j], 0, 0, 0);
+    };
+    // A wave's copies retire in order: a stage has landed once at most S - 1
+    // younger stages are outstanding.  Its slot is refilled as soon as this wave
+    // has its operands in registers; no other wave touches the ring.
+#pragma unroll
+    for (int t = 0; t < S; t++)
+        if (t < n) copy(t, t);
+    for (int t = S; t < n; t++) {
+        wait_vm<(S - 1) * C>();
+        read();
+        wait_lgkm();
+        copy(t, slot);
+        mma();
+    }
+    // the last S stages (or all, where there are fewer), nothing left to issue
+    const int left = min(S, n);
+#pragma unroll
+    for (int l = S; l > 0; l--)
+        if (l <= left) {
+            if (l == 4) wait_vm<(S > 3 ? 3 : 0) * C>();
+            else if (l == 3) wait_vm<(S > 2 ? 2 : 0) * C>();
+            else if (l == 2) wait_vm<(S > 1 ? 1 : 0) * C>();
+            else wait_vm<0>();
+            read();
+            mma();
+        }
+    wait_lgkm();
+
+#pragma unroll
+    for (int i = 0; i < A; i++)
+#pragma unroll
+        for (int j = 0; j < B; j++) *(i32x4 *)(lds + wave * kRing + (64 * (i * B + j) + lane) * 16) = acc[i][j];
+    __syncthreads();
+    auto sum = [&](int q) __attribute__((always_inline)) {
+        i32x4 s = *(const i32x4 *)(lds + q * 16);
+#pragma unroll
+        for (int p = 1; p < 4; p++) s += *(const i32x4 *)(lds + p * kRing + q * 16);
+        return s;
+    };
+#pragma unroll
+    for (int u = 0; u < NQ; u++) {
+        const int q = tid + 256 * u, fr = q >> 6, i = fr / B, j = fr - i * B;
+        const int f = f0 + 16 * i + 4 * grp, t = t0 + 16 * j + c;
+        if (q >= Q || t >= g.m || f >= g.n) continue;
+        float ws[4], us[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            ws[e] = g.ws[min(f + e, g.n - 1)];
+            us[e] = GLU ? g.us[min(f + e, g.n - 1)] : 0.f;
+        }
+        const i32x4 s = sum(q);
+        store4<OUT>(a, t, f, s, GLU ? sum(q + Q) : s, ws, us, g.xs[t]);
+    }
+}
+
+// ---- which kernel --------------------------------------------------------------
+
+// The tiles: features x tokens (SwiGLU: half as many outputs), the first kSkinny
+// of them the few-token kernel's.
+struct Shape {
+    const char *name;
+    int f, t;
+};
+constexpr Shape kShapes[] = {{"16x16", 16, 16},   {"32x16", 32, 16},   {"32x32", 32, 32},   {"32x64", 32, 64},
+                             {"64x64", 64, 64},   {"96x64", 96, 64},   {"128x64", 128, 64}, {"128x96", 128, 96},
+                             {"128x128", 128, 128}, {"192x128", 192, 128}, {"256x128", 256, 128}, {"128x256", 128, 256},
+                             {"192x256", 192, 256}, {"256x256", 256, 256}};
+constexpr int kNumShapes = sizeof(kShapes) / sizeof(kShapes[0]), kSkinny = 6;
+
+template <int OUT> int plan(const I8Gemm &g) {
+    constexpr int first = OUT == kGlu ? 1 : 0;  // gate and up: two row blocks at least
+    if (const char *e = std::getenv("HYMT_HIP_I8_TILE"))
+        for (int i = first; i < kNumShapes; i++)
+            if (!std::strcmp(e, kShapes[i].name)) return i;
+    const long n = (long)g.n * (OUT == kGlu ? 2 : 1);
+    auto tiles = [&](int i) { return (n + kShapes[i].f - 1) / kShapes[i].f * ((g.m + kShapes[i].t - 1) / kShapes[i].t); };
+    for (int i = first; i < kSkinny; i++)
+        if (tiles(i) <= 256) return i;
+    int best = kSkinny;
+    double fill = 0;
+    for (int i = kSkinny; i < kNumShapes; i++) {
+        const long w = tiles(i);
+        const double f = (double)w / (256.0 * ((w + 255) / 256)) * (0.9 + 0.01 * i);
+        if (f > fill) {
+            fill = f;
+            best = i;
+        }
+    }
+    return best;
+}
+
+template <int OUT>
+void launch_shape(int i, const Args &a, const KernelSpan &span, hipStream_t s) {
+    const dim3 grid(8 * a.per_xcd);
+    switch (i) {
+    case 0:
+        if constexpr (OUT != kGlu) launch(span, skinny_kernel<1, 1, 4, OUT>, grid, dim3(256), 0, s, a);
+        break;
+    case 1: launch(span, skinny_kernel<2, 1, 3, OUT>, grid, dim3(256), 0, s, a); break;
+    case 2: launch(span, skinny_kernel<2, 2, 2, OUT>, grid, dim3(256), 0, s, a); break;
+    case 3: launch(span, skinny_kernel<2, 4, 2, OUT>, grid, dim3(256), 0, s, a); break;
+    case 4: launch(span, skinny_kernel<4, 4, 2, OUT>, grid, dim3(256), 0, s, a); break;
+    case 5: launch(span, skinny_kernel<6, 4, 2, OUT>, grid, dim3(256), 0, s, a); break;
+    case 6: launch(span, tile_kernel<4, 2, 2, 4, false, OUT>, grid, dim3(256), 0, s, a); break;
+    case 7: launch(span, tile_kernel<4, 3, 2, 4, false, OUT>, grid, dim3(256), 0, s, a); break;
+    case 8: launch(span, tile_kernel<4, 4, 2, 4, false, OUT>, grid, dim3(256), 0, s, a); break;
+    case 9: launch(span, tile_kernel<6, 4, 4, 4, true, OUT>, grid, dim3(512), 0, s, a); break;
+    case 10: launch(span, tile_kernel<8, 4, 2, 3, true, OUT>, grid, dim3(256), 0, s, a); break;
+    case 11: launch(span, tile_kernel<4, 8, 2, 3, true, OUT>, grid, dim3(256), 0, s, a); break;
+    case 12: launch(span, tile_kernel<6, 8, 4, 2, true, OUT>, grid, dim3(512), 0, s, a); break;
+    default: launch(span, tile_kernel<8, 8, 4, 2, true, OUT>, grid, dim3(512), 0, s, a); break;
+    }
 }
 
 bool fits(const I8Gemm &g) {
     auto a16 = [](const void *p) { return ((uintptr_t)p & 15u) == 0; };
-    return g.n > 0 && g.m >= 0 && g.k >= 2 * kI8StepK && g.k <= kI8MaxK && g.k % kI8StepK == 0 && g.ldy >= g.n &&
-           a16(g.w) && a16(g.x) && a16(g.up);
+    return g.n > 0 && g.m >= 0 && g.n <= kI8MaxRows && g.m <= kI8MaxRows && g.k >= 2 * kI8StepK && g.k <= kI8MaxK &&
+           g.k % kI8StepK == 0 && g.ldy >= g.n && a16(g.w) && a16(g.x) && a16(g.up);
 }
 
 template <int OUT>
 hipError_t run(const I8Gemm &g, const char *name, hipStream_t s) {
     if (!fits(g)) return hipErrorInvalidValue;
     if (g.m == 0) return hipSuccess;
-    const size_t grid = (size_t)((g.n + 63) / 64) * ((g.m + 63) / 64);
-    if (grid > 0x7fffffffu) return hipErrorInvalidValue;
+    const int i = plan<OUT>(g);
+    const int of = OUT == kGlu ? kShapes[i].f / 2 : kShapes[i].f;
+    Args a{};
+    a.g = g;
+    a.tiles_f = (g.n + of - 1) / of;
+    a.tiles_t = (g.m + kShapes[i].t - 1) / kShapes[i].t;
+    const size_t tiles = (size_t)a.tiles_f * a.tiles_t;
+    if (tiles > 0x7ffffff0u) return hipErrorInvalidValue;
+    a.tiles = (int)tiles;
+    a.per_xcd = (int)((tiles + 7) / 8);
+    constexpr int es = OUT == kBf16 || OUT == kGlu ? 2 : 4;
+    a.vec = ((uintptr_t)g.y & 15u) == 0 && g.ldy % (16 / es) == 0;
     KernelSpan span(name, s, true);
-    launch(span, simple_kernel<OUT>, dim3((unsigned)grid), dim3(256), 0, s, g);
+    launch_shape<OUT>(i, a, span, s);
     return hipGetLastError();
 }
 

@@ -1383,6 +1383,7 @@ int check_i8_gemm(const I8Gemm &g, size_t y_bytes) {
     if (g.n < 1 || g.ldy < g.n) return fail(HYMT_E_ARG, "n must be positive and the output's rows at least n apart");
     if (g.k % kI8StepK || g.k < 2 * kI8StepK || g.k > kI8MaxK)
         return fail(HYMT_E_UNSUPPORTED, "k must be a multiple of 128, 256 to 65536");
+    if (g.m > kI8MaxRows || g.n > kI8MaxRows) return fail(HYMT_E_UNSUPPORTED, "more than 2^30 tokens or channels");
     if (misaligned(g.w, 16) || misaligned(g.up, 16) || misaligned(g.x, 16))
         return fail(HYMT_E_ARG, "codes must be 16-byte aligned");
     if (misaligned(g.ws, 4) || misaligned(g.us, 4) || misaligned(g.xs, 4) || misaligned(g.y, y_bytes))

@@ -13,6 +13,7 @@ namespace hymt {
 // The largest row of codes that a product sums: 128 * 128 * 65536 = 2^30 fits
 // an int32 with room.
 constexpr int kI8MaxK = 65536;
+constexpr int kI8MaxRows = 1 << 30;  // of tokens and of channels: indexes a tile past the end fit an int
 constexpr int kI8StepK = 128;  // k is a multiple of this, two of them at least
 
 // out[r] = rint(127 v / max|v|) (ties to even) and scale[r] = max|v| / 127 of

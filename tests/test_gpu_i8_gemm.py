@@ -204,3 +204,24 @@ def test_offsets_past_32_bits(be):
         be.free(dx)
         be.free(dy)
         r.close()
+
+
+TILES = ["16x16", "32x16", "32x32", "32x64", "64x64", "96x64", "128x64", "128x96", "128x128", "192x128", "256x128",
+         "128x256", "192x256", "256x256"]
+
+
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("m,n,k", [(1, 1, 256), (2, 190, 384), (31, 257, 640), (130, 100, 1152), (300, 520, 2048)])
+def test_every_tile(be, monkeypatch, tile, m, n, k):
+    """Each tile on shapes that end inside it in every direction, from the
+    shortest k on, for every output."""
+    w, x, up = codes(1, n, k), codes(2, m, k), codes(3, n, k)
+    ws, us, xs = scales(4, n), scales(5, n), scales(6, m, 1e-3, 1e-1)
+    y0 = np.random.default_rng(7).standard_normal((m, n)).astype(np.float32)
+    y = product(w, ws, x, xs)
+    monkeypatch.setenv("HYMT_HIP_I8_TILE", tile)
+    for ldy in (n, n + 3, (n + 15) // 8 * 8):
+        check(run(be, w, ws, x, xs, "f32", ldy), y, "f32")
+        check(run(be, w, ws, x, xs, "acc", ldy, y0=y0), y, "acc", y0)
+        check(run(be, w, ws, x, xs, "bf16", ldy), y, "bf16")
+        check_glu(run(be, w, ws, x, xs, "glu", ldy, up=up, us=us), w, ws, up, us, x, xs)
