@@ -11,6 +11,7 @@
 #include <cstdint>
 #include <cstdlib>
 #include <cstring>
+#include <type_traits>
 
 #include "device_common.hpp"
 #include "int8.hpp"
@@ -505,6 +506,63 @@ __global__ __launch_bounds__(256) void skinny_kernel(Args a) {
     }
 }
 
+// ---- up to 16 tokens -------------------------------------------------------------
+//
+// A stream of W: a workgroup takes 16 channels (SwiGLU: 16 gate and their 16 up
+// rows), its four waves a quarter of k each, straight from memory into the
+// operand registers, 4 stages (8 KiB of W a wave) at a time with no ring and no
+// LDS before the end, so that many workgroups share a CU and keep loads in
+// flight for each other.
+template <int OUT>
+__global__ __launch_bounds__(256) void gemv_kernel(Args a) {
+    constexpr bool GLU = OUT == kGlu;
+    constexpr int A = GLU ? 2 : 1, U = GLU ? 2 : 4;  // row blocks; stages at a time
+    __shared__ __attribute__((aligned(16))) i32x4 part[4][A][64];
+    const I8Gemm &g = a.g;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = lane >> 4, c = lane & 15;
+    const int f0 = 16 * blockIdx.x;
+    const int kt = g.k / kBK, s0 = kt * wave / 4, s1 = kt * (wave + 1) / 4;
+    const size_t wo = (size_t)min(f0 + c, g.n - 1) * g.k + 16 * grp;
+    const int8_t *wp[2] = {g.w + wo, GLU ? g.up + wo : nullptr};
+    const int8_t *xp = g.x + (size_t)min(c, g.m - 1) * g.k + 16 * grp;
+    i32x4 acc[A] = {};
+    auto stages = [&](int s, auto count) __attribute__((always_inline)) {
+        constexpr int N = 2 * decltype(count)::value;
+        i32x4 w[A][N], x[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+#pragma unroll
+            for (int i = 0; i < A; i++) w[i][j] = *(const i32x4 *)(wp[i] + s * kBK + 64 * j);
+            x[j] = *(const i32x4 *)(xp + s * kBK + 64 * j);
+        }
+#pragma unroll
+        for (int j = 0; j < N; j++)
+#pragma unroll
+            for (int i = 0; i < A; i++) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i][j], x[j], acc[i], 0, 0, 0);
+    };
+    int s = s0;
+    for (; s + U <= s1; s += U) stages(s, std::integral_constant<int, U>{});
+    for (; s < s1; s++) stages(s, std::integral_constant<int, 1>{});
+#pragma unroll
+    for (int i = 0; i < A; i++) part[wave][i][lane] = acc[i];
+    __syncthreads();
+    const int f = f0 + 4 * grp;
+    if (tid >= 64 || c >= g.m || f >= g.n) return;
+    auto sum = [&](int i) __attribute__((always_inline)) {
+        return (part[0][i][lane] + part[1][i][lane]) + (part[2][i][lane] + part[3][i][lane]);
+    };
+    float ws[4], us[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        ws[e] = g.ws[min(f + e, g.n - 1)];
+        us[e] = GLU ? g.us[min(f + e, g.n - 1)] : 0.f;
+    }
+    const i32x4 v = sum(0);
+    store4<OUT>(a, c, f, v, GLU ? sum(A - 1) : v, ws, us, g.xs[c]);
+}
+
 // ---- which kernel --------------------------------------------------------------
 
 // The tiles: features x tokens (SwiGLU: half as many outputs), the first kSkinny
@@ -513,17 +571,18 @@ struct Shape {
     const char *name;
     int f, t;
 };
-constexpr Shape kShapes[] = {{"16x16", 16, 16},   {"32x16", 32, 16},   {"32x32", 32, 32},   {"32x64", 32, 64},
+constexpr Shape kShapes[] = {{"stream", 16, 16}, {"16x16", 16, 16},   {"32x16", 32, 16},   {"32x32", 32, 32},   {"32x64", 32, 64},
                              {"64x64", 64, 64},   {"96x64", 96, 64},   {"128x64", 128, 64}, {"128x96", 128, 96},
                              {"128x128", 128, 128}, {"192x128", 192, 128}, {"256x128", 256, 128}, {"128x256", 128, 256},
                              {"192x256", 192, 256}, {"256x256", 256, 256}};
-constexpr int kNumShapes = sizeof(kShapes) / sizeof(kShapes[0]), kSkinny = 6;
+constexpr int kNumShapes = sizeof(kShapes) / sizeof(kShapes[0]), kSkinny = 7;
 
 template <int OUT> int plan(const I8Gemm &g) {
-    constexpr int first = OUT == kGlu ? 1 : 0;  // gate and up: two row blocks at least
+    constexpr int first = OUT == kGlu ? 2 : 1;  // gate and up: two row blocks at least
     if (const char *e = std::getenv("HYMT_HIP_I8_TILE"))
         for (int i = first; i < kNumShapes; i++)
             if (!std::strcmp(e, kShapes[i].name)) return i;
+    if (std::getenv("HYMT_STREAM") && g.m <= 16) return 0;
     const long n = (long)g.n * (OUT == kGlu ? 2 : 1);
     auto tiles = [&](int i) { return (n + kShapes[i].f - 1) / kShapes[i].f * ((g.m + kShapes[i].t - 1) / kShapes[i].t); };
     for (int i = first; i < kSkinny; i++)
@@ -545,21 +604,22 @@ template <int OUT>
 void launch_shape(int i, const Args &a, const KernelSpan &span, hipStream_t s) {
     const dim3 grid(8 * a.per_xcd);
     switch (i) {
-    case 0:
+    case 0: launch(span, gemv_kernel<OUT>, dim3(a.tiles_f), dim3(256), 0, s, a); break;
+    case 1:
         if constexpr (OUT != kGlu) launch(span, skinny_kernel<1, 1, 4, OUT>, grid, dim3(256), 0, s, a);
         break;
-    case 1: launch(span, skinny_kernel<2, 1, 3, OUT>, grid, dim3(256), 0, s, a); break;
-    case 2: launch(span, skinny_kernel<2, 2, 2, OUT>, grid, dim3(256), 0, s, a); break;
-    case 3: launch(span, skinny_kernel<2, 4, 2, OUT>, grid, dim3(256), 0, s, a); break;
-    case 4: launch(span, skinny_kernel<4, 4, 2, OUT>, grid, dim3(256), 0, s, a); break;
-    case 5: launch(span, skinny_kernel<6, 4, 2, OUT>, grid, dim3(256), 0, s, a); break;
-    case 6: launch(span, tile_kernel<4, 2, 2, 4, false, OUT>, grid, dim3(256), 0, s, a); break;
-    case 7: launch(span, tile_kernel<4, 3, 2, 4, false, OUT>, grid, dim3(256), 0, s, a); break;
-    case 8: launch(span, tile_kernel<4, 4, 2, 4, false, OUT>, grid, dim3(256), 0, s, a); break;
-    case 9: launch(span, tile_kernel<6, 4, 4, 4, true, OUT>, grid, dim3(512), 0, s, a); break;
-    case 10: launch(span, tile_kernel<8, 4, 2, 3, true, OUT>, grid, dim3(256), 0, s, a); break;
-    case 11: launch(span, tile_kernel<4, 8, 2, 3, true, OUT>, grid, dim3(256), 0, s, a); break;
-    case 12: launch(span, tile_kernel<6, 8, 4, 2, true, OUT>, grid, dim3(512), 0, s, a); break;
+    case 2: launch(span, skinny_kernel<2, 1, 3, OUT>, grid, dim3(256), 0, s, a); break;
+    case 3: launch(span, skinny_kernel<2, 2, 2, OUT>, grid, dim3(256), 0, s, a); break;
+    case 4: launch(span, skinny_kernel<2, 4, 2, OUT>, grid, dim3(256), 0, s, a); break;
+    case 5: launch(span, skinny_kernel<4, 4, 2, OUT>, grid, dim3(256), 0, s, a); break;
+    case 6: launch(span, skinny_kernel<6, 4, 2, OUT>, grid, dim3(256), 0, s, a); break;
+    case 7: launch(span, tile_kernel<4, 2, 2, 4, false, OUT>, grid, dim3(256), 0, s, a); break;
+    case 8: launch(span, tile_kernel<4, 3, 2, 4, false, OUT>, grid, dim3(256), 0, s, a); break;
+    case 9: launch(span, tile_kernel<4, 4, 2, 4, false, OUT>, grid, dim3(256), 0, s, a); break;
+    case 10: launch(span, tile_kernel<6, 4, 4, 4, true, OUT>, grid, dim3(512), 0, s, a); break;
+    case 11: launch(span, tile_kernel<8, 4, 2, 3, true, OUT>, grid, dim3(256), 0, s, a); break;
+    case 12: launch(span, tile_kernel<4, 8, 2, 3, true, OUT>, grid, dim3(256), 0, s, a); break;
+    case 13: launch(span, tile_kernel<6, 8, 4, 2, true, OUT>, grid, dim3(512), 0, s, a); break;
     default: launch(span, tile_kernel<8, 8, 4, 2, true, OUT>, grid, dim3(512), 0, s, a); break;
     }
 }
@@ -575,7 +635,7 @@ hipError_t run(const I8Gemm &g, const char *name, hipStream_t s) {
     if (!fits(g)) return hipErrorInvalidValue;
     if (g.m == 0) return hipSuccess;
     const int i = plan<OUT>(g);
-    const int of = OUT == kGlu ? kShapes[i].f / 2 : kShapes[i].f;
+    const int of = OUT == kGlu && i > 0 ? kShapes[i].f / 2 : kShapes[i].f;
     Args a{};
     a.g = g;
     a.tiles_f = (g.n + of - 1) / of;

@@ -6,12 +6,18 @@
 // v and a, so q = rint(127 x w / max|x w|) needs no statistics, and only the
 // scale has the root: a / (127 sqrt(mean(x^2) + eps)).
 //
-// The codes are those of exact arithmetic: x w is formed in fp64 (exact: 48
-// bits) and so are the maximum and the quotient.  In fp32 a value within a few
+// The codes are those of exact arithmetic; in fp32 alone a value within a few
 // ulps of a border would take the one code or the other by the order of the
-// roundings.  A quotient is a product with 127 / a, and only where that lands
-// within 1e-9 of a border (ties of bf16 rows: a half of the maximum is 63.5) a
-// division.
+// roundings.  a is exact: fp32 for plain rows, the fp64 product (48 bits) for x w.
+// A code is first rounded from the fp32 product with fp32(127 / a), which is off
+// by at most 127 (2^-24 + 2^-24 + 2^-24) < 2.4e-5 (the reciprocal's rounding, x w's, and as
+// much for values that x w flushes); where that lands within 6e-5 of a border,
+// one value in ten thousand, the code is taken from the fp64 quotient.  Rows
+// whose maximum is outside [2^-90, 2^100], where fp32 could flush or overflow, take
+// the quotient throughout.  (All in fp64, 2048 x 6144 bf16 rows took 15.0 us.)
+//
+// HBM-bound: each value is read once, held in registers between the passes, and
+// its code written once.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -35,77 +41,124 @@ struct RowsArgs {
     float *scale;
 };
 
-__device__ __forceinline__ int code_of(double v, double a, double r) {
-    const double s = v * r;
-    double q = rint(s);
-    if (fabs(fabs(s - q) - 0.5) < 1e-9) q = rint(v * 127.0 / a);
-    return (int)q;
+constexpr float kMagic = 12582912.f;  // 1.5 2^23: an addition rounds to whole numbers, in the low bits
+constexpr float kNear = 0.5f - 6e-5f;
+
+// The maximum and the sum over a wave, in every lane: rows of 16 lanes by DPP
+// (quad_perm xor 1, xor 2, half-row and row mirrors), the four rows from lanes 0,
+// 16, 32 and 48.
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));
+}
+template <int CTRL> __device__ __forceinline__ double dpp(double v) {
+    const int2 b = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_update_dpp(0, b.x, CTRL, 0xF, 0xF, false),
+                                                __builtin_amdgcn_update_dpp(0, b.y, CTRL, 0xF, 0xF, false)));
+}
+__device__ __forceinline__ float lane_of(float v, int l) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l));
+}
+__device__ __forceinline__ double lane_of(double v, int l) {
+    const int2 b = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_readlane(b.x, l), __builtin_amdgcn_readlane(b.y, l)));
+}
+template <typename T, typename F> __device__ __forceinline__ T wave_reduce(T v, F f) {
+    v = f(v, dpp<0xB1>(v));
+    v = f(v, dpp<0x4E>(v));
+    v = f(v, dpp<0x141>(v));
+    v = f(v, dpp<0x140>(v));
+    return f(f(lane_of(v, 0), lane_of(v, 16)), f(lane_of(v, 32), lane_of(v, 48)));
 }
 
-__device__ __forceinline__ float4 load4_bf16(const uint16_t *p) {
-    const uint2 b = *(const uint2 *)p;
-    return make_float4(bf16_to_f32(b.x & 0xFFFF), bf16_to_f32(b.x >> 16), bf16_to_f32(b.y & 0xFFFF),
-                       bf16_to_f32(b.y >> 16));
+// V values of a row from element e on
+template <int V> struct Vals {
+    float v[V];
+};
+template <int V> __device__ __forceinline__ Vals<V> load_f32(const float *p) {
+    Vals<V> r;
+#pragma unroll
+    for (int q = 0; q < V / 4; q++) {
+        const float4 f = ((const float4 *)p)[q];
+        r.v[4 * q] = f.x, r.v[4 * q + 1] = f.y, r.v[4 * q + 2] = f.z, r.v[4 * q + 3] = f.w;
+    }
+    return r;
+}
+template <int V> __device__ __forceinline__ Vals<V> load_bf16(const uint16_t *p) {
+    uint32_t b[V / 2];
+    if constexpr (V == 8) {
+        const uint4 u = *(const uint4 *)p;
+        b[0] = u.x, b[1] = u.y, b[2] = u.z, b[3] = u.w;
+    } else {
+        const uint2 u = *(const uint2 *)p;
+        b[0] = u.x, b[1] = u.y;
+    }
+    Vals<V> r;
+#pragma unroll
+    for (int q = 0; q < V / 2; q++) {
+        r.v[2 * q] = bf16_to_f32(b[q] & 0xFFFF);
+        r.v[2 * q + 1] = bf16_to_f32(b[q] >> 16);
+    }
+    return r;
 }
 
-// WPR waves of a workgroup of 4 take a row of n <= 256 WPR NJ values, 4 values
-// of a lane at a time, held in registers between the two passes.
-template <int KIND, int WPR, int NJ>
+// WPR waves of a workgroup of 4 take a row of n <= 64 V WPR NJ values, V values of
+// a lane at a time (n a multiple of V).
+template <int KIND, int WPR, int NJ, int V>
 __global__ __launch_bounds__(256) void rows_i8_kernel(RowsArgs a) {
     constexpr bool NORM = KIND >= kNorm, ADD = KIND >= kNormAddBf16;
+    using A = std::conditional_t<NORM, double, float>;  // exact products x w; exact values
     const int tid = threadIdx.x, wave = tid >> 6;
     const int row = blockIdx.x * (4 / WPR) + (WPR == 1 ? wave : 0);
-    const int i0 = WPR == 1 ? (tid & 63) : tid, n4 = a.n / 4;
+    const int i0 = WPR == 1 ? (tid & 63) : tid, nv = a.n / V;
     const bool live = row < a.m;
     const size_t base = (size_t)(live ? row : a.m - 1) * a.n;
-    float4 v[NJ], g[NJ];
+    Vals<V> v[NJ], g[NJ], d[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
-        const size_t e = base + 4 * min(i0 + 64 * WPR * j, n4 - 1);
-        if constexpr (KIND == kBf16) v[j] = load4_bf16((const uint16_t *)a.x + e);
-        else v[j] = *(const float4 *)((const float *)a.x + e);
-        if constexpr (ADD) {
-            const float4 d = KIND == kNormAddBf16 ? load4_bf16((const uint16_t *)a.add + e)
-                                                  : *(const float4 *)((const float *)a.add + e);
-            v[j] = make_float4(v[j].x + d.x, v[j].y + d.y, v[j].z + d.z, v[j].w + d.w);
-        }
-        if constexpr (NORM) g[j] = ((const float4 *)a.w)[min(i0 + 64 * WPR * j, n4 - 1)];
-        // past the row's end: zeros, whatever was loaded there (the row's last
-        // values, which another wave may already have written with the addition)
-        if (i0 + 64 * WPR * j >= n4) v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int i = V * min(i0 + 64 * WPR * j, nv - 1);
+        if constexpr (KIND == kBf16) v[j] = load_bf16<V>((const uint16_t *)a.x + base + i);
+        else v[j] = load_f32<V>((const float *)a.x + base + i);
+        if constexpr (KIND == kNormAddBf16) d[j] = load_bf16<V>((const uint16_t *)a.add + base + i);
+        if constexpr (KIND == kNormAddF32) d[j] = load_f32<V>((const float *)a.add + base + i);
+        if constexpr (NORM) g[j] = load_f32<V>(a.w + i);
     }
-    double top = 0.0, ss = 0.0;
-    bool bad = false;
-    auto val = [&](int j, int e) __attribute__((always_inline)) {
-        const float x = e == 0 ? v[j].x : e == 1 ? v[j].y : e == 2 ? v[j].z : v[j].w;
-        if constexpr (NORM) {
-            const float w = e == 0 ? g[j].x : e == 1 ? g[j].y : e == 2 ? g[j].z : g[j].w;
-            return (double)x * (double)w;
-        }
-        return (double)x;
-    };
+    A top = 0;
+    double ss = 0.0;
+    float nan = 0.f;  // stays 0 while every value (norm: weight) is finite
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
+        const bool in = i0 + 64 * WPR * j < nv;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const double t = fabs(val(j, e));
-            bad |= !(t < __builtin_inf());
-            top = t > top ? t : top;
+        for (int e = 0; e < V; e++) {
+            // past the row's end: zeros, whatever was loaded there (the row's
+            // last values, which another wave may already have written with
+            // the addition)
+            float x = v[j].v[e];
+            if constexpr (ADD) x += d[j].v[e];
+            x = in ? x : 0.f;
+            v[j].v[e] = x;
             if constexpr (NORM) {
-                const double x = e == 0 ? v[j].x : e == 1 ? v[j].y : e == 2 ? v[j].z : v[j].w;
-                ss += x * x;
+                const double xd = x;
+                top = fmax(top, fabs(xd * (double)g[j].v[e]));
+                ss = fma(xd, xd, ss);
+                nan = fmaf(g[j].v[e], 0.f, nan);
+            } else {
+                top = fmaxf(top, fabsf(x));
+                nan = fmaf(x, 0.f, nan);
             }
         }
         if constexpr (ADD)
-            if (live && i0 + 64 * WPR * j < n4) *(float4 *)((float *)a.x + base + 4 * (i0 + 64 * WPR * j)) = v[j];
-    }
-    if (bad) top = __builtin_inf();
+            if (live && in)
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        const double t = __shfl_xor(top, o);
-        top = t > top ? t : top;
-        if constexpr (NORM) ss += __shfl_xor(ss, o);
+                for (int q = 0; q < V / 4; q++)
+                    *(float4 *)((float *)a.x + base + V * (i0 + 64 * WPR * j) + 4 * q) =
+                        make_float4(v[j].v[4 * q], v[j].v[4 * q + 1], v[j].v[4 * q + 2], v[j].v[4 * q + 3]);
     }
+    if (!(nan == 0.f)) top = __builtin_inf();
+    auto larger = [](A p, A q) { return p > q ? p : q; };
+    auto plus = [](double p, double q) { return p + q; };
+    top = wave_reduce(top, larger);
+    if constexpr (NORM) ss = wave_reduce(ss, plus);
     if constexpr (WPR > 1) {
         __shared__ double red[2][4];
         if ((tid & 63) == 0) {
@@ -113,39 +166,75 @@ __global__ __launch_bounds__(256) void rows_i8_kernel(RowsArgs a) {
             red[1][wave] = ss;
         }
         __syncthreads();
-        top = fmax(fmax(red[0][0], red[0][1]), fmax(red[0][2], red[0][3]));
+        top = larger(larger((A)red[0][0], (A)red[0][1]), larger((A)red[0][2], (A)red[0][3]));
         ss = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
     }
     if (!live) return;
-    const bool none = !(top > 0.0) || top == __builtin_inf();
-    const double r = 127.0 / top;
+    // a value that is not finite: the norm's sum of squares shows those of x
+    const bool bad = !(top < (A)__builtin_inf()) || !(ss < __builtin_inf());
+    const bool none = bad || !(top > 0);
+    const bool mid = top >= (A)0x1p-90 && top <= (A)0x1p100;
+    const float r = 127.f / (float)top;
+    auto exact = [&](int j, int e) __attribute__((always_inline)) {
+        const double t = NORM ? (double)v[j].v[e] * (double)g[j].v[e] : (double)v[j].v[e];
+        return (uint32_t)(uint8_t)(int)rint(t * 127.0 / (double)top);
+    };
 #pragma unroll
     for (int j = 0; j < NJ; j++) {
         const int i = i0 + 64 * WPR * j;
-        if (i < n4) {
-            uint32_t c = 0;
-            if (!none)
+        uint32_t c[V / 4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) c |= (uint32_t)(uint8_t)code_of(val(j, e), top, r) << (8 * e);
-            *(uint32_t *)(a.out + base + 4 * i) = c;
+        for (int q = 0; q < V / 4; q++) {
+            uint32_t k[4];
+            float off = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float t = NORM ? v[j].v[4 * q + e] * g[j].v[4 * q + e] : v[j].v[4 * q + e];
+                const float s = fmaf(t, r, kMagic);
+                k[e] = __float_as_uint(s);
+                off = fmaxf(off, fabsf(fmaf(t, r, -(s - kMagic))));
+            }
+            if (!none && (!mid || off > kNear))
+#pragma unroll
+                for (int e = 0; e < 4; e++) k[e] = exact(j, 4 * q + e);
+            c[q] = none ? 0 : (k[0] & 0xFF) | (k[1] & 0xFF) << 8 | (k[2] & 0xFF) << 16 | k[3] << 24;
+        }
+        if (i < nv) {
+            if constexpr (V == 8) *(uint2 *)(a.out + base + 8 * i) = make_uint2(c[0], c[1]);
+            else *(uint32_t *)(a.out + base + 4 * i) = c[0];
         }
     }
     if (i0 == 0) {
-        double sc = top / 127.0;
+        double sc = (double)top / 127.0;
         if constexpr (NORM) sc = sc / sqrt(ss / (double)a.n + (double)a.eps);
-        a.scale[row] = top == __builtin_inf() ? __builtin_nanf("") : none ? 0.f : (float)sc;
+        a.scale[row] = bad ? __builtin_nanf("") : none ? 0.f : (float)sc;
     }
 }
 
-template <int KIND>
+// A wave a row where the rows fill the chip, a workgroup a row for few or long
+// ones.
+template <int KIND, int V>
 void launch_kind(const RowsArgs &a, const char *name, hipStream_t s) {
     KernelSpan span(name, s, true);
-    const dim3 block(256);
-    const dim3 rows4((unsigned)(((size_t)a.m + 3) / 4)), rows1((unsigned)a.m);
-    if (a.n <= 512) launch(span, rows_i8_kernel<KIND, 1, 2>, rows4, block, 0, s, a);
-    else if (a.n <= 2048) launch(span, rows_i8_kernel<KIND, 1, 8>, rows4, block, 0, s, a);
-    else launch(span, rows_i8_kernel<KIND, 4, 8>, rows1, block, 0, s, a);
+    const int nv = a.n / V, per_wave = (nv + 63) / 64, per_wg = (nv + 255) / 256;
+    if (per_wave <= 2 || (a.m >= 1024 && per_wave <= 32 / V)) {
+        const dim3 grid((unsigned)(((size_t)a.m + 3) / 4));
+        if (per_wave <= 1) launch(span, rows_i8_kernel<KIND, 1, 1, V>, grid, dim3(256), 0, s, a);
+        else if (per_wave <= 2) launch(span, rows_i8_kernel<KIND, 1, 2, V>, grid, dim3(256), 0, s, a);
+        else if (per_wave <= 4) launch(span, rows_i8_kernel<KIND, 1, 4, V>, grid, dim3(256), 0, s, a);
+        else launch(span, rows_i8_kernel<KIND, 1, 32 / V, V>, grid, dim3(256), 0, s, a);
+    } else {
+        const dim3 grid((unsigned)a.m);
+        if (per_wg <= 1) launch(span, rows_i8_kernel<KIND, 4, 1, V>, grid, dim3(256), 0, s, a);
+        else if (per_wg <= 2) launch(span, rows_i8_kernel<KIND, 4, 2, V>, grid, dim3(256), 0, s, a);
+        else if (per_wg <= 3) launch(span, rows_i8_kernel<KIND, 4, 3, V>, grid, dim3(256), 0, s, a);
+        else if (per_wg <= 4) launch(span, rows_i8_kernel<KIND, 4, 4, V>, grid, dim3(256), 0, s, a);
+        else if (per_wg <= 6) launch(span, rows_i8_kernel<KIND, 4, V == 8 ? 4 : 6, V>, grid, dim3(256), 0, s, a);
+        else launch(span, rows_i8_kernel<KIND, 4, V == 8 ? 4 : 8, V>, grid, dim3(256), 0, s, a);
+    }
 }
+
+bool aligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
 }  // namespace
 
@@ -153,8 +242,9 @@ hipError_t launch_to_i8(const void *x, bool x_bf16, int m, int n, int8_t *out, f
     if (n % 4 != 0 || n < 4 || n > 8192 || m < 0) return hipErrorInvalidValue;
     if (m == 0) return hipSuccess;
     const RowsArgs a{x, nullptr, nullptr, 0.f, m, n, out, scale};
-    if (x_bf16) launch_kind<kBf16>(a, "to_i8", s);
-    else launch_kind<kF32>(a, "to_i8", s);
+    if (!x_bf16) launch_kind<kF32, 4>(a, "to_i8", s);
+    else if (n % 8 == 0 && aligned(x, 16) && aligned(out, 8)) launch_kind<kBf16, 8>(a, "to_i8", s);
+    else launch_kind<kBf16, 4>(a, "to_i8", s);
     return hipGetLastError();
 }
 
@@ -163,9 +253,9 @@ hipError_t launch_rows_rmsnorm_i8(float *x, const void *add, bool add_bf16, int 
     if (n % 4 != 0 || n < 4 || n > 8192 || m < 0) return hipErrorInvalidValue;
     if (m == 0) return hipSuccess;
     const RowsArgs a{x, add, w, eps, m, n, out, scale};
-    if (!add) launch_kind<kNorm>(a, "rows_rmsnorm_i8", s);
-    else if (add_bf16) launch_kind<kNormAddBf16>(a, "rows_rmsnorm_i8", s);
-    else launch_kind<kNormAddF32>(a, "rows_rmsnorm_i8", s);
+    if (!add) launch_kind<kNorm, 4>(a, "rows_rmsnorm_i8", s);
+    else if (add_bf16) launch_kind<kNormAddBf16, 4>(a, "rows_rmsnorm_i8", s);
+    else launch_kind<kNormAddF32, 4>(a, "rows_rmsnorm_i8", s);
     return hipGetLastError();
 }
 
