@@ -20,7 +20,9 @@
 // its code written once.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "device_common.hpp"
 #include "int8.hpp"
@@ -211,28 +213,35 @@ __global__ __launch_bounds__(256) void rows_i8_kernel(RowsArgs a) {
     }
 }
 
-// A wave a row where the rows fill the chip, a workgroup a row for few or long
-// ones.
+// A wave a row up to 1024 values, a workgroup a row beyond: us a wave / a workgroup,
+// rows after an addition in bf16: 2048 x 1024 6.7 / 7.2, 2048 x 512 4.1 / 5.3, 2048 x
+// 2048 10.2 / 9.6, 256 x 2048 4.8 / 3.4.
 template <int KIND, int V>
 void launch_kind(const RowsArgs &a, const char *name, hipStream_t s) {
     KernelSpan span(name, s, true);
-    const int nv = a.n / V, per_wave = (nv + 63) / 64, per_wg = (nv + 255) / 256;
-    if (per_wave <= 2 || (a.m >= 1024 && per_wave <= 32 / V)) {
+    const int nv = a.n / V;
+    if (a.n <= 1024) {
         const dim3 grid((unsigned)(((size_t)a.m + 3) / 4));
-        if (per_wave <= 1) launch(span, rows_i8_kernel<KIND, 1, 1, V>, grid, dim3(256), 0, s, a);
-        else if (per_wave <= 2) launch(span, rows_i8_kernel<KIND, 1, 2, V>, grid, dim3(256), 0, s, a);
-        else if (per_wave <= 4) launch(span, rows_i8_kernel<KIND, 1, 4, V>, grid, dim3(256), 0, s, a);
-        else launch(span, rows_i8_kernel<KIND, 1, 32 / V, V>, grid, dim3(256), 0, s, a);
-    } else {
-        const dim3 grid((unsigned)a.m);
-        if (per_wg <= 1) launch(span, rows_i8_kernel<KIND, 4, 1, V>, grid, dim3(256), 0, s, a);
-        else if (per_wg <= 2) launch(span, rows_i8_kernel<KIND, 4, 2, V>, grid, dim3(256), 0, s, a);
-        else if (per_wg <= 3) launch(span, rows_i8_kernel<KIND, 4, 3, V>, grid, dim3(256), 0, s, a);
-        else if (per_wg <= 4) launch(span, rows_i8_kernel<KIND, 4, 4, V>, grid, dim3(256), 0, s, a);
-        else if (per_wg <= 6) launch(span, rows_i8_kernel<KIND, 4, V == 8 ? 4 : 6, V>, grid, dim3(256), 0, s, a);
-        else launch(span, rows_i8_kernel<KIND, 4, V == 8 ? 4 : 8, V>, grid, dim3(256), 0, s, a);
+        if (nv <= 64) launch(span, rows_i8_kernel<KIND, 1, 1, V>, grid, dim3(256), 0, s, a);
+        else if (nv <= 128) launch(span, rows_i8_kernel<KIND, 1, 2, V>, grid, dim3(256), 0, s, a);
+        else if constexpr (V == 4) launch(span, rows_i8_kernel<KIND, 1, 4, V>, grid, dim3(256), 0, s, a);
+        return;
+    }
+    const dim3 grid((unsigned)a.m);
+    const int nj = (nv + 255) / 256;  // a lane's loads: at most 4 of 8 values, 8 of 4
+    if (nj <= 1) launch(span, rows_i8_kernel<KIND, 4, 1, V>, grid, dim3(256), 0, s, a);
+    else if (nj <= 2) launch(span, rows_i8_kernel<KIND, 4, 2, V>, grid, dim3(256), 0, s, a);
+    else if (nj <= 3) launch(span, rows_i8_kernel<KIND, 4, 3, V>, grid, dim3(256), 0, s, a);
+    else if (nj <= 4) launch(span, rows_i8_kernel<KIND, 4, 4, V>, grid, dim3(256), 0, s, a);
+    else if constexpr (V == 4) {
+        if (nj <= 6) launch(span, rows_i8_kernel<KIND, 4, 6, V>, grid, dim3(256), 0, s, a);
+        else launch(span, rows_i8_kernel<KIND, 4, 8, V>, grid, dim3(256), 0, s, a);
     }
 }
+
+// rows of one launch: a grid holds less than 2^32 threads (kMaxRows is a
+// multiple of 4, so later parts are aligned as the first)
+constexpr int kMaxRows = 1 << 23;
 
 bool aligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 
@@ -240,23 +249,32 @@ bool aligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; 
 
 hipError_t launch_to_i8(const void *x, bool x_bf16, int m, int n, int8_t *out, float *scale, hipStream_t s) {
     if (n % 4 != 0 || n < 4 || n > 8192 || m < 0) return hipErrorInvalidValue;
-    if (m == 0) return hipSuccess;
-    const RowsArgs a{x, nullptr, nullptr, 0.f, m, n, out, scale};
-    if (!x_bf16) launch_kind<kF32, 4>(a, "to_i8", s);
-    else if (n % 8 == 0 && aligned(x, 16) && aligned(out, 8)) launch_kind<kBf16, 8>(a, "to_i8", s);
-    else launch_kind<kBf16, 4>(a, "to_i8", s);
-    return hipGetLastError();
+    hipError_t e = hipSuccess;
+    for (int r = 0; m - r > 0 && e == hipSuccess; r += std::min(m - r, kMaxRows)) {
+        const char *xr = (const char *)x + (size_t)r * n * (x_bf16 ? 2 : 4);
+        const RowsArgs a{(void *)xr, nullptr, nullptr, 0.f, std::min(m - r, kMaxRows), n, out + (size_t)r * n, scale + r};
+        if (!x_bf16) launch_kind<kF32, 4>(a, "to_i8", s);
+        else if (n % 8 == 0 && aligned(x, 16) && aligned(out, 8)) launch_kind<kBf16, 8>(a, "to_i8", s);
+        else launch_kind<kBf16, 4>(a, "to_i8", s);
+        e = hipGetLastError();
+    }
+    return e;
 }
 
 hipError_t launch_rows_rmsnorm_i8(float *x, const void *add, bool add_bf16, int m, int n, const float *w, float eps,
                                   int8_t *out, float *scale, hipStream_t s) {
     if (n % 4 != 0 || n < 4 || n > 8192 || m < 0) return hipErrorInvalidValue;
-    if (m == 0) return hipSuccess;
-    const RowsArgs a{x, add, w, eps, m, n, out, scale};
-    if (!add) launch_kind<kNorm, 4>(a, "rows_rmsnorm_i8", s);
-    else if (add_bf16) launch_kind<kNormAddBf16, 4>(a, "rows_rmsnorm_i8", s);
-    else launch_kind<kNormAddF32, 4>(a, "rows_rmsnorm_i8", s);
-    return hipGetLastError();
+    hipError_t e = hipSuccess;
+    for (int r = 0; m - r > 0 && e == hipSuccess; r += std::min(m - r, kMaxRows)) {
+        const size_t at = (size_t)r * n;
+        const RowsArgs a{x + at, add ? (const char *)add + at * (add_bf16 ? 2 : 4) : nullptr, w, eps,
+                         std::min(m - r, kMaxRows), n, out + at, scale + r};
+        if (!add) launch_kind<kNorm, 4>(a, "rows_rmsnorm_i8", s);
+        else if (add_bf16) launch_kind<kNormAddBf16, 4>(a, "rows_rmsnorm_i8", s);
+        else launch_kind<kNormAddF32, 4>(a, "rows_rmsnorm_i8", s);
+        e = hipGetLastError();
+    }
+    return e;
 }
 
 }  // namespace hymt
