@@ -176,12 +176,13 @@ __global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
     constexpr int OI = GLU ? IF / 2 : IF;    // ... and their row blocks per wave
     static_assert((2 * NB) % NW == 0 && BJ >= 1 && AHEAD >= 2 && C * (AHEAD - 1) <= 63, "tile shape");
     static_assert(!GLU || IF % 2 == 0, "gate and up row blocks");
-    // after the loop: bf16 rows of the tile (16 bytes of padding a row), the scales
-    constexpr int RS = OF + 8, NS = TF + TT;
-    constexpr int kScaleAt = OUT == kBf16 || GLU ? TT * RS * 2 : 0;
-    constexpr int kLds = S * kStageBytes > kScaleAt + NS * 4 ? S * kStageBytes : kScaleAt + NS * 4;
-    static_assert(kScaleAt % 16 == 0 && kLds <= 160 * 1024, "LDS");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
+    // after the loop: the scales, then each wave's bf16 rows (16 bytes of
+    // padding each), all its token blocks at once where they fit
+    constexpr int NS = TF + TT, kStageAt = NS * 4, RS = 16 * OI + 8;
+    constexpr int JB = kStageAt + NW * BJ * 16 * RS * 2 <= S * kStageBytes ? BJ : BJ / 2;
+    static_assert(kStageAt % 16 == 0 && kStageAt + NW * JB * 16 * RS * 2 <= S * kStageBytes && BJ % JB == 0, "epilogue");
+    static_assert(S * kStageBytes <= 160 * 1024, "LDS");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[S * kStageBytes];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = lane >> 4, c = lane & 15;
@@ -300,70 +301,112 @@ __global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
     wait_vm<0>();     // the copies past the last stage have landed before the ring is reused or freed
     __syncthreads();  // every wave's operand reads are done
 
-    float *scales = (float *)(lds + kScaleAt);
+    float *scales = (float *)lds;
 #pragma unroll
     for (int p = 0; p < PS; p++)
         if (tid + NT * p < NS) scales[tid + NT * p] = sc[p];
     __syncthreads();
 
+    // Each wave writes its own part of the tile, a block of 16 tokens at a time.
+    // chunks: the output's rows are whole 16-byte chunks, which are inside it or
+    // not; whole: the part lies inside the output (its writes have no branch).
+    const int fw = f0 + (OF / 2) * wf, tw = t0 + (TT / WT) * wt;
+    const bool chunks = a.vec && g.n % (OUT == kBf16 || GLU ? 8 : 4) == 0;
+    const bool whole = a.vec && fw + OF / 2 <= g.n && tw + TT / WT <= g.m;
+    float4 ws[OI], us[GLU ? OI : 1];
+#pragma unroll
+    for (int i = 0; i < OI; i++) {
+        ws[i] = *(const float4 *)(scales + (OF / 2) * wf + 16 * i + 4 * grp);
+        if constexpr (GLU) us[i] = *(const float4 *)(scales + OF + (OF / 2) * wf + 16 * i + 4 * grp);
+    }
     if constexpr (OUT == kBf16 || GLU) {
-        // restaged through the (idle) ring as [token][feature] rows, then
-        // written as whole 128-byte lines, 16 bytes a lane
-        uint16_t *st = (uint16_t *)lds;
+        // through LDS as [token][feature] rows, then whole rows, 16 bytes a
+        // lane (the wave's own rows: no barrier)
+        constexpr int CPR = 2 * OI, NQ = JB * 16 * CPR;  // 16-byte chunks of a row, of a batch
+        uint16_t *st = (uint16_t *)(lds + kStageAt) + wave * JB * 16 * RS;
 #pragma unroll
-        for (int j = 0; j < BJ; j++) {
-            const int tl = (TT / WT) * wt + 16 * j + c;
-            const float xs = scales[TF + tl];
+        for (int j0 = 0; j0 < BJ; j0 += JB) {
+            asm volatile("" ::: "memory");  // the rows change hands between the wave's lanes
 #pragma unroll
-            for (int i = 0; i < OI; i++) {
-                const int fl = (OF / 2) * wf + 16 * i + 4 * grp;
-                const float4 ws = *(const float4 *)(scales + fl);
-                const i32x4 v = acc[i][j];
-                float o[4];
-                if constexpr (GLU) {
-                    const float4 us = *(const float4 *)(scales + OF + fl);
-                    const i32x4 u = acc[i + OI][j];
-                    o[0] = glu(v[0], u[0], ws.x, us.x, xs);
-                    o[1] = glu(v[1], u[1], ws.y, us.y, xs);
-                    o[2] = glu(v[2], u[2], ws.z, us.z, xs);
-                    o[3] = glu(v[3], u[3], ws.w, us.w, xs);
-                } else {
-                    o[0] = scaled(v[0], ws.x) * xs;
-                    o[1] = scaled(v[1], ws.y) * xs;
-                    o[2] = scaled(v[2], ws.z) * xs;
-                    o[3] = scaled(v[3], ws.w) * xs;
+            for (int j = j0; j < j0 + JB; j++) {
+                const float xs = scales[TF + (TT / WT) * wt + 16 * j + c];
+#pragma unroll
+                for (int i = 0; i < OI; i++) {
+                    const i32x4 v = acc[i][j];
+                    float o[4];
+                    if constexpr (GLU) {
+                        const i32x4 u = acc[i + OI][j];
+                        o[0] = glu(v[0], u[0], ws[i].x, us[i].x, xs);
+                        o[1] = glu(v[1], u[1], ws[i].y, us[i].y, xs);
+                        o[2] = glu(v[2], u[2], ws[i].z, us[i].z, xs);
+                        o[3] = glu(v[3], u[3], ws[i].w, us[i].w, xs);
+                    } else {
+                        o[0] = scaled(v[0], ws[i].x) * xs;
+                        o[1] = scaled(v[1], ws[i].y) * xs;
+                        o[2] = scaled(v[2], ws[i].z) * xs;
+                        o[3] = scaled(v[3], ws[i].w) * xs;
+                    }
+                    *(uint2 *)(st + (16 * (j - j0) + c) * RS + 16 * i + 4 * grp) = make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
                 }
-                *(uint2 *)(st + tl * RS + fl) = make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3]));
             }
-        }
-        __syncthreads();
-        constexpr int CPR = OF / 8;  // 16-byte chunks of a token row
-        static_assert((TT * CPR) % NT == 0, "restage");
+            asm volatile("" ::: "memory");
 #pragma unroll
-        for (int n = 0; n < TT * CPR / NT; n++) {
-            const int q = n * NT + tid, row = q / CPR, col = q - row * CPR;
-            const int t = t0 + row, f = f0 + 8 * col;
-            if (t >= g.m || f >= g.n) continue;
-            uint16_t *y = (uint16_t *)g.y + (size_t)t * g.ldy + f;
-            const uint16_t *s = st + row * RS + 8 * col;
-            if (a.vec && f + 8 <= g.n) {
-                *(uint4 *)y = *(const uint4 *)s;
-            } else {
-                for (int e = 0; e < min(8, g.n - f); e++) y[e] = s[e];
+            for (int q0 = 0; q0 < NQ; q0 += 64) {
+                const int q = q0 + lane, row = q / CPR, col = q - row * CPR;
+                if (NQ % 64 != 0 && q >= NQ) continue;
+                const int t = tw + 16 * j0 + row, f = fw + 8 * col;
+                const uint16_t *from = st + row * RS + 8 * col;
+                uint16_t *y = (uint16_t *)g.y + (size_t)t * g.ldy + f;
+                if (whole) {
+                    *(uint4 *)y = *(const uint4 *)from;
+                } else if (chunks) {
+                    if (t < g.m && f < g.n) *(uint4 *)y = *(const uint4 *)from;
+                } else if (t < g.m) {
+                    for (int e = 0; e < 8; e++)
+                        if (f + e < g.n) y[e] = from[e];
+                }
             }
         }
+    } else if (whole || chunks) {
+        float *y = (float *)g.y + (size_t)(tw + c) * g.ldy + fw + 4 * grp;
+        const size_t step = (size_t)16 * g.ldy;
+        auto write = [&](auto all) __attribute__((always_inline)) {
+            auto inside = [&](int i, int j) __attribute__((always_inline)) {
+                return decltype(all)::value || (tw + 16 * j + c < g.m && fw + 16 * i + 4 * grp < g.n);
+            };
+#pragma unroll
+            for (int j = 0; j < BJ; j++) {
+                const float xs = scales[TF + (TT / WT) * wt + 16 * j + c];
+                float4 old[OUT == kAcc ? IF : 1];
+                if constexpr (OUT == kAcc)
+#pragma unroll
+                    for (int i = 0; i < IF; i++)
+                        if (inside(i, j)) old[i] = *(const float4 *)(y + j * step + 16 * i);
+#pragma unroll
+                for (int i = 0; i < IF; i++) {
+                    const i32x4 v = acc[i][j];
+                    const float o[4] = {scaled(v[0], ws[i].x), scaled(v[1], ws[i].y), scaled(v[2], ws[i].z),
+                                        scaled(v[3], ws[i].w)};
+                    float4 r = make_float4(o[0] * xs, o[1] * xs, o[2] * xs, o[3] * xs);
+                    if constexpr (OUT == kAcc)
+                        r = make_float4(fmaf(o[0], xs, old[i].x), fmaf(o[1], xs, old[i].y), fmaf(o[2], xs, old[i].z),
+                                        fmaf(o[3], xs, old[i].w));
+                    if (inside(i, j)) *(float4 *)(y + j * step + 16 * i) = r;
+                }
+            }
+        };
+        if (whole) write(std::true_type{});
+        else write(std::false_type{});
     } else {
 #pragma unroll
         for (int j = 0; j < BJ; j++) {
-            const int tl = (TT / WT) * wt + 16 * j + c;
-            if (t0 + tl >= g.m) continue;
-            const float xs = scales[TF + tl];
+            const int t = tw + 16 * j + c;
+            if (t >= g.m) continue;
+            const float xs = scales[TF + (TT / WT) * wt + 16 * j + c];
 #pragma unroll
-            for (int i = 0; i < IF; i++) {
-                const int fl = (TF / 2) * wf + 16 * i + 4 * grp;
-                const float4 w4 = *(const float4 *)(scales + fl);
-                const float ws[4] = {w4.x, w4.y, w4.z, w4.w};
-                store4<OUT>(a, t0 + tl, f0 + fl, acc[i][j], acc[i][j], ws, ws, xs);
+            for (int i = 0; i < OI; i++) {
+                const float w4[4] = {ws[i].x, ws[i].y, ws[i].z, ws[i].w};
+                store4<OUT>(a, t, fw + 16 * i + 4 * grp, acc[i][j], acc[i][j], w4, w4, xs);
             }
         }
     }
