@@ -417,7 +417,11 @@ __global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
 // A workgroup owns 16 A features x 16 B tokens and its four waves split k: each
 // streams its own quarter of the tile's W and x rows through an LDS ring of its
 // own, so there is no barrier before the end and four load streams run per
-// workgroup.  The four partial tiles meet in LDS.  SwiGLU: the first A / 2 row
+// workgroup.  The four partial tiles meet in LDS.  Bound by the stream of W (one
+// token, 120818 channels: 44 us, 5.6 TB/s) or, where that is short, by a launch and
+// two memory round trips (one token, 2048 x 2048: 2.8 us in a recording).  Deeper
+// rings and eight waves a workgroup were no faster at 1-700 tokens; W straight
+// into registers was (43 us) at one token of 120818 channels alone.  SwiGLU: the first A / 2 row
 // blocks are gate rows, the others the same rows of up.
 template <int A, int B, int S, int OUT>
 __global__ __launch_bounds__(256) void skinny_kernel(Args a) {
@@ -485,15 +489,12 @@ __global__ __launch_bounds__(256) void skinny_kernel(Args a) {
             for (int j = 0; j < B; j++) x[ks][j] = *(const i32x4 *)(p + off[ks] + (A + j) * kPair);
         }
     };
-    auto mma = [&]() __attribute__((always_inline)) {
-        slot = slot + 1 == S ? 0 : slot + 1;
+    auto mma = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ks++)
+        for (int i = 0; i < A; i++)
 #pragma unroll
-            for (int i = 0; i < A; i++)
-#pragma unroll
-                for (int j = 0; j < B; j++)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[ks][i], x[ks][j], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < B; j++)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[ks][i], x[ks][j], acc[i][j], 0, 0, 0);
     };
     // A wave's copies retire in order: a stage has landed once at most S - 1
     // younger stages are outstanding.  Its slot is refilled as soon as this wave
@@ -504,9 +505,13 @@ __global__ __launch_bounds__(256) void skinny_kernel(Args a) {
     for (int t = S; t < n; t++) {
         wait_vm<(S - 1) * C>();
         read();
+        mma(0);
+        __builtin_amdgcn_sched_barrier(0);
         wait_lgkm();
         copy(t, slot);
-        mma();
+        __builtin_amdgcn_sched_barrier(0);
+        mma(1);
+        slot = slot + 1 == S ? 0 : slot + 1;
     }
     // the last S stages (or all, where there are fewer), nothing left to issue
     const int left = min(S, n);
@@ -518,7 +523,9 @@ __global__ __launch_bounds__(256) void skinny_kernel(Args a) {
             else if (l == 2) wait_vm<(S > 1 ? 1 : 0) * C>();
             else wait_vm<0>();
             read();
-            mma();
+            mma(0);
+            mma(1);
+            slot = slot + 1 == S ? 0 : slot + 1;
         }
     wait_lgkm();
 
@@ -549,95 +556,64 @@ __global__ __launch_bounds__(256) void skinny_kernel(Args a) {
     }
 }
 
-// ---- up to 16 tokens -------------------------------------------------------------
-//
-// A stream of W: a workgroup takes 16 channels (SwiGLU: 16 gate and their 16 up
-// rows), its four waves a quarter of k each, straight from memory into the
-// operand registers, 4 stages (8 KiB of W a wave) at a time with no ring and no
-// LDS before the end, so that many workgroups share a CU and keep loads in
-// flight for each other.
-template <int OUT>
-__global__ __launch_bounds__(256) void gemv_kernel(Args a) {
-    constexpr bool GLU = OUT == kGlu;
-    constexpr int A = GLU ? 2 : 1, U = GLU ? 2 : 4;  // row blocks; stages at a time
-    __shared__ __attribute__((aligned(16))) i32x4 part[4][A][64];
-    const I8Gemm &g = a.g;
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int grp = lane >> 4, c = lane & 15;
-    const int f0 = 16 * blockIdx.x;
-    const int kt = g.k / kBK, s0 = kt * wave / 4, s1 = kt * (wave + 1) / 4;
-    const size_t wo = (size_t)min(f0 + c, g.n - 1) * g.k + 16 * grp;
-    const int8_t *wp[2] = {g.w + wo, GLU ? g.up + wo : nullptr};
-    const int8_t *xp = g.x + (size_t)min(c, g.m - 1) * g.k + 16 * grp;
-    i32x4 acc[A] = {};
-    auto stages = [&](int s, auto count) __attribute__((always_inline)) {
-        constexpr int N = 2 * decltype(count)::value;
-        i32x4 w[A][N], x[N];
-#pragma unroll
-        for (int j = 0; j < N; j++) {
-#pragma unroll
-            for (int i = 0; i < A; i++) w[i][j] = *(const i32x4 *)(wp[i] + s * kBK + 64 * j);
-            x[j] = *(const i32x4 *)(xp + s * kBK + 64 * j);
-        }
-#pragma unroll
-        for (int j = 0; j < N; j++)
-#pragma unroll
-            for (int i = 0; i < A; i++) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i][j], x[j], acc[i], 0, 0, 0);
-    };
-    int s = s0;
-    for (; s + U <= s1; s += U) stages(s, std::integral_constant<int, U>{});
-    for (; s < s1; s++) stages(s, std::integral_constant<int, 1>{});
-#pragma unroll
-    for (int i = 0; i < A; i++) part[wave][i][lane] = acc[i];
-    __syncthreads();
-    const int f = f0 + 4 * grp;
-    if (tid >= 64 || c >= g.m || f >= g.n) return;
-    auto sum = [&](int i) __attribute__((always_inline)) {
-        return (part[0][i][lane] + part[1][i][lane]) + (part[2][i][lane] + part[3][i][lane]);
-    };
-    float ws[4], us[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        ws[e] = g.ws[min(f + e, g.n - 1)];
-        us[e] = GLU ? g.us[min(f + e, g.n - 1)] : 0.f;
-    }
-    const i32x4 v = sum(0);
-    store4<OUT>(a, c, f, v, GLU ? sum(A - 1) : v, ws, us, g.xs[c]);
-}
-
 // ---- which kernel --------------------------------------------------------------
 
-// The tiles: features x tokens (SwiGLU: half as many outputs), the first kSkinny
-// of them the few-token kernel's.
+// The tiles: features x tokens (SwiGLU: half as many outputs), the first 8 the
+// few-token kernel's, and what a launch of `tiles` of them takes: us =
+//   launch + R (round + stage kt) + F (fill + fill_stage kt),
+// R = ceil(tiles / 256) rounds of the chip, F = tiles / 256 (what grows with the traffic of
+// all CUs together), kt = k / 128.  Fitted to 955 measurements: 1-4096 tokens, 64-120818
+// channels, k 256-8192, every output; the tile of the least estimate takes 0.5 %
+// longer on average than the fastest one (worst 31 %: 2555 x 128 x 512).  E.g., us
+// estimated / measured: 2048 x 2048 x 2048 bf16 128 x 128 14.5 / 12.9, 128 x 64 18.5 / 16.2, 192 x
+// 256 23.7 / 22.1; 61 x 2048 x 6144 fp32 32 x 16 6.4 / 6.5, 32 x 32 6.6 / 7.6.
 struct Shape {
     const char *name;
-    int f, t;
+    int f, t, threads;
+    float launch, round, stage, fill, fill_stage;
 };
-constexpr Shape kShapes[] = {{"stream", 16, 16}, {"16x16", 16, 16},   {"32x16", 32, 16},   {"32x32", 32, 32},   {"32x64", 32, 64},
-                             {"64x64", 64, 64},   {"96x64", 96, 64},   {"128x64", 128, 64}, {"128x96", 128, 96},
-                             {"128x128", 128, 128}, {"192x128", 192, 128}, {"256x128", 256, 128}, {"128x256", 128, 256},
-                             {"192x256", 192, 256}, {"256x256", 256, 256}};
-constexpr int kNumShapes = sizeof(kShapes) / sizeof(kShapes[0]), kSkinny = 7;
+constexpr Shape kShapes[] = {
+    {"16x16", 16, 16, 256, 2.40f, 0.26f, 0.027f, 0.08f, 0.021f},
+    {"32x16", 32, 16, 256, 2.56f, 0.19f, 0.042f, 0.17f, 0.030f},
+    {"48x16", 48, 16, 256, 2.80f, 0.00f, 0.056f, 0.37f, 0.038f},
+    {"64x16", 64, 16, 256, 2.88f, 0.00f, 0.075f, 0.40f, 0.040f},
+    {"32x32", 32, 32, 256, 2.58f, 0.28f, 0.055f, 0.17f, 0.044f},
+    {"64x32", 64, 32, 256, 2.17f, 1.08f, 0.092f, 0.40f, 0.074f},
+    {"64x64", 64, 64, 256, 2.01f, 2.05f, 0.132f, 0.38f, 0.105f},
+    {"96x64", 96, 64, 256, 2.34f, 2.48f, 0.194f, 0.96f, 0.114f},
+    {"128x64", 128, 64, 256, 2.86f, 0.48f, 0.250f, 1.98f, 0.085f},
+    {"128x96", 128, 96, 256, 2.66f, 1.54f, 0.277f, 1.71f, 0.103f},
+    {"128x128", 128, 128, 256, 3.24f, 1.46f, 0.344f, 2.37f, 0.118f},
+    {"192x128", 192, 128, 512, 3.33f, 2.03f, 0.417f, 3.09f, 0.237f},
+    {"256x128", 256, 128, 256, 4.82f, 1.60f, 0.604f, 4.78f, 0.210f},
+    {"192x256", 192, 256, 512, 5.15f, 1.26f, 0.865f, 6.43f, 0.230f},
+    {"256x256", 256, 256, 512, 8.01f, 0.68f, 0.944f, 7.05f, 0.433f},
+};
+constexpr int kNumShapes = sizeof(kShapes) / sizeof(kShapes[0]);
+constexpr size_t kMaxTiles = 1u << 22;  // of a launch: a grid holds less than 2^32 threads
 
-template <int OUT> int plan(const I8Gemm &g) {
-    constexpr int first = OUT == kGlu ? 2 : 1;  // gate and up: two row blocks at least
-    if (const char *e = std::getenv("HYMT_HIP_I8_TILE"))
-        for (int i = first; i < kNumShapes; i++)
-            if (!std::strcmp(e, kShapes[i].name)) return i;
-    if (std::getenv("HYMT_STREAM") && g.m <= 16) return 0;
-    const long n = (long)g.n * (OUT == kGlu ? 2 : 1);
-    auto tiles = [&](int i) { return (n + kShapes[i].f - 1) / kShapes[i].f * ((g.m + kShapes[i].t - 1) / kShapes[i].t); };
-    for (int i = first; i < kSkinny; i++)
-        if (tiles(i) <= 256) return i;
-    int best = kSkinny;
-    double fill = 0;
-    for (int i = kSkinny; i < kNumShapes; i++) {
-        const long w = tiles(i);
-        const double f = (double)w / (256.0 * ((w + 255) / 256)) * (0.9 + 0.01 * i);
-        if (f > fill) {
-            fill = f;
+size_t tiles_of(const Shape &p, const I8Gemm &g, bool glu) {
+    const int of = glu ? p.f / 2 : p.f;
+    return (size_t)((g.n + of - 1) / of) * ((g.m + p.t - 1) / p.t);
+}
+
+// The tile of the least estimated time; HYMT_HIP_I8_TILE=<tile> forces one (a
+// tuning knob).  SwiGLU takes the tiles whose row blocks split into gate and up.
+int plan(const I8Gemm &g, bool glu) {
+    const char *forced = std::getenv("HYMT_HIP_I8_TILE");
+    const float kt = (float)(g.k / kBK);
+    int best = -1;
+    float least = 0.f;
+    for (int i = 0; i < kNumShapes; i++) {
+        const Shape &p = kShapes[i];
+        const size_t tiles = tiles_of(p, g, glu);
+        if (tiles > kMaxTiles || (glu && p.f % 32 != 0)) continue;
+        if (forced && !std::strcmp(forced, p.name)) return i;
+        const float rounds = (float)((tiles + 255) / 256), fill = (float)tiles / 256.f;
+        const float us = p.launch + rounds * (p.round + p.stage * kt) + fill * (p.fill + p.fill_stage * kt);
+        if (best < 0 || us < least) {
             best = i;
+            least = us;
         }
     }
     return best;
@@ -645,25 +621,27 @@ template <int OUT> int plan(const I8Gemm &g) {
 
 template <int OUT>
 void launch_shape(int i, const Args &a, const KernelSpan &span, hipStream_t s) {
-    const dim3 grid(8 * a.per_xcd);
+    const dim3 grid(8 * a.per_xcd), block(kShapes[i].threads);
     switch (i) {
-    case 0: launch(span, gemv_kernel<OUT>, dim3(a.tiles_f), dim3(256), 0, s, a); break;
-    case 1:
-        if constexpr (OUT != kGlu) launch(span, skinny_kernel<1, 1, 4, OUT>, grid, dim3(256), 0, s, a);
+    case 0:
+        if constexpr (OUT != kGlu) launch(span, skinny_kernel<1, 1, 4, OUT>, grid, block, 0, s, a);
         break;
-    case 2: launch(span, skinny_kernel<2, 1, 3, OUT>, grid, dim3(256), 0, s, a); break;
-    case 3: launch(span, skinny_kernel<2, 2, 2, OUT>, grid, dim3(256), 0, s, a); break;
-    case 4: launch(span, skinny_kernel<2, 4, 2, OUT>, grid, dim3(256), 0, s, a); break;
-    case 5: launch(span, skinny_kernel<4, 4, 2, OUT>, grid, dim3(256), 0, s, a); break;
-    case 6: launch(span, skinny_kernel<6, 4, 2, OUT>, grid, dim3(256), 0, s, a); break;
-    case 7: launch(span, tile_kernel<4, 2, 2, 4, false, OUT>, grid, dim3(256), 0, s, a); break;
-    case 8: launch(span, tile_kernel<4, 3, 2, 4, false, OUT>, grid, dim3(256), 0, s, a); break;
-    case 9: launch(span, tile_kernel<4, 4, 2, 4, false, OUT>, grid, dim3(256), 0, s, a); break;
-    case 10: launch(span, tile_kernel<6, 4, 4, 4, true, OUT>, grid, dim3(512), 0, s, a); break;
-    case 11: launch(span, tile_kernel<8, 4, 2, 3, true, OUT>, grid, dim3(256), 0, s, a); break;
-    case 12: launch(span, tile_kernel<4, 8, 2, 3, true, OUT>, grid, dim3(256), 0, s, a); break;
-    case 13: launch(span, tile_kernel<6, 8, 4, 2, true, OUT>, grid, dim3(512), 0, s, a); break;
-    default: launch(span, tile_kernel<8, 8, 4, 2, true, OUT>, grid, dim3(512), 0, s, a); break;
+    case 1: launch(span, skinny_kernel<2, 1, 3, OUT>, grid, block, 0, s, a); break;
+    case 2:
+        if constexpr (OUT != kGlu) launch(span, skinny_kernel<3, 1, 2, OUT>, grid, block, 0, s, a);
+        break;
+    case 3: launch(span, skinny_kernel<4, 1, 2, OUT>, grid, block, 0, s, a); break;
+    case 4: launch(span, skinny_kernel<2, 2, 2, OUT>, grid, block, 0, s, a); break;
+    case 5: launch(span, skinny_kernel<4, 2, 2, OUT>, grid, block, 0, s, a); break;
+    case 6: launch(span, skinny_kernel<4, 4, 2, OUT>, grid, block, 0, s, a); break;
+    case 7: launch(span, skinny_kernel<6, 4, 2, OUT>, grid, block, 0, s, a); break;
+    case 8: launch(span, tile_kernel<4, 2, 2, 4, false, OUT>, grid, block, 0, s, a); break;
+    case 9: launch(span, tile_kernel<4, 3, 2, 4, false, OUT>, grid, block, 0, s, a); break;
+    case 10: launch(span, tile_kernel<4, 4, 2, 4, false, OUT>, grid, block, 0, s, a); break;
+    case 11: launch(span, tile_kernel<6, 4, 4, 4, true, OUT>, grid, block, 0, s, a); break;
+    case 12: launch(span, tile_kernel<8, 4, 2, 3, true, OUT>, grid, block, 0, s, a); break;
+    case 13: launch(span, tile_kernel<6, 8, 4, 2, true, OUT>, grid, block, 0, s, a); break;
+    default: launch(span, tile_kernel<8, 8, 4, 2, true, OUT>, grid, block, 0, s, a); break;
     }
 }
 
@@ -677,16 +655,15 @@ template <int OUT>
 hipError_t run(const I8Gemm &g, const char *name, hipStream_t s) {
     if (!fits(g)) return hipErrorInvalidValue;
     if (g.m == 0) return hipSuccess;
-    const int i = plan<OUT>(g);
-    const int of = OUT == kGlu && i > 0 ? kShapes[i].f / 2 : kShapes[i].f;
+    const int i = plan(g, OUT == kGlu);
+    if (i < 0) return hipErrorInvalidValue;  // more tiles than a launch holds
+    const int of = OUT == kGlu ? kShapes[i].f / 2 : kShapes[i].f;
     Args a{};
     a.g = g;
     a.tiles_f = (g.n + of - 1) / of;
     a.tiles_t = (g.m + kShapes[i].t - 1) / kShapes[i].t;
-    const size_t tiles = (size_t)a.tiles_f * a.tiles_t;
-    if (tiles > 0x7ffffff0u) return hipErrorInvalidValue;
-    a.tiles = (int)tiles;
-    a.per_xcd = (int)((tiles + 7) / 8);
+    a.tiles = a.tiles_f * a.tiles_t;
+    a.per_xcd = (a.tiles + 7) / 8;
     constexpr int es = OUT == kBf16 || OUT == kGlu ? 2 : 4;
     a.vec = ((uintptr_t)g.y & 15u) == 0 && g.ldy % (16 / es) == 0;
     KernelSpan span(name, s, true);

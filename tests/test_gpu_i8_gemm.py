@@ -206,8 +206,8 @@ def test_offsets_past_32_bits(be):
         r.close()
 
 
-TILES = ["16x16", "32x16", "32x32", "32x64", "64x64", "96x64", "128x64", "128x96", "128x128", "192x128", "256x128",
-         "128x256", "192x256", "256x256"]
+TILES = ["16x16", "32x16", "48x16", "64x16", "32x32", "64x32", "64x64", "96x64", "128x64", "128x96", "128x128",
+         "192x128", "256x128", "192x256", "256x256"]
 
 
 @pytest.mark.parametrize("tile", TILES)
