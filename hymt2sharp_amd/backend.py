@@ -224,16 +224,18 @@ class HipBackend:
 
     # ---- the model: IComputeBackend.LoadModel / ForwardStep (IComputeBackend.cs:25-47)
     def LoadModel(self, tensors: dict, config, max_tokens: int = 4096, kv_dtype: int = N.BF16,
-                  prefill: bool = True):
+                  prefill: bool = True, int8: bool = False):
         """tensors: GGUF name -> model.Tensor; config: model.ModelConfig.
         Uploads every weight, creates the KV cache, keeps activations on the
         device (hymt2sharp_amd/model.py).  prefill: also keep bf16 dense
-        copies of the layer weights so that multi-token calls run as GEMMs."""
+        copies of the layer weights so that multi-token calls run as GEMMs.
+        int8: keep int8 codes of them instead, and run those calls in 8-bit
+        integers (HYMT_PREFILL_INT8)."""
         from .model import DeviceModel
         if getattr(self, "_model", None) is not None:
             self._model.free()
             self._model = None
-        self._model = DeviceModel(self, config, tensors, max_tokens, kv_dtype, prefill=prefill)
+        self._model = DeviceModel(self, config, tensors, max_tokens, kv_dtype, prefill=prefill, int8=int8)
         return self
 
     def ForwardStep(self, tokens, pos: int) -> np.ndarray:

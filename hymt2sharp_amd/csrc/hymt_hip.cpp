@@ -1532,7 +1532,10 @@ struct hymt_model {
     // [C][q|k|v], ao16 bf16 [C][qd] (the attention writes it as bf16), gu [C][2F] (bf16, or fp32
     // with HYMT_PREFILL_GATE_UP_F32), act bf16 [C][F]; token ids through a
     // pinned buffer whose last copy is marked by tok_ev
-    DevBuf px, pxn, pqkv, pao16, pgu, pact, ptok;
+    // HYMT_PREFILL_INT8 takes xn, ao and act as int8 codes pq8 [C][n] with scales
+    // pq8s [C], and the o and down products as bf16 pdelta [C][H], which the
+    // next norm adds to x
+    DevBuf px, pxn, pqkv, pao16, pgu, pact, ptok, pq8, pq8s, pdelta;
     HostBuf htok;
     hipEvent_t tok_ev = nullptr;
 };
@@ -1550,6 +1553,52 @@ bool prefill_ready(const hymt_model *m) {
         if (!Ly.down->dense) return false;
     }
     return true;
+}
+
+bool prefill_i8_ready(const hymt_model *m) {
+    for (const auto &Ly : m->L) {
+        for (const hymt_weight *w : Ly.w)
+            if (w && !w->i8) return false;
+        if (!Ly.down->i8) return false;
+    }
+    return true;
+}
+
+// A layer's prompt rows over the weights' int8 codes (x and the rows' norms as
+// the bf16 sequence has them).  first: x holds the residual; else the product
+// in pdelta is added to it first.  last: the down product goes onto x itself.
+int prefill_layer_i8(hymt_model *m, int l, int p0, int rows, bool first, bool last) {
+    hymt_ctx *c = m->ctx;
+    const hymt_model::Layer &Ly = m->L[l];
+    const int H = m->hidden, F = m->ffn, qd = c->heads * c->head_dim, kd = c->kv_heads * c->head_dim;
+    const int ld = qd + 2 * kd;
+    float *x = (float *)m->px.p, *xs = (float *)m->pq8s.p;
+    int8_t *q8 = (int8_t *)m->pq8.p;
+    uint16_t *qkv = (uint16_t *)m->pqkv.p, *ao16 = (uint16_t *)m->pao16.p, *act = (uint16_t *)m->pact.p;
+    uint16_t *delta = (uint16_t *)m->pdelta.p;
+    auto gemm = [&](const hymt_weight *w, void *y, int ldy, I8Out out) {
+        HIP_TRY(launch_gemm_i8(I8Gemm{w->i8, w->i8_scale, nullptr, nullptr, q8, xs, y, w->dev.rows, w->dev.cols, rows, ldy},
+                               out, c->stream));
+    };
+    HIP_TRY(launch_rows_rmsnorm_i8(x, first ? nullptr : delta, true, rows, H, Ly.attn_norm, m->eps, q8, xs, c->stream));
+    gemm(Ly.w[0], qkv, ld, kI8Bf16);
+    if (Ly.w[1]) {
+        gemm(Ly.w[1], qkv + qd, ld, kI8Bf16);
+        gemm(Ly.w[2], qkv + qd + kd, ld, kI8Bf16);
+    }
+    if (int r = prefill_impl(c, l, p0, rows, qkv, ld, qkv + qd, qkv + qd + kd, ld, HYMT_BF16, Ly.q_norm, Ly.k_norm,
+                             (float *)ao16, HYMT_FLAG_DEVICE_PTRS, true))
+        return r;
+    HIP_TRY(launch_to_i8(ao16, true, rows, qd, q8, xs, c->stream));
+    gemm(Ly.w[3], delta, H, kI8Bf16);
+    HIP_TRY(launch_rows_rmsnorm_i8(x, delta, true, rows, H, Ly.ffn_norm, m->eps, q8, xs, c->stream));
+    const hymt_weight *wg = Ly.w[4], *wu = Ly.w[5];
+    HIP_TRY(launch_gemm_i8_swiglu(I8Gemm{wg->i8, wg->i8_scale, wu ? wu->i8 : wg->i8 + (size_t)F * H,
+                                         wu ? wu->i8_scale : wg->i8_scale + F, q8, xs, act, F, H, rows, F},
+                                  c->stream));
+    HIP_TRY(launch_to_i8(act, true, rows, F, q8, xs, c->stream));
+    gemm(Ly.down, last ? (void *)x : delta, H, last ? kI8Acc : kI8Bf16);
+    return HYMT_OK;
 }
 
 // y (+)= x . W^T over the weight's dense copy, rows ldy elements apart
@@ -1705,7 +1754,13 @@ int hymt_model_prefill(hymt_model *m, const int32_t *tokens, int n, int pos, flo
     if (!m->embd || !logits) return fail(HYMT_E_STATE, "hymt_model_set_io first (and a logits buffer)");
     for (const auto &Ly : m->L)
         if (!Ly.set) return fail(HYMT_E_STATE, "every layer needs hymt_model_set_layer");
-    if (flags & ~HYMT_PREFILL_GATE_UP_F32) return fail(HYMT_E_ARG, "unknown prefill flags");
+    if (flags & ~(HYMT_PREFILL_GATE_UP_F32 | HYMT_PREFILL_INT8)) return fail(HYMT_E_ARG, "unknown prefill flags");
+    const bool int8 = flags & HYMT_PREFILL_INT8;
+    if (int8 && (flags & HYMT_PREFILL_GATE_UP_F32))
+        return fail(HYMT_E_ARG, "HYMT_PREFILL_INT8 and HYMT_PREFILL_GATE_UP_F32 exclude each other");
+    if (int8 && !prefill_i8_ready(m))
+        return fail(HYMT_E_STATE, "a layer weight has no int8 codes (hymt_weight_i8)");
+    if (int8 && m->ffn > 8192) return fail(HYMT_E_UNSUPPORTED, "HYMT_PREFILL_INT8 takes rows of up to 8192 values");
     if (n < 1 || !tokens) return fail(HYMT_E_ARG, "empty token list");
     for (int i = 0; i < n; i++)
         if (tokens[i] < 0 || tokens[i] >= m->vocab) return fail(HYMT_E_ARG, "token out of range");
@@ -1715,7 +1770,7 @@ int hymt_model_prefill(hymt_model *m, const int32_t *tokens, int n, int pos, flo
                                          std::to_string((long)pos + n));
     if (!c->pages.resident(pos)) return fail(HYMT_E_STATE, "device KV must hold [0, pos) before prefill");
     if (int r = refuse_in_capture(c, "hymt_model_prefill")) return r;
-    if (n == 1 || !prefill_ready(m)) {
+    if (n == 1 || c->kv_dtype == HYMT_F32 || (!int8 && !prefill_ready(m))) {
         // one token, an fp32 cache or no dense copies: the tokens run as
         // decode steps, as ForwardStep does without a prefill path
         for (int i = 0; i < n; i++)
@@ -1729,11 +1784,17 @@ int hymt_model_prefill(hymt_model *m, const int32_t *tokens, int n, int pos, flo
     try {
         HIP_TRY(hipSetDevice(c->device));
         m->px.reserve(C * H * 4);
-        m->pxn.reserve(C * H * 2);
         m->pqkv.reserve(C * ld * 2);
         m->pao16.reserve(C * qd * 2);
-        m->pgu.reserve(C * 2 * F * 4);
         m->pact.reserve(C * F * 2);
+        if (int8) {
+            m->pq8.reserve(C * std::max({H, F, qd}));
+            m->pq8s.reserve(C * 4);
+            m->pdelta.reserve(C * H * 2);
+        } else {
+            m->pxn.reserve(C * H * 2);
+            m->pgu.reserve(C * 2 * F * 4);
+        }
         m->ptok.reserve(C * 4);
         if (!m->htok.p) {
             m->htok.reserve(C * 4);
@@ -1754,6 +1815,10 @@ int hymt_model_prefill(hymt_model *m, const int32_t *tokens, int n, int pos, flo
             HIP_TRY(launch_rows(m->embd->dev, (const int *)m->ptok.p, 0, rows, x, c->stream));
             for (int l = 0; l < m->layers; l++) {
                 const hymt_model::Layer &Ly = m->L[l];
+                if (int8) {
+                    if (int r = prefill_layer_i8(m, l, p0, rows, l == 0, l == m->layers - 1)) return r;
+                    continue;
+                }
                 HIP_TRY(launch_rows_rmsnorm(x, rows, H, Ly.attn_norm, m->eps, xn, c->stream));
                 if (!Ly.w[1]) {
                     model_gemm(c, Ly.w[0], xn, rows, qkv, ld, true, false);
@@ -1807,7 +1872,7 @@ int hymt_model_destroy(hymt_model *m) {
         (void)hipStreamSynchronize(c->stream);
     }
     for (DevBuf *b : {&m->h, &m->qkv, &m->ao, &m->gu, &m->px, &m->pxn, &m->pqkv, &m->pao16, &m->pgu,
-                      &m->pact, &m->ptok})
+                      &m->pact, &m->ptok, &m->pq8, &m->pq8s, &m->pdelta})
         b->release();
     m->htok.release();
     if (m->tok_ev) (void)hipEventDestroy(m->tok_ev);

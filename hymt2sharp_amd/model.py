@@ -81,8 +81,8 @@ class DeviceModel:
     PREFILL_CHUNK = 2048
 
     def __init__(self, be, cfg: ModelConfig, tensors: dict, max_tokens: int, kv_dtype: int = N.BF16,
-                 prefill: bool = True):
-        self.be, self.cfg, self.prefill_enabled = be, cfg, prefill
+                 prefill: bool = True, int8: bool = False):
+        self.be, self.cfg, self.prefill_enabled, self.int8 = be, cfg, prefill, prefill and int8
         c = cfg
         self._weights, self._bufs = [], []
         be.configure(c.num_heads, c.num_kv_heads, c.head_dim, c.rope_dim, c.rope_base, c.eps)
@@ -111,7 +111,7 @@ class DeviceModel:
         def dense(ws):
             if prefill:
                 for w in ws:
-                    be.weight_dense(w)
+                    be.weight_i8(w) if int8 else be.weight_dense(w)
             return ws
 
         self.layers = []
@@ -136,7 +136,7 @@ class DeviceModel:
         self.ao = self._buf(qd)
         self.gu = self._buf(2 * c.ffn_size)
         self.logits = self._buf(c.vocab_size)
-        self._pf = None  # prefill activations, allocated on the first prefill
+        self._pf = self._pf8 = None  # prefill activations, allocated on the first composed prefill
         # the decode step runs natively: one hymt_model_decode per token
         lib, h = be._lib, ctypes.c_void_p()
         N.check(lib.hymt_model_create(be._h, c.num_layers, c.hidden_size, c.ffn_size, c.vocab_size,
@@ -193,9 +193,10 @@ class DeviceModel:
         hymt_model_prefill call (chunks of 2048 rows, or decode steps without
         dense copies or with an fp32 cache); the last row's logits land in
         self.logits.  gate_up_f32 keeps the gate/up GEMM output in fp32, as
-        the reference's prefill does."""
+        the reference's prefill does.  A model loaded with int8 runs it over
+        the int8 codes."""
         t = np.ascontiguousarray(tokens, dtype=np.int32)
-        flags = N.PREFILL_GATE_UP_F32 if gate_up_f32 else 0
+        flags = (N.PREFILL_GATE_UP_F32 if gate_up_f32 else 0) | (N.PREFILL_INT8 if self.int8 else 0)
         N.check(self.be._lib.hymt_model_prefill(self._native, t.ctypes.data_as(ctypes.c_void_p), t.size, pos,
                                                 self.logits, flags))
 
@@ -241,6 +242,58 @@ class DeviceModel:
             be.rows_swiglu_bf16(B["gu"], m, F, B["act"])
             be.gemm(L["down"], B["act"], m, B["x"], accumulate=True)
         be.gemv(self.out, B["x"] + 4 * (m - 1) * H, self.logits, rmsnorm=self.out_norm, eps=c.eps)
+
+    def _prefill_i8_bufs(self):
+        if self._pf8 is None:
+            c, C = self.cfg, self.PREFILL_CHUNK
+            H, F, qd, kd = c.hidden_size, c.ffn_size, self.qd, self.kd
+            self._pf8 = {"x": self._buf(C * H), "codes": self._buf(C * max(H, F, qd) // 4), "scale": self._buf(C),
+                         "qkv": self._buf(C * (qd + 2 * kd) // 2), "ao": self._buf(C * qd),
+                         "ao16": self._buf(C * qd // 2), "act": self._buf(C * F // 2), "delta": self._buf(C * H // 2)}
+        return self._pf8
+
+    def prefill_composed_i8(self, tokens, pos: int):
+        """The sequence of hymt_model_prefill with HYMT_PREFILL_INT8 for one
+        chunk, as separate C ABI calls (a model loaded with int8):
+            per layer l:
+                X += D (but in the first layer); X8 = codes of RMSNorm(X, attn_norm)   hymt_rows_rmsnorm_i8
+                [Q|K|V] = X8 . [Wq; Wk; Wv]^T (bf16)                                   hymt_gemm_i8 OUT_BF16
+                AO = causal attention; A8 = codes of bf16(AO)          hymt_attn_prefill_ld, hymt_to_i8
+                D = A8 . Wo^T (bf16)                                                   hymt_gemm_i8 OUT_BF16
+                X += D; X8 = codes of RMSNorm(X, ffn_norm)                             hymt_rows_rmsnorm_i8
+                act = silu(X8 . Wgate^T) * (X8 . Wup^T) (bf16)                         hymt_gemm_i8_swiglu
+                D = codes of act . Wdown^T (bf16; of the last layer onto X)            hymt_to_i8, hymt_gemm_i8
+        """
+        be, c, B = self.be, self.cfg, self._prefill_i8_bufs()
+        m, H, F, qd, kd = len(tokens), c.hidden_size, c.ffn_size, self.qd, self.kd
+        assert 0 < m <= self.PREFILL_CHUNK
+        x, codes, scale, qkv, delta = B["x"], B["codes"], B["scale"], B["qkv"], B["delta"]
+        ld = qd + 2 * kd
+
+        def product(w, y, ldy, **kw):
+            (q, s), info = be.weight_i8_data(w), be.weight_info(w)
+            be.gemm_i8(q, s, info["rows"], info["cols"], codes, scale, m, y, ldy, **kw)
+
+        be.embed_rows(self.embd, tokens, x)
+        for l, L in enumerate(self.layers):
+            be.rows_rmsnorm_i8(x, m, H, L["attn_norm"], c.eps, codes, scale, add=delta if l else None)
+            for w, off in zip(L["qkv"], (0, qd, qd + kd)):
+                product(w, qkv + 2 * off, ld, out_bf16=True)
+            be.prefill_dev_ld(l, pos, m, qkv, ld, qkv + 2 * qd, qkv + 2 * (qd + kd), ld, N.BF16, L["q_norm"],
+                              L["k_norm"], B["ao"])
+            be.to_bf16(B["ao"], m * qd, B["ao16"])  # the attention of the one-call prefill writes bf16
+            be.to_i8(B["ao16"], m, qd, codes, scale, x_dtype=N.BF16)
+            product(L["o"], delta, H, out_bf16=True)
+            be.rows_rmsnorm_i8(x, m, H, L["ffn_norm"], c.eps, codes, scale, add=delta)
+            gu = [be.weight_i8_data(w) for w in L["gate_up"]]
+            (g, gs), (u, us) = gu if len(gu) == 2 else (gu[0], (gu[0][0] + F * H, gu[0][1] + 4 * F))
+            be.gemm_i8_swiglu(g, gs, u, us, F, H, codes, scale, m, B["act"])
+            be.to_i8(B["act"], m, F, codes, scale, x_dtype=N.BF16)
+            if l + 1 < c.num_layers:
+                product(L["down"], delta, H, out_bf16=True)
+            else:
+                product(L["down"], x, H, accumulate=True)
+        be.gemv(self.out, x + 4 * (m - 1) * H, self.logits, rmsnorm=self.out_norm, eps=c.eps)
 
     def forward(self, tokens, pos: int) -> np.ndarray:
         """ForwardStep (IComputeBackend.cs:40-47): the tokens at positions

@@ -232,8 +232,9 @@ int hymt_sync(hymt_ctx *ctx);
  * over the calls timed since creation or hymt_timing_reset; HYMT_E_STATE when
  * the context does not time, HYMT_E_ARG for a kernel never timed.  Kernel
  * names: decode_attn, decode_merge, prefill_kv, prefill_flash, prefill_merge,
- * gemv_<type>, gemm_bf16_out_{f32,bf16}, rows_*, kv_*, embed, weight_rows,
- * tab_update, graph (a whole replay).
+ * gemv_<type>, gemm_bf16_out_{f32,bf16}, gemm_i8_out_{f32,bf16},
+ * gemm_i8_swiglu, to_i8, rows_*, kv_*, embed, weight_rows, tab_update, graph
+ * (a whole replay).
  */
 /* mode 0 stops timing (the totals are kept), 1 times and prints, 2 times
  * quietly; a device context only (HYMT_E_NO_DEVICE otherwise). */
@@ -495,6 +496,17 @@ int hymt_model_decode(hymt_model *model, int token, int pos, float *logits);
  * tokens is a host array (read before the call returns); logits a device
  * pointer (vocab floats, the last token's).  Not recordable. */
 #define HYMT_PREFILL_GATE_UP_F32 1u
+/* The same over the layer weights' int8 codes (hymt_weight_i8, else
+ * HYMT_E_STATE; no dense copies needed), every product in 8-bit integers:
+ *   per layer: X8 = codes of RMSNorm(X, attn_norm); [Q|K|V] = X8 W_qkv^T (bf16)
+ *              AO as above (bf16); D = codes(AO) W_o^T (bf16)
+ *              X += D; X8 = codes of RMSNorm(X, ffn_norm)
+ *              act = silu(X8 W_gate^T) * (X8 W_up^T) (bf16)
+ *              X += codes(act) W_down^T (rounded to bf16, of the last layer fp32)
+ * i.e. hymt_rows_rmsnorm_i8, hymt_gemm_i8, hymt_to_i8 and hymt_gemm_i8_swiglu.
+ * Excludes HYMT_PREFILL_GATE_UP_F32; ffn up to 8192.  n = 1 or an fp32 cache run
+ * as decode steps over the quantized weights. */
+#define HYMT_PREFILL_INT8 2u
 int hymt_model_prefill(hymt_model *model, const int32_t *tokens, int n, int pos, float *logits,
                        unsigned flags);
 int hymt_model_destroy(hymt_model *model);
