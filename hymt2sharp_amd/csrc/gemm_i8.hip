@@ -21,6 +21,8 @@ namespace hymt {
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 enum Out { kF32, kAcc, kBf16, kGlu };
 
@@ -54,8 +56,10 @@ __device__ __forceinline__ float scaled(int s, float ws) { return (float)s * ws;
 __device__ __forceinline__ float glu(int g, int u, float ws, float us, float xs) {
     return silu_fast(scaled(g, ws) * xs) * (scaled(u, us) * xs);
 }
+// bf16, rounded to nearest even by v_cvt_pk_bf16_f32; a NaN stays one whatever its
+// bits (a token's scale may be any NaN)
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
-    return (uint32_t)f32_to_bf16(a) | ((uint32_t)f32_to_bf16(b) << 16);
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
 }
 
 // Features f .. f + 3 of token t from the sums, where f + e < n.
@@ -75,7 +79,7 @@ __device__ __forceinline__ void store4(const Args &a, int t, int f, i32x4 s, i32
         } else {
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                if (f + e < g.n) y[e] = f32_to_bf16(v[e]);
+                if (f + e < g.n) y[e] = (uint16_t)pack2(v[e], 0.f);
         }
     } else {
         float *y = (float *)g.y + at;

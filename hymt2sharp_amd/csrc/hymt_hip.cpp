@@ -1760,7 +1760,6 @@ int hymt_model_prefill(hymt_model *m, const int32_t *tokens, int n, int pos, flo
         return fail(HYMT_E_ARG, "HYMT_PREFILL_INT8 and HYMT_PREFILL_GATE_UP_F32 exclude each other");
     if (int8 && !prefill_i8_ready(m))
         return fail(HYMT_E_STATE, "a layer weight has no int8 codes (hymt_weight_i8)");
-    if (int8 && m->ffn > 8192) return fail(HYMT_E_UNSUPPORTED, "HYMT_PREFILL_INT8 takes rows of up to 8192 values");
     if (n < 1 || !tokens) return fail(HYMT_E_ARG, "empty token list");
     for (int i = 0; i < n; i++)
         if (tokens[i] < 0 || tokens[i] >= m->vocab) return fail(HYMT_E_ARG, "token out of range");

@@ -504,8 +504,8 @@ int hymt_model_decode(hymt_model *model, int token, int pos, float *logits);
  *              act = silu(X8 W_gate^T) * (X8 W_up^T) (bf16)
  *              X += codes(act) W_down^T (rounded to bf16, of the last layer fp32)
  * i.e. hymt_rows_rmsnorm_i8, hymt_gemm_i8, hymt_to_i8 and hymt_gemm_i8_swiglu.
- * Excludes HYMT_PREFILL_GATE_UP_F32; ffn up to 8192.  n = 1 or an fp32 cache run
- * as decode steps over the quantized weights. */
+ * Excludes HYMT_PREFILL_GATE_UP_F32.  n = 1 or an fp32 cache run as decode
+ * steps over the quantized weights. */
 #define HYMT_PREFILL_INT8 2u
 int hymt_model_prefill(hymt_model *model, const int32_t *tokens, int n, int pos, float *logits,
                        unsigned flags);

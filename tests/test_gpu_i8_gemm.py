@@ -151,13 +151,15 @@ def test_a_row_has_the_same_bits_in_every_call(be, out, n, k):
 
 
 def test_nan_and_zero_scales_stay_in_their_rows(be):
-    """A token's NaN scale (a row with a NaN before the quantiser) makes its
-    outputs NaN and no others; zero codes or scales give zeros."""
+    """A token's NaN scale (a row with a NaN before the quantiser), also one of
+    all ones, makes its outputs NaN and no others; zero codes or scales give
+    zeros."""
     n, k = 300, 512
-    for m in (3, 90):
+    for m, bits in ((3, 0x7FC00000), (90, 0xFFFFFFFF), (3, 0x7FFFFFFF)):
         w, x = codes(1, n, k), codes(2, m, k)
         ws, xs = scales(3, n), scales(4, m)
-        xs[1], x[1] = np.nan, 0
+        x[1] = 0
+        xs.view(np.uint32)[1] = bits
         xs[2] = 0
         ws[7] = 0
         for out in ("f32", "bf16", "glu"):

@@ -153,6 +153,29 @@ def test_no_rows(be):
     r.close()
 
 
+def test_more_rows_than_one_launch_takes(be):
+    """Row counts past the 2^23 of one launch: the rows on either side of the
+    border, and the last ones."""
+    m, n = (1 << 23) + 6, 4
+    x = np.random.default_rng(1).standard_normal((m, n)).astype(np.float32)
+    d = bf16_bits(np.random.default_rng(2).standard_normal((m, n)))
+    w = np.array([1, 0.5, -2, 1], np.float32)
+    r = Room(be)
+    dx, dd, dw = r.put(x), r.put(d), r.put(w)
+    dq, ds = r.put(np.zeros((m, n), np.int8)), r.put(np.zeros(m, np.float32))
+    at = np.r_[0:8, (1 << 23) - 8:m]
+    be.to_i8(dx, m, n, dq, ds)
+    q, a = codes_of(x[at])
+    check(be, r.get(dq, np.empty((m, n), np.int8))[at], r.get(ds, np.empty(m, np.float32))[at], q,
+          (a / 127.0).astype(np.float32).astype(np.float64), 0.0)
+    be.rows_rmsnorm_i8(dx, m, n, dw, 1e-5, dq, ds, add=dd)
+    h, q, s = norm_rows(x[at], bf16_val(d[at]), w, 1e-5)
+    np.testing.assert_array_equal(r.get(dx, x)[at], h)
+    check(be, r.get(dq, np.empty((m, n), np.int8))[at], r.get(ds, np.empty(m, np.float32))[at], q, s,
+          U32 * (1 + 2.0 ** -10))
+    r.close()
+
+
 @pytest.mark.parametrize("wtype,rows_,cols", [(N.W_Q4_K, 40, 2048), (N.W_Q6_K, 17, 6144), (N.W_Q8_0, 5, 4096),
                                               (N.W_F32, 9000, 2048), (N.W_F16, 3, 8192)])
 def test_weight_i8(be, wtype, rows_, cols):
