@@ -5,6 +5,19 @@
 //
 // The sum is exact, so its order is free: every kernel and tile below gives the
 // same bits, and which one runs is a matter of time alone.
+//
+// What it takes (us, in a recording; the floor is the bytes at 5.05 TB/s or the
+// operations at 2058 TOP/s, what a large copy and a large int8 product reach, and
+// 1.8 for a launch):
+//   tokens x channels x k      output       floor    here   rate
+//   1 x 2048 x 2048            fp32           2.6     2.9
+//   1 x 120818 x 2048          fp32          50.8    44.5   5.6 TB/s
+//   61 x 2048 x 6144           fp32 +=        4.6     6.3   2.1 TB/s
+//   700 x 2048 x 6144          bf16          10.4    16.8   1050 TOP/s
+//   2048 x 2048 x 2048         bf16          10.1    12.0   1440
+//   2048 x 2048 x 6144         fp32          26.8    27.9   1850
+//   61 x 2 6144 x 2048         SwiGLU         6.9     8.2   3.2 TB/s
+//   2048 x 2 6144 x 2048       SwiGLU        51.9    49.5   2080 TOP/s
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -566,32 +579,33 @@ __global__ __launch_bounds__(256) void skinny_kernel(Args a) {
 // few-token kernel's, and what a launch of `tiles` of them takes: us =
 //   launch + R (round + stage kt) + F (fill + fill_stage kt),
 // R = ceil(tiles / 256) rounds of the chip, F = tiles / 256 (what grows with the traffic of
-// all CUs together), kt = k / 128.  Fitted to 955 measurements: 1-4096 tokens, 64-120818
+// all CUs together), kt = k / 128.  Fitted to 1500 measurements: 1-4096 tokens, 64-120818
 // channels, k 256-8192, every output; the tile of the least estimate takes 0.5 %
 // longer on average than the fastest one (worst 31 %: 2555 x 128 x 512).  E.g., us
-// estimated / measured: 2048 x 2048 x 2048 bf16 128 x 128 14.5 / 12.9, 128 x 64 18.5 / 16.2, 192 x
-// 256 23.7 / 22.1; 61 x 2048 x 6144 fp32 32 x 16 6.4 / 6.5, 32 x 32 6.6 / 7.6.
+// estimated / measured: 2048 x 2048 x 2048 bf16 128 x 128 14.0 / 12.6, 128 x 64 18.2 / 16.0;
+// 61 x 2048 x 6144 fp32 32 x 16 6.1 / 6.5, 32 x 32 6.5 / 7.5.  (It knows nothing of HBM: one
+// token of 120818 channels takes 44 us, not 20; the order of the tiles holds.)
 struct Shape {
     const char *name;
     int f, t, threads;
     float launch, round, stage, fill, fill_stage;
 };
 constexpr Shape kShapes[] = {
-    {"16x16", 16, 16, 256, 2.40f, 0.26f, 0.027f, 0.08f, 0.021f},
-    {"32x16", 32, 16, 256, 2.56f, 0.19f, 0.042f, 0.17f, 0.030f},
-    {"48x16", 48, 16, 256, 2.80f, 0.00f, 0.056f, 0.37f, 0.038f},
-    {"64x16", 64, 16, 256, 2.88f, 0.00f, 0.075f, 0.40f, 0.040f},
-    {"32x32", 32, 32, 256, 2.58f, 0.28f, 0.055f, 0.17f, 0.044f},
-    {"64x32", 64, 32, 256, 2.17f, 1.08f, 0.092f, 0.40f, 0.074f},
-    {"64x64", 64, 64, 256, 2.01f, 2.05f, 0.132f, 0.38f, 0.105f},
-    {"96x64", 96, 64, 256, 2.34f, 2.48f, 0.194f, 0.96f, 0.114f},
-    {"128x64", 128, 64, 256, 2.86f, 0.48f, 0.250f, 1.98f, 0.085f},
-    {"128x96", 128, 96, 256, 2.66f, 1.54f, 0.277f, 1.71f, 0.103f},
-    {"128x128", 128, 128, 256, 3.24f, 1.46f, 0.344f, 2.37f, 0.118f},
-    {"192x128", 192, 128, 512, 3.33f, 2.03f, 0.417f, 3.09f, 0.237f},
-    {"256x128", 256, 128, 256, 4.82f, 1.60f, 0.604f, 4.78f, 0.210f},
-    {"192x256", 192, 256, 512, 5.15f, 1.26f, 0.865f, 6.43f, 0.230f},
-    {"256x256", 256, 256, 512, 8.01f, 0.68f, 0.944f, 7.05f, 0.433f},
+    {"16x16", 16, 16, 256, 2.41f, 0.24f, 0.028f, 0.11f, 0.018f},
+    {"32x16", 32, 16, 256, 2.55f, 0.17f, 0.044f, 0.23f, 0.022f},
+    {"48x16", 48, 16, 256, 2.74f, 0.02f, 0.059f, 0.43f, 0.028f},
+    {"64x16", 64, 16, 256, 2.81f, 0.05f, 0.078f, 0.43f, 0.029f},
+    {"32x32", 32, 32, 256, 2.57f, 0.25f, 0.058f, 0.25f, 0.035f},
+    {"64x32", 64, 32, 256, 2.17f, 1.07f, 0.096f, 0.51f, 0.059f},
+    {"64x64", 64, 64, 256, 2.21f, 1.79f, 0.143f, 0.73f, 0.076f},
+    {"96x64", 96, 64, 256, 2.38f, 2.40f, 0.212f, 1.25f, 0.064f},
+    {"128x64", 128, 64, 256, 2.82f, 0.45f, 0.269f, 1.98f, 0.060f},
+    {"128x96", 128, 96, 256, 2.59f, 1.51f, 0.303f, 1.69f, 0.074f},
+    {"128x128", 128, 128, 256, 2.81f, 1.92f, 0.366f, 1.88f, 0.095f},
+    {"192x128", 192, 128, 512, 3.33f, 2.09f, 0.435f, 3.01f, 0.199f},
+    {"256x128", 256, 128, 256, 4.33f, 2.41f, 0.620f, 3.81f, 0.178f},
+    {"192x256", 192, 256, 512, 4.54f, 2.11f, 0.852f, 5.12f, 0.283f},
+    {"256x256", 256, 256, 512, 7.16f, 0.58f, 0.979f, 6.97f, 0.417f},
 };
 constexpr int kNumShapes = sizeof(kShapes) / sizeof(kShapes[0]);
 constexpr size_t kMaxTiles = 1u << 22;  // of a launch: a grid holds less than 2^32 threads

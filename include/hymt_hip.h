@@ -433,9 +433,9 @@ int hymt_rows_rmsnorm_i8(hymt_ctx *ctx, float *x, const void *add, int add_dtype
  * channels, w [n][k] and x [m][k] int8 (-128 too).  The sum is exact, and fp32
  * is multiplied by w_scale, then by x_scale, so the result does not depend on the
  * kernel or on m.  y is fp32, rows ldy >= n elements apart, or as the flags
- * say: HYMT_GEMM_ACCUMULATE y += in fp32, HYMT_GEMM_OUT_BF16 bf16.  k a
- * multiple of 128, 256 to 65536; w and x 16-byte aligned, y and the scales by
- * their elements. */
+ * say: HYMT_GEMM_ACCUMULATE y += in fp32 (fused with the last product),
+ * HYMT_GEMM_OUT_BF16 bf16.  k a multiple of 128, 256 to 65536; up to 2^30 tokens
+ * and channels; w and x 16-byte aligned, y and the scales by their elements. */
 int hymt_gemm_i8(hymt_ctx *ctx, const int8_t *w, const float *w_scale, int n, int k, const int8_t *x,
                  const float *x_scale, int m, void *y, int ldy, int flags);
 

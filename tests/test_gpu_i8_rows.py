@@ -153,6 +153,38 @@ def test_no_rows(be):
     r.close()
 
 
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -60, 2.0 ** -100, 2.0 ** 110])
+def test_codes_next_to_a_border(be, size):
+    """Rows of values within two fp32 steps of every border between two codes,
+    of many maxima, in the ranges of both ways to the code."""
+    rng = np.random.default_rng(5)
+    m, n = 300, 5 * 254 + 2
+    a = (rng.uniform(1, 2, m) * size).astype(np.float32)
+    mid = (a[:, None].astype(np.float64) * (2 * np.arange(-127, 127) + 1) / 254).astype(np.float32)
+    x = np.zeros((m, n), np.float32)
+    steps = [mid]
+    for to in (np.inf, -np.inf):
+        one = np.nextafter(mid, np.float32(to))
+        steps += [one, np.nextafter(one, np.float32(to))]
+    x[:, :5 * 254] = np.concatenate(steps, 1)
+    x[:, -2] = a
+    x = np.where(np.abs(x) > a[:, None], np.copysign(a[:, None], x), x)
+    w = rng.uniform(0.5, 1.5, n).astype(np.float32)
+    near = rng.uniform(0.5, 1.5, (m, 1)).astype(np.float32) * x  # times w: other borders
+    r = Room(be)
+    dx, dn, dw = r.put(x), r.put(near), r.put(w)
+    dq, ds = r.put(np.zeros((m, n), np.int8)), r.put(np.zeros(m, np.float32))
+    be.to_i8(dx, m, n, dq, ds)
+    q, a = codes_of(x)
+    check(be, r.get(dq, np.empty((m, n), np.int8)), r.get(ds, np.empty(m, np.float32)), q,
+          (a / 127.0).astype(np.float32).astype(np.float64), 0.0)
+    be.rows_rmsnorm_i8(dn, m, n, dw, 0.0, dq, ds)
+    np.testing.assert_array_equal(r.get(dq, np.empty((m, n), np.int8)), norm_rows(near, None, w, 0.0)[1])
+    be.rows_rmsnorm_i8(dx, m, n, r.put(np.ones(n, np.float32)), 0.0, dq, ds)  # the same borders through the norm
+    np.testing.assert_array_equal(r.get(dq, np.empty((m, n), np.int8)), q)
+    r.close()
+
+
 def test_more_rows_than_one_launch_takes(be):
     """Row counts past the 2^23 of one launch: the rows on either side of the
     border, and the last ones."""
