@@ -13,11 +13,11 @@
 //   1 x 2048 x 2048            fp32           2.6     2.9
 //   1 x 120818 x 2048          fp32          50.8    44.5   5.6 TB/s
 //   61 x 2048 x 6144           fp32 +=        4.6     6.3   2.1 TB/s
-//   700 x 2048 x 6144          bf16          10.4    16.8   1050 TOP/s
-//   2048 x 2048 x 2048         bf16          10.1    12.0   1440
-//   2048 x 2048 x 6144         fp32          26.8    27.9   1850
-//   61 x 2 6144 x 2048         SwiGLU         6.9     8.2   3.2 TB/s
-//   2048 x 2 6144 x 2048       SwiGLU        51.9    49.5   2080 TOP/s
+//   700 x 2048 x 6144          bf16          10.4    15.4   1140 TOP/s
+//   2048 x 2048 x 2048         bf16          10.1    12.0   1430
+//   2048 x 2048 x 6144         fp32          26.8    27.5   1870
+//   61 x 2 6144 x 2048         SwiGLU         6.9     7.5   3.5 TB/s
+//   2048 x 2 6144 x 2048       SwiGLU        51.9    47.6   2170 TOP/s
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -125,6 +125,14 @@ __device__ __forceinline__ void store4(const Args &a, int t, int f, i32x4 s, i32
 // stage's copies between them.  The bytes moved, the LDS reads and the MFMA cycles
 // of a stage are those of a bf16 stage of 64 k, for twice the k.
 //
+// KG = 2: two groups of waves take every other stage, each through a ring of its
+// own, two waves a SIMD: one wave's copies, which hold its issue for about 50
+// cycles each, run under the other's MFMAs.  Their sums meet in LDS at the end.
+// Taken for the tiles whose two rings fit (us, one group / two, bf16: 128 x 64 over
+// 1024 x 2048 x 6144 18.6 / 17.4; few-token kernel / two groups: 64 x 64 over 300 x
+// 2048 x 2048 6.4 / 5.2, 96 x 64 over 700 x 2048 x 6144 16.3 / 15.1; 128 x 128, whose
+// rings then hold two stages each, 12.0 / 13.7 over 2048 x 2048 x 2048).
+//
 // SwiGLU: the tile holds TF / 2 outputs, of a wave's IF row blocks the first half
 // gate rows and the others the same rows of up, so that g and u of an output
 // meet in one lane's registers.
@@ -180,11 +188,12 @@ __device__ __forceinline__ void substep(i32x4 (&w)[IF], const i32x4 (&cx)[BJ], c
 // after its last operand reads (each wave first waits for its own reads), so
 // S - 1 stages are ahead of the one being read; else one barrier later, with
 // S - 2 ahead and no wait on the reads.
-template <int IF, int JT, int WT, int S, bool LGKM, int OUT>
-__global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
+template <int IF, int JT, int WT, int S, bool LGKM, int KG, int OUT>
+__global__ __launch_bounds__(128 * WT * KG, 1) void tile_kernel(Args a) {
     constexpr bool GLU = OUT == kGlu;
     constexpr int TF = 32 * IF, TT = 32 * JT;
-    constexpr int NW = 2 * WT, NT = 64 * NW, BJ = TT / (16 * WT);  // waves, threads, token blocks per wave
+    constexpr int NW = 2 * WT, NT = 64 * NW * KG, BJ = TT / (16 * WT);  // waves of a k group, threads, token blocks per wave
+    constexpr int BE = BJ / KG;                                          // ... that a wave writes
     constexpr int NBF = TF / 16, NB = (TF + TT) / 16;               // row blocks: W, all
     constexpr int C = 2 * NB / NW;                                   // copy instructions per wave per stage
     constexpr int kStageBytes = NB * kPair;
@@ -196,17 +205,22 @@ __global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
     // after the loop: the scales, then each wave's bf16 rows (16 bytes of
     // padding each), all its token blocks at once where they fit
     constexpr int NS = TF + TT, kStageAt = NS * 4, RS = 16 * OI + 8;
-    constexpr int JB = kStageAt + NW * BJ * 16 * RS * 2 <= S * kStageBytes ? BJ : BJ / 2;
-    static_assert(kStageAt % 16 == 0 && kStageAt + NW * JB * 16 * RS * 2 <= S * kStageBytes && BJ % JB == 0, "epilogue");
-    static_assert(S * kStageBytes <= 160 * 1024, "LDS");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[S * kStageBytes];
+    constexpr int kRing = S * kStageBytes, kLds = KG * kRing;
+    constexpr int JB = kStageAt + NW * KG * BE * 16 * RS * 2 <= kLds ? BE : BE / 2;
+    static_assert(kStageAt % 16 == 0 && kStageAt + NW * KG * JB * 16 * RS * 2 <= kLds && BE % JB == 0, "epilogue");
+    static_assert(kLds <= 160 * 1024 && BJ % KG == 0 && (KG == 1 || KG * NW * IF * BE * 1024 <= kLds), "LDS");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kg = KG == 1 ? 0 : wave / NW, wg = KG == 1 ? wave : wave % NW;  // k group, wave of it
     const int grp = lane >> 4, c = lane & 15;
     const I8Gemm &g = a.g;
     int tf, tt;
     if (!tile_of(a, tf, tt)) return;
-    const int f0 = tf * OF, t0 = tt * TT, kt = g.k / kBK;
+    const int f0 = tf * OF, t0 = tt * TT, stages = g.k / kBK;
+    // a group's stages: kg, kg + KG, ..., of which the last may lie past the end
+    const int kt = (stages + KG - 1) / KG;
+    const bool last = KG == 1 || KG * (kt - 1) + kg < stages;
 
     // The scales of the tile's features (gate, then up) and tokens, one or two a
     // thread, loaded here and handed over through LDS once the ring is idle.
@@ -232,7 +246,7 @@ __global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
     const int8_t *xt0 = g.x + (size_t)t0 * g.k;
 #pragma unroll
     for (int j = 0; j < C; j++) {
-        const int l = wave * C + j, gb = l >> 1, h = l & 1;
+        const int l = wg * C + j, gb = l >> 1, h = l & 1;
         const int ga = 8 * h + (lane >> 3);
         const int rl = (ga >> 1) + 8 * (ga & 1);
         const int piece = (lane & 7) ^ (ga >> 1);
@@ -243,12 +257,13 @@ __global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
         voff[j] = (uint32_t)row * (uint32_t)g.k + 16 * piece;
         sbase[j] = !isw ? xt0 : GLU && i >= OI ? ut0 : wt0;
     }
-    const uint32_t lds0 = lds_addr(lds) + wave * C * kFrag;
+    uint8_t *const ring = lds + kg * kRing;
+    const uint32_t lds0 = lds_addr(lds) + kg * kRing + wg * C * kFrag;
     // copy j of stage t into its ring slot t % S.  Stages past the last copy the
     // last stage's rows again: their slots are never read, every iteration issues
     // C copies, and the waits and the loop have no branch.
     auto copy = [&](int t, int j) __attribute__((always_inline)) {
-        lds_dma16_sv(sbase[j] + min(t, kt - 1) * kBK, voff[j], lds0 + (t % S) * kStageBytes + j * kFrag);
+        lds_dma16_sv(sbase[j] + min(KG * t + kg, stages - 1) * kBK, voff[j], lds0 + (t % S) * kStageBytes + j * kFrag);
     };
     // A stage's copies are spread over the MFMA rows of two steps: [0, CB) in
     // the step after the barrier that frees its slot, [CB, C) in the next one
@@ -275,7 +290,7 @@ __global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
         off[ks] = 16 * (16 * r + 8 * i + ((4 * ks + grp) ^ r));
     }
 
-    const int wf = wave & 1, wt = wave >> 1;
+    const int wf = wg & 1, wt = wg >> 1;
     i32x4 acc[IF][BJ];
 #pragma unroll
     for (int i = 0; i < IF; i++)
@@ -294,30 +309,59 @@ __global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
     asm volatile("s_barrier" ::: "memory");
     i32x4 w[IF], ax[BJ], bx[BJ];
 #pragma unroll
-    for (int i = 0; i < IF; i++) w[i] = *(const i32x4 *)(lds + off[0] + (IF * wf + i) * kPair);
+    for (int i = 0; i < IF; i++) w[i] = *(const i32x4 *)(ring + off[0] + (IF * wf + i) * kPair);
 #pragma unroll
-    for (int j = 0; j < BJ; j++) ax[j] = *(const i32x4 *)(lds + off[0] + (NBF + BJ * wt + j) * kPair);
+    for (int j = 0; j < BJ; j++) ax[j] = *(const i32x4 *)(ring + off[0] + (NBF + BJ * wt + j) * kPair);
 
     // The last stage is peeled, so that the accumulators meet no branch.
     for (int s = 0; s < kt - 1; s++) {
         // step (s, 0): its operands in (w, ax); read step (s, 1) into (w, bx);
         // the second half of stage s - 1 + AHEAD
-        substep<IF, BJ>(w, ax, lds + (s % S) * kStageBytes, off[1], wf, wt, bx, acc, second_half(s - 1 + AHEAD));
+        substep<IF, BJ>(w, ax, ring + (s % S) * kStageBytes, off[1], wf, wt, bx, acc, second_half(s - 1 + AHEAD));
         // stage s + 1 landed: AHEAD - 2 later ones may stay in flight
         wait_vm<C * (AHEAD - 2), LGKM>();
         asm volatile("s_barrier" ::: "memory");
         // step (s, 1): operands in (w, bx); read step (s + 1, 0) into (w, ax);
         // the first half of stage s + AHEAD
-        substep<IF, BJ>(w, bx, lds + ((s + 1) % S) * kStageBytes, off[0], wf, wt, ax, acc, first_half(s + AHEAD));
+        substep<IF, BJ>(w, bx, ring + ((s + 1) % S) * kStageBytes, off[0], wf, wt, ax, acc, first_half(s + AHEAD));
     }
-    substep<IF, BJ>(w, ax, lds + ((kt - 1) % S) * kStageBytes, off[1], wf, wt, bx, acc, [](int) {});
+    if (last) {
+        substep<IF, BJ>(w, ax, ring + ((kt - 1) % S) * kStageBytes, off[1], wf, wt, bx, acc, [](int) {});
 #pragma unroll
-    for (int i = 0; i < IF; i++)
+        for (int i = 0; i < IF; i++)
 #pragma unroll
-        for (int j = 0; j < BJ; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], bx[j], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < BJ; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], bx[j], acc[i][j], 0, 0, 0);
+    }
     wait_vm<0>();     // the copies past the last stage have landed before the ring is reused or freed
     __syncthreads();  // every wave's operand reads are done
 
+    // The groups' sums meet: of the token blocks of a wave and the wave of the
+    // other group over the same ones each hands the other half over and writes
+    // its own.
+    i32x4 sum[IF][BE];
+    if constexpr (KG == 1) {
+#pragma unroll
+        for (int i = 0; i < IF; i++)
+#pragma unroll
+            for (int j = 0; j < BE; j++) sum[i][j] = acc[i][j];
+    } else {
+        static_assert(KG == 2, "two groups");
+        i32x4 *mine = (i32x4 *)lds + (size_t)wave * IF * BE * 64 + lane;
+        const i32x4 *others = (const i32x4 *)lds + (size_t)(wave ^ NW) * IF * BE * 64 + lane;
+#pragma unroll
+        for (int i = 0; i < IF; i++)
+#pragma unroll
+            for (int j = 0; j < BE; j++) {
+                mine[(i * BE + j) * 64] = kg ? acc[i][j] : acc[i][BE + j];
+                sum[i][j] = kg ? acc[i][BE + j] : acc[i][j];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < IF; i++)
+#pragma unroll
+            for (int j = 0; j < BE; j++) sum[i][j] += others[(i * BE + j) * 64];
+        __syncthreads();
+    }
     float *scales = (float *)lds;
 #pragma unroll
     for (int p = 0; p < PS; p++)
@@ -327,9 +371,9 @@ __global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
     // Each wave writes its own part of the tile, a block of 16 tokens at a time.
     // chunks: the output's rows are whole 16-byte chunks, which are inside it or
     // not; whole: the part lies inside the output (its writes have no branch).
-    const int fw = f0 + (OF / 2) * wf, tw = t0 + (TT / WT) * wt;
+    const int fw = f0 + (OF / 2) * wf, tl = (TT / WT) * wt + 16 * BE * kg, tw = t0 + tl;
     const bool chunks = a.vec && g.n % (OUT == kBf16 || GLU ? 8 : 4) == 0;
-    const bool whole = a.vec && fw + OF / 2 <= g.n && tw + TT / WT <= g.m;
+    const bool whole = a.vec && fw + OF / 2 <= g.n && tw + 16 * BE <= g.m;
     float4 ws[OI], us[GLU ? OI : 1];
 #pragma unroll
     for (int i = 0; i < OI; i++) {
@@ -342,17 +386,17 @@ __global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
         constexpr int CPR = 2 * OI, NQ = JB * 16 * CPR;  // 16-byte chunks of a row, of a batch
         uint16_t *st = (uint16_t *)(lds + kStageAt) + wave * JB * 16 * RS;
 #pragma unroll
-        for (int j0 = 0; j0 < BJ; j0 += JB) {
+        for (int j0 = 0; j0 < BE; j0 += JB) {
             asm volatile("" ::: "memory");  // the rows change hands between the wave's lanes
 #pragma unroll
             for (int j = j0; j < j0 + JB; j++) {
-                const float xs = scales[TF + (TT / WT) * wt + 16 * j + c];
+                const float xs = scales[TF + tl + 16 * j + c];
 #pragma unroll
                 for (int i = 0; i < OI; i++) {
-                    const i32x4 v = acc[i][j];
+                    const i32x4 v = sum[i][j];
                     float o[4];
                     if constexpr (GLU) {
-                        const i32x4 u = acc[i + OI][j];
+                        const i32x4 u = sum[i + OI][j];
                         o[0] = glu(v[0], u[0], ws[i].x, us[i].x, xs);
                         o[1] = glu(v[1], u[1], ws[i].y, us[i].y, xs);
                         o[2] = glu(v[2], u[2], ws[i].z, us[i].z, xs);
@@ -392,8 +436,8 @@ __global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
                 return decltype(all)::value || (tw + 16 * j + c < g.m && fw + 16 * i + 4 * grp < g.n);
             };
 #pragma unroll
-            for (int j = 0; j < BJ; j++) {
-                const float xs = scales[TF + (TT / WT) * wt + 16 * j + c];
+            for (int j = 0; j < BE; j++) {
+                const float xs = scales[TF + tl + 16 * j + c];
                 float4 old[OUT == kAcc ? IF : 1];
                 if constexpr (OUT == kAcc)
 #pragma unroll
@@ -401,7 +445,7 @@ __global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
                         if (inside(i, j)) old[i] = *(const float4 *)(y + j * step + 16 * i);
 #pragma unroll
                 for (int i = 0; i < IF; i++) {
-                    const i32x4 v = acc[i][j];
+                    const i32x4 v = sum[i][j];
                     const float o[4] = {scaled(v[0], ws[i].x), scaled(v[1], ws[i].y), scaled(v[2], ws[i].z),
                                         scaled(v[3], ws[i].w)};
                     float4 r = make_float4(o[0] * xs, o[1] * xs, o[2] * xs, o[3] * xs);
@@ -416,14 +460,14 @@ __global__ __launch_bounds__(128 * WT, 1) void tile_kernel(Args a) {
         else write(std::false_type{});
     } else {
 #pragma unroll
-        for (int j = 0; j < BJ; j++) {
+        for (int j = 0; j < BE; j++) {
             const int t = tw + 16 * j + c;
             if (t >= g.m) continue;
-            const float xs = scales[TF + (TT / WT) * wt + 16 * j + c];
+            const float xs = scales[TF + tl + 16 * j + c];
 #pragma unroll
             for (int i = 0; i < OI; i++) {
                 const float w4[4] = {ws[i].x, ws[i].y, ws[i].z, ws[i].w};
-                store4<OUT>(a, t, fw + 16 * i + 4 * grp, acc[i][j], acc[i][j], w4, w4, xs);
+                store4<OUT>(a, t, fw + 16 * i + 4 * grp, sum[i][j], sum[i][j], w4, w4, xs);
             }
         }
     }
@@ -575,37 +619,40 @@ __global__ __launch_bounds__(256) void skinny_kernel(Args a) {
 
 // ---- which kernel --------------------------------------------------------------
 
-// The tiles: features x tokens (SwiGLU: half as many outputs), the first 8 the
-// few-token kernel's, and what a launch of `tiles` of them takes: us =
+// The tiles: features x tokens (SwiGLU: half as many outputs) and what a launch
+// of `tiles` of them takes, us =
 //   launch + R (round + stage kt) + F (fill + fill_stage kt),
 // R = ceil(tiles / 256) rounds of the chip, F = tiles / 256 (what grows with the traffic of
-// all CUs together), kt = k / 128.  Fitted to 1500 measurements: 1-4096 tokens, 64-120818
+// all CUs together), kt = k / 128.  Fitted to 1558 measurements: 1-4096 tokens, 64-120818
 // channels, k 256-8192, every output; the tile of the least estimate takes 0.5 %
-// longer on average than the fastest one (worst 31 %: 2555 x 128 x 512).  E.g., us
-// estimated / measured: 2048 x 2048 x 2048 bf16 128 x 128 14.0 / 12.6, 128 x 64 18.2 / 16.0;
-// 61 x 2048 x 6144 fp32 32 x 16 6.1 / 6.5, 32 x 32 6.5 / 7.5.  (It knows nothing of HBM: one
-// token of 120818 channels takes 44 us, not 20; the order of the tiles holds.)
+// longer on average than the fastest one (worst 21 %: SwiGLU, 178 x 3606 x 768).  E.g.,
+// us estimated / measured: 2048 x 2048 x 2048 bf16 128 x 128 13.8 / 12.0, 128 x 64 18.4 /
+// 15.2; 700 x 2048 x 6144 bf16 96 x 64 17.0 / 15.4, 128 x 64 18.3 / 16.5.  (It knows nothing
+// of HBM: one token of 120818 channels takes 44 us, not 20; the order of the tiles
+// holds.)
 struct Shape {
     const char *name;
     int f, t, threads;
+    int glu;  // 0: any output, 1: SwiGLU only, 2: the others only
     float launch, round, stage, fill, fill_stage;
 };
 constexpr Shape kShapes[] = {
-    {"16x16", 16, 16, 256, 2.41f, 0.24f, 0.028f, 0.11f, 0.018f},
-    {"32x16", 32, 16, 256, 2.55f, 0.17f, 0.044f, 0.23f, 0.022f},
-    {"48x16", 48, 16, 256, 2.74f, 0.02f, 0.059f, 0.43f, 0.028f},
-    {"64x16", 64, 16, 256, 2.81f, 0.05f, 0.078f, 0.43f, 0.029f},
-    {"32x32", 32, 32, 256, 2.57f, 0.25f, 0.058f, 0.25f, 0.035f},
-    {"64x32", 64, 32, 256, 2.17f, 1.07f, 0.096f, 0.51f, 0.059f},
-    {"64x64", 64, 64, 256, 2.21f, 1.79f, 0.143f, 0.73f, 0.076f},
-    {"96x64", 96, 64, 256, 2.38f, 2.40f, 0.212f, 1.25f, 0.064f},
-    {"128x64", 128, 64, 256, 2.82f, 0.45f, 0.269f, 1.98f, 0.060f},
-    {"128x96", 128, 96, 256, 2.59f, 1.51f, 0.303f, 1.69f, 0.074f},
-    {"128x128", 128, 128, 256, 2.81f, 1.92f, 0.366f, 1.88f, 0.095f},
-    {"192x128", 192, 128, 512, 3.33f, 2.09f, 0.435f, 3.01f, 0.199f},
-    {"256x128", 256, 128, 256, 4.33f, 2.41f, 0.620f, 3.81f, 0.178f},
-    {"192x256", 192, 256, 512, 4.54f, 2.11f, 0.852f, 5.12f, 0.283f},
-    {"256x256", 256, 256, 512, 7.16f, 0.58f, 0.979f, 6.97f, 0.417f},
+    {"16x16", 16, 16, 256, 2, 2.43f, 0.21f, 0.028f, 0.14f, 0.018f},
+    {"32x16", 32, 16, 256, 0, 2.57f, 0.13f, 0.044f, 0.28f, 0.022f},
+    {"48x16", 48, 16, 256, 2, 2.75f, 0.00f, 0.059f, 0.45f, 0.028f},
+    {"64x16", 64, 16, 256, 0, 2.84f, 0.00f, 0.077f, 0.49f, 0.029f},
+    {"32x32", 32, 32, 256, 0, 2.63f, 0.17f, 0.058f, 0.33f, 0.034f},
+    {"64x32", 64, 32, 256, 0, 2.22f, 0.98f, 0.096f, 0.60f, 0.058f},
+    {"64x64", 64, 64, 512, 0, 2.44f, 1.12f, 0.124f, 1.16f, 0.070f},
+    {"96x64", 96, 64, 256, 1, 2.50f, 1.79f, 0.206f, 1.12f, 0.068f},
+    {"96x64", 96, 64, 512, 2, 2.49f, 1.44f, 0.168f, 1.66f, 0.076f},
+    {"128x64", 128, 64, 512, 0, 3.10f, 0.79f, 0.227f, 2.29f, 0.058f},
+    {"128x96", 128, 96, 256, 0, 3.02f, 0.94f, 0.308f, 2.04f, 0.052f},
+    {"128x128", 128, 128, 256, 0, 3.36f, 1.23f, 0.375f, 2.32f, 0.053f},
+    {"192x128", 192, 128, 512, 0, 3.78f, 1.51f, 0.452f, 3.22f, 0.123f},
+    {"256x128", 256, 128, 256, 0, 4.78f, 1.92f, 0.641f, 3.87f, 0.089f},
+    {"192x256", 192, 256, 512, 0, 4.50f, 2.00f, 0.896f, 4.99f, 0.140f},
+    {"256x256", 256, 256, 512, 0, 6.93f, 0.87f, 0.994f, 6.18f, 0.299f},
 };
 constexpr int kNumShapes = sizeof(kShapes) / sizeof(kShapes[0]);
 constexpr size_t kMaxTiles = 1u << 22;  // of a launch: a grid holds less than 2^32 threads
@@ -625,7 +672,7 @@ int plan(const I8Gemm &g, bool glu) {
     for (int i = 0; i < kNumShapes; i++) {
         const Shape &p = kShapes[i];
         const size_t tiles = tiles_of(p, g, glu);
-        if (tiles > kMaxTiles || (glu && p.f % 32 != 0)) continue;
+        if (tiles > kMaxTiles || p.glu == (glu ? 2 : 1)) continue;
         if (forced && !std::strcmp(forced, p.name)) return i;
         const float rounds = (float)((tiles + 255) / 256), fill = (float)tiles / 256.f;
         const float us = p.launch + rounds * (p.round + p.stage * kt) + fill * (p.fill + p.fill_stage * kt);
@@ -640,26 +687,32 @@ int plan(const I8Gemm &g, bool glu) {
 template <int OUT>
 void launch_shape(int i, const Args &a, const KernelSpan &span, hipStream_t s) {
     const dim3 grid(8 * a.per_xcd), block(kShapes[i].threads);
+    constexpr bool GLU = OUT == kGlu;
     switch (i) {
     case 0:
-        if constexpr (OUT != kGlu) launch(span, skinny_kernel<1, 1, 4, OUT>, grid, block, 0, s, a);
+        if constexpr (!GLU) launch(span, skinny_kernel<1, 1, 4, OUT>, grid, block, 0, s, a);
         break;
     case 1: launch(span, skinny_kernel<2, 1, 3, OUT>, grid, block, 0, s, a); break;
     case 2:
-        if constexpr (OUT != kGlu) launch(span, skinny_kernel<3, 1, 2, OUT>, grid, block, 0, s, a);
+        if constexpr (!GLU) launch(span, skinny_kernel<3, 1, 2, OUT>, grid, block, 0, s, a);
         break;
     case 3: launch(span, skinny_kernel<4, 1, 2, OUT>, grid, block, 0, s, a); break;
     case 4: launch(span, skinny_kernel<2, 2, 2, OUT>, grid, block, 0, s, a); break;
     case 5: launch(span, skinny_kernel<4, 2, 2, OUT>, grid, block, 0, s, a); break;
-    case 6: launch(span, skinny_kernel<4, 4, 2, OUT>, grid, block, 0, s, a); break;
-    case 7: launch(span, skinny_kernel<6, 4, 2, OUT>, grid, block, 0, s, a); break;
-    case 8: launch(span, tile_kernel<4, 2, 2, 4, false, OUT>, grid, block, 0, s, a); break;
-    case 9: launch(span, tile_kernel<4, 3, 2, 4, false, OUT>, grid, block, 0, s, a); break;
-    case 10: launch(span, tile_kernel<4, 4, 2, 4, false, OUT>, grid, block, 0, s, a); break;
-    case 11: launch(span, tile_kernel<6, 4, 4, 4, true, OUT>, grid, block, 0, s, a); break;
-    case 12: launch(span, tile_kernel<8, 4, 2, 3, true, OUT>, grid, block, 0, s, a); break;
-    case 13: launch(span, tile_kernel<6, 8, 4, 2, true, OUT>, grid, block, 0, s, a); break;
-    default: launch(span, tile_kernel<8, 8, 4, 2, true, OUT>, grid, block, 0, s, a); break;
+    case 6: launch(span, tile_kernel<2, 2, 2, 4, true, 2, OUT>, grid, block, 0, s, a); break;
+    case 7:
+        if constexpr (GLU) launch(span, skinny_kernel<6, 4, 2, OUT>, grid, block, 0, s, a);
+        break;
+    case 8:
+        if constexpr (!GLU) launch(span, tile_kernel<3, 2, 2, 4, true, 2, OUT>, grid, block, 0, s, a);
+        break;
+    case 9: launch(span, tile_kernel<4, 2, 2, 3, true, 2, OUT>, grid, block, 0, s, a); break;
+    case 10: launch(span, tile_kernel<4, 3, 2, 4, false, 1, OUT>, grid, block, 0, s, a); break;
+    case 11: launch(span, tile_kernel<4, 4, 2, 4, false, 1, OUT>, grid, block, 0, s, a); break;
+    case 12: launch(span, tile_kernel<6, 4, 4, 4, true, 1, OUT>, grid, block, 0, s, a); break;
+    case 13: launch(span, tile_kernel<8, 4, 2, 3, true, 1, OUT>, grid, block, 0, s, a); break;
+    case 14: launch(span, tile_kernel<6, 8, 4, 2, true, 1, OUT>, grid, block, 0, s, a); break;
+    default: launch(span, tile_kernel<8, 8, 4, 2, true, 1, OUT>, grid, block, 0, s, a); break;
     }
 }
 
