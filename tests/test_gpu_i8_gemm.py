@@ -227,3 +227,32 @@ def test_every_tile(be, monkeypatch, tile, m, n, k):
         check(run(be, w, ws, x, xs, "acc", ldy, y0=y0), y, "acc", y0)
         check(run(be, w, ws, x, xs, "bf16", ldy), y, "bf16")
         check_glu(run(be, w, ws, x, xs, "glu", ldy, up=up, us=us), w, ws, up, us, x, xs)
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_random_shapes(be, monkeypatch, seed):
+    """Seeded shapes, outputs, row strides, offsets and tiles (a quarter of them
+    the plan's own)."""
+    rng = np.random.default_rng(seed)
+
+    def log_int(lo, hi):
+        return int(round(np.exp(rng.uniform(np.log(lo), np.log(hi)))))
+
+    for case in range(40):
+        m, n, k = log_int(1, 600), log_int(1, 2000), 128 * log_int(2, 24)
+        out = rng.choice(["f32", "acc", "bf16", "glu"])
+        ldy, offset = n + int(rng.choice([0, 0, 1, 3, 4, 8])), int(rng.choice([0, 0, 4, 8, 2]))
+        offset = offset // 4 * 4 if out in ("f32", "acc") else offset
+        tile = str(rng.choice(TILES))
+        if case % 4:
+            monkeypatch.setenv("HYMT_HIP_I8_TILE", tile)
+        else:
+            monkeypatch.delenv("HYMT_HIP_I8_TILE", raising=False)
+        w, x, up = codes(case, n, k), codes(case + 1, m, k), codes(case + 2, n, k)
+        ws, us, xs = scales(case, n), scales(case + 1, n, 1e-5, 1e-3), scales(case + 2, m, 1e-4, 1e-2)
+        y0 = rng.standard_normal((m, n)).astype(np.float32) if out == "acc" else None
+        got = run(be, w, ws, x, xs, out, ldy, offset, y0, up, us)
+        if out == "glu":
+            check_glu(got, w, ws, up, us, x, xs)
+        else:
+            check(got, product(w, ws, x, xs), out, y0)
