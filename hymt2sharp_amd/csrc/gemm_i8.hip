@@ -11,7 +11,7 @@
 // 1.8 for a launch):
 //   tokens x channels x k      output       floor    here   rate
 //   1 x 2048 x 2048            fp32           2.6     2.9
-//   1 x 120818 x 2048          fp32          50.8    44.5   5.6 TB/s
+//   1 x 120818 x 2048          fp32          50.8    39.4   6.3 TB/s
 //   61 x 2048 x 6144           fp32 +=        4.6     6.3   2.1 TB/s
 //   700 x 2048 x 6144          bf16          10.4    15.4   1140 TOP/s
 //   2048 x 2048 x 2048         bf16          10.1    12.0   1430
@@ -61,6 +61,14 @@ template <int N, bool LGKM = false> __device__ __forceinline__ void wait_vm() {
 __device__ __forceinline__ void wait_lgkm() {
     __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));
     asm volatile("" ::: "memory");
+}
+
+// lds_dma16_sv past the caches.
+__device__ __forceinline__ void lds_dma16_sv_nt(const void *sbase, uint32_t voff, uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds_base)), "v"(voff), "s"(sbase)
+                 : "memory", "m0");
 }
 
 // The one arithmetic of an output: the channel's scale first, then the token's,
@@ -479,12 +487,15 @@ __global__ __launch_bounds__(128 * WT * KG, 1) void tile_kernel(Args a) {
 // streams its own quarter of the tile's W and x rows through an LDS ring of its
 // own, so there is no barrier before the end and four load streams run per
 // workgroup.  The four partial tiles meet in LDS.  Bound by the stream of W (one
-// token, 120818 channels: 44 us, 5.6 TB/s) or, where that is short, by a launch and
+// token, 120818 channels: 39 us, 6.3 TB/s) or, where that is short, by a launch and
 // two memory round trips (one token, 2048 x 2048: 2.8 us in a recording).  Deeper
-// rings and eight waves a workgroup were no faster at 1-700 tokens; W straight
-// into registers was (43 us) at one token of 120818 channels alone.  SwiGLU: the first A / 2 row
+// rings and eight waves a workgroup were no faster at 1-700 tokens, nor was W
+// straight into registers.  SwiGLU: the first A / 2 row
 // blocks are gate rows, the others the same rows of up.
-template <int A, int B, int S, int OUT>
+// ONCE: W goes past the caches (nt), where each of its rows is read by one
+// workgroup alone and it is too large to be found in the L2s by the next call
+// anyway (reads_once).
+template <int A, int B, int S, bool ONCE, int OUT>
 __global__ __launch_bounds__(256) void skinny_kernel(Args a) {
     constexpr bool GLU = OUT == kGlu;
     constexpr int C = 2 * (A + B);  // copies (1 KiB each) of a stage
@@ -525,7 +536,10 @@ __global__ __launch_bounds__(256) void skinny_kernel(Args a) {
 #pragma unroll
         for (int l = 0; l < C; l++) {
             const int gb = l >> 1;
-            lds_dma16_sv((gb >= A ? xb : GLU && gb >= AO ? ub : wb) + t * kBK, voff[l], ring + slot * kStage + l * 1024);
+            const int8_t *from = (gb >= A ? xb : GLU && gb >= AO ? ub : wb) + t * kBK;
+            const uint32_t to = ring + slot * kStage + l * 1024;
+            if (ONCE && gb < A) lds_dma16_sv_nt(from, voff[l], to);
+            else lds_dma16_sv(from, voff[l], to);
         }
     };
     uint32_t off[2];
@@ -628,7 +642,7 @@ __global__ __launch_bounds__(256) void skinny_kernel(Args a) {
 // longer on average than the fastest one (worst 21 %: SwiGLU, 178 x 3606 x 768).  E.g.,
 // us estimated / measured: 2048 x 2048 x 2048 bf16 128 x 128 13.8 / 12.0, 128 x 64 18.4 /
 // 15.2; 700 x 2048 x 6144 bf16 96 x 64 17.0 / 15.4, 128 x 64 18.3 / 16.5.  (It knows nothing
-// of HBM: one token of 120818 channels takes 44 us, not 20; the order of the tiles
+// of HBM: one token of 120818 channels takes 39 us, not 20; the order of the tiles
 // holds.)
 struct Shape {
     const char *name;
@@ -690,18 +704,18 @@ void launch_shape(int i, const Args &a, const KernelSpan &span, hipStream_t s) {
     constexpr bool GLU = OUT == kGlu;
     switch (i) {
     case 0:
-        if constexpr (!GLU) launch(span, skinny_kernel<1, 1, 4, OUT>, grid, block, 0, s, a);
+        if constexpr (!GLU) launch(span, skinny_kernel<1, 1, 4, false, OUT>, grid, block, 0, s, a);
         break;
-    case 1: launch(span, skinny_kernel<2, 1, 3, OUT>, grid, block, 0, s, a); break;
+    case 1: launch(span, skinny_kernel<2, 1, 3, false, OUT>, grid, block, 0, s, a); break;
     case 2:
-        if constexpr (!GLU) launch(span, skinny_kernel<3, 1, 2, OUT>, grid, block, 0, s, a);
+        if constexpr (!GLU) launch(span, skinny_kernel<3, 1, 2, false, OUT>, grid, block, 0, s, a);
         break;
-    case 3: launch(span, skinny_kernel<4, 1, 2, OUT>, grid, block, 0, s, a); break;
-    case 4: launch(span, skinny_kernel<2, 2, 2, OUT>, grid, block, 0, s, a); break;
-    case 5: launch(span, skinny_kernel<4, 2, 2, OUT>, grid, block, 0, s, a); break;
+    case 3: launch(span, skinny_kernel<4, 1, 2, false, OUT>, grid, block, 0, s, a); break;
+    case 4: launch(span, skinny_kernel<2, 2, 2, false, OUT>, grid, block, 0, s, a); break;
+    case 5: launch(span, skinny_kernel<4, 2, 2, false, OUT>, grid, block, 0, s, a); break;
     case 6: launch(span, tile_kernel<2, 2, 2, 4, true, 2, OUT>, grid, block, 0, s, a); break;
     case 7:
-        if constexpr (GLU) launch(span, skinny_kernel<6, 4, 2, OUT>, grid, block, 0, s, a);
+        if constexpr (GLU) launch(span, skinny_kernel<6, 4, 2, false, OUT>, grid, block, 0, s, a);
         break;
     case 8:
         if constexpr (!GLU) launch(span, tile_kernel<3, 2, 2, 4, true, 2, OUT>, grid, block, 0, s, a);
@@ -713,6 +727,32 @@ void launch_shape(int i, const Args &a, const KernelSpan &span, hipStream_t s) {
     case 13: launch(span, tile_kernel<8, 4, 2, 3, true, 1, OUT>, grid, block, 0, s, a); break;
     case 14: launch(span, tile_kernel<6, 8, 4, 2, true, 1, OUT>, grid, block, 0, s, a); break;
     default: launch(span, tile_kernel<8, 8, 4, 2, true, 1, OUT>, grid, block, 0, s, a); break;
+    }
+}
+
+// Whether the few-token kernel's W copies pass the caches: one token tile, so that
+// a row of W is read once, and 8 MiB of W or more.  us through the caches / past
+// them, over nine sets of weights in turn: 1 x 120818 x 2048 (64 x 16) 44.6 / 39.9, 16 x 120818
+// x 2048 51.2 / 44.5, 1 x 40000 x 4096 31.3 / 27.1, 1 x 16384 x 2048 (32 x 16) 8.3 / 7.5, 1 x 4096 x
+// 2048 (16 x 16) 4.1 / 3.5; 1 x 2048 x 6144 4.5 / 4.8 or, over three sets, 4.6 / 4.3; below
+// 8 MiB, where three sets stay in the L2s, the same or up to a quarter slower.
+bool reads_once(int i, const Args &a, bool glu) {
+    return i < 4 && a.tiles_t == 1 && (size_t)a.g.n * a.g.k * (glu ? 2 : 1) >= (8u << 20);
+}
+
+template <int OUT>
+void launch_once(int i, const Args &a, const KernelSpan &span, hipStream_t s) {
+    const dim3 grid(8 * a.per_xcd), block(kShapes[i].threads);
+    constexpr bool GLU = OUT == kGlu;
+    switch (i) {
+    case 0:
+        if constexpr (!GLU) launch(span, skinny_kernel<1, 1, 4, true, OUT>, grid, block, 0, s, a);
+        break;
+    case 1: launch(span, skinny_kernel<2, 1, 3, true, OUT>, grid, block, 0, s, a); break;
+    case 2:
+        if constexpr (!GLU) launch(span, skinny_kernel<3, 1, 2, true, OUT>, grid, block, 0, s, a);
+        break;
+    default: launch(span, skinny_kernel<4, 1, 2, true, OUT>, grid, block, 0, s, a); break;
     }
 }
 
@@ -738,7 +778,8 @@ hipError_t run(const I8Gemm &g, const char *name, hipStream_t s) {
     constexpr int es = OUT == kBf16 || OUT == kGlu ? 2 : 4;
     a.vec = ((uintptr_t)g.y & 15u) == 0 && g.ldy % (16 / es) == 0;
     KernelSpan span(name, s, true);
-    launch_shape<OUT>(i, a, span, s);
+    if (reads_once(i, a, OUT == kGlu)) launch_once<OUT>(i, a, span, s);
+    else launch_shape<OUT>(i, a, span, s);
     return hipGetLastError();
 }
 

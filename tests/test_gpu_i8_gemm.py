@@ -229,6 +229,25 @@ def test_every_tile(be, monkeypatch, tile, m, n, k):
         check_glu(run(be, w, ws, x, xs, "glu", ldy, up=up, us=us), w, ws, up, us, x, xs)
 
 
+@pytest.mark.parametrize("tile", ["16x16", "32x16", "48x16", "64x16"])
+@pytest.mark.parametrize("m", [1, 9, 16])
+def test_weights_read_past_the_caches(be, monkeypatch, tile, m):
+    """Up to 16 tokens over 8 MiB of weights and more (4099 x 2048; SwiGLU 2 x
+    2051 x 2048), and just below."""
+    monkeypatch.setenv("HYMT_HIP_I8_TILE", tile)
+    for n, f in ((4099, 2051), (4095, 2047)):
+        k = 2048
+        w, x, up = codes(1, n, k), codes(2, m, k), codes(3, f, k)
+        ws, us, xs = scales(4, n, 1e-5, 1e-3), scales(5, f, 1e-5, 1e-3), scales(6, m, 1e-3, 1e-1)
+        y0 = np.random.default_rng(7).standard_normal((m, n)).astype(np.float32)
+        y = product(w, ws, x, xs)
+        check(run(be, w, ws, x, xs, "f32"), y, "f32")
+        check(run(be, w, ws, x, xs, "acc", y0=y0), y, "acc", y0)
+        check(run(be, w, ws, x, xs, "bf16"), y, "bf16")
+        g, gs = np.ascontiguousarray(w[:f]), np.ascontiguousarray(ws[:f])
+        check_glu(run(be, g, gs, x, xs, "glu", up=up, us=us), g, gs, up, us, x, xs)
+
+
 @pytest.mark.parametrize("seed", range(4))
 def test_random_shapes(be, monkeypatch, seed):
     """Seeded shapes, outputs, row strides, offsets and tiles (a quarter of them
