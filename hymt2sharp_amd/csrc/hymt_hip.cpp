@@ -30,6 +30,9 @@ namespace {
 thread_local std::string g_err;
 
 int fail(int code, const std::string &msg) {
+    // the runtime keeps a failed call's error for its next hipGetLastError, which
+    // is that of the next launch: one that went well would report this failure
+    if (code == HYMT_E_OOM || code == HYMT_E_DEVICE) (void)hipGetLastError();
     g_err = msg;
     return code;
 }
