@@ -677,9 +677,11 @@ size_t tiles_of(const Shape &p, const I8Gemm &g, bool glu) {
 }
 
 // The tile of the least estimated time; HYMT_HIP_I8_TILE=<tile> forces one (a
-// tuning knob).  SwiGLU takes the tiles whose row blocks split into gate and up.
+// tuning knob) on the outputs that it serves: SwiGLU takes the tiles whose row
+// blocks split into gate and up.
 int plan(const I8Gemm &g, bool glu) {
     const char *forced = std::getenv("HYMT_HIP_I8_TILE");
+    if (forced && !gemm_i8_tile_known()) return -1;
     const float kt = (float)(g.k / kBK);
     int best = -1;
     float least = 0.f;
@@ -767,7 +769,7 @@ hipError_t run(const I8Gemm &g, const char *name, hipStream_t s) {
     if (!fits(g)) return hipErrorInvalidValue;
     if (g.m == 0) return hipSuccess;
     const int i = plan(g, OUT == kGlu);
-    if (i < 0) return hipErrorInvalidValue;  // more tiles than a launch holds
+    if (i < 0) return hipErrorInvalidValue;  // more tiles than a launch holds, or no such tile
     const int of = OUT == kGlu ? kShapes[i].f / 2 : kShapes[i].f;
     Args a{};
     a.g = g;
@@ -784,6 +786,14 @@ hipError_t run(const I8Gemm &g, const char *name, hipStream_t s) {
 }
 
 }  // namespace
+
+bool gemm_i8_tile_known() {
+    const char *forced = std::getenv("HYMT_HIP_I8_TILE");
+    if (!forced) return true;
+    for (const Shape &p : kShapes)
+        if (!std::strcmp(forced, p.name)) return true;
+    return false;
+}
 
 hipError_t launch_gemm_i8(const I8Gemm &g, I8Out out, hipStream_t s) {
     if (out == kI8Bf16) return run<kBf16>(g, "gemm_i8_out_bf16", s);

@@ -1380,6 +1380,10 @@ int check_i8_rows(int m, int n) {
     return HYMT_OK;
 }
 
+int check_i8_tile() {
+    return gemm_i8_tile_known() ? HYMT_OK : fail(HYMT_E_ARG, "HYMT_HIP_I8_TILE names no tile of the int8 products");
+}
+
 // What the two int8 products check alike (up null: no up rows).
 int check_i8_gemm(const I8Gemm &g, size_t y_bytes) {
     if (g.m < 0) return fail(HYMT_E_ARG, "negative row count");
@@ -1391,7 +1395,7 @@ int check_i8_gemm(const I8Gemm &g, size_t y_bytes) {
         return fail(HYMT_E_ARG, "codes must be 16-byte aligned");
     if (misaligned(g.ws, 4) || misaligned(g.us, 4) || misaligned(g.xs, 4) || misaligned(g.y, y_bytes))
         return fail(HYMT_E_ARG, "scales and the output must be aligned to their elements");
-    return HYMT_OK;
+    return check_i8_tile();
 }
 }  // namespace
 
@@ -1763,6 +1767,8 @@ int hymt_model_prefill(hymt_model *m, const int32_t *tokens, int n, int pos, flo
         return fail(HYMT_E_ARG, "HYMT_PREFILL_INT8 and HYMT_PREFILL_GATE_UP_F32 exclude each other");
     if (int8 && !prefill_i8_ready(m))
         return fail(HYMT_E_STATE, "a layer weight has no int8 codes (hymt_weight_i8)");
+    if (int8)
+        if (int r = check_i8_tile()) return r;
     if (n < 1 || !tokens) return fail(HYMT_E_ARG, "empty token list");
     for (int i = 0; i < n; i++)
         if (tokens[i] < 0 || tokens[i] >= m->vocab) return fail(HYMT_E_ARG, "token out of range");

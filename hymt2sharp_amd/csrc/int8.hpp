@@ -41,6 +41,9 @@ struct I8Gemm {
     int n, k, m, ldy;
 };
 hipError_t launch_gemm_i8(const I8Gemm &g, I8Out out, hipStream_t s);
+// Whether HYMT_HIP_I8_TILE is unset or the name of a tile; the launches refuse
+// another.
+bool gemm_i8_tile_known();
 // act[m][n] = bf16(silu(gate) up) of the two products in fp32
 hipError_t launch_gemm_i8_swiglu(const I8Gemm &g, hipStream_t s);
 
