@@ -787,6 +787,11 @@ hipError_t run(const I8Gemm &g, const char *name, hipStream_t s) {
 
 }  // namespace
 
+bool gemm_i8_launches(const I8Gemm &g) {
+    // no tile makes fewer than the last, the largest
+    return tiles_of(kShapes[kNumShapes - 1], g, g.up != nullptr) <= kMaxTiles;
+}
+
 bool gemm_i8_tile_known() {
     const char *forced = std::getenv("HYMT_HIP_I8_TILE");
     if (!forced) return true;

@@ -1395,6 +1395,7 @@ int check_i8_gemm(const I8Gemm &g, size_t y_bytes) {
         return fail(HYMT_E_ARG, "codes must be 16-byte aligned");
     if (misaligned(g.ws, 4) || misaligned(g.us, 4) || misaligned(g.xs, 4) || misaligned(g.y, y_bytes))
         return fail(HYMT_E_ARG, "scales and the output must be aligned to their elements");
+    if (!gemm_i8_launches(g)) return fail(HYMT_E_UNSUPPORTED, "more than 2^22 tiles of 256 x 256 outputs (SwiGLU 128 x 256)");
     return check_i8_tile();
 }
 }  // namespace

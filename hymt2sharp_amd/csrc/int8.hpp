@@ -41,6 +41,8 @@ struct I8Gemm {
     int n, k, m, ldy;
 };
 hipError_t launch_gemm_i8(const I8Gemm &g, I8Out out, hipStream_t s);
+// Whether some tile covers g (up: SwiGLU) in as many workgroups as a launch holds.
+bool gemm_i8_launches(const I8Gemm &g);
 // Whether HYMT_HIP_I8_TILE is unset or the name of a tile; the launches refuse
 // another.
 bool gemm_i8_tile_known();

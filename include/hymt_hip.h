@@ -435,7 +435,8 @@ int hymt_rows_rmsnorm_i8(hymt_ctx *ctx, float *x, const void *add, int add_dtype
  * kernel or on m.  y is fp32, rows ldy >= n elements apart, or as the flags
  * say: HYMT_GEMM_ACCUMULATE y += in fp32 (fused with the last product),
  * HYMT_GEMM_OUT_BF16 bf16.  k a multiple of 128, 256 to 65536; up to 2^30 tokens
- * and channels; w and x 16-byte aligned, y and the scales by their elements. */
+ * and channels, and 2^22 tiles of 256 x 256 outputs (SwiGLU 128 channels x 256
+ * tokens); w and x 16-byte aligned, y and the scales by their elements. */
 int hymt_gemm_i8(hymt_ctx *ctx, const int8_t *w, const float *w_scale, int n, int k, const int8_t *x,
                  const float *x_scale, int m, void *y, int ldy, int flags);
 
