@@ -6,18 +6,22 @@
 // The sum is exact, so its order is free: every kernel and tile below gives the
 // same bits, and which one runs is a matter of time alone.
 //
-// What it takes (us, in a recording; the floor is the bytes at 5.05 TB/s or the
-// operations at 2058 TOP/s, what a large copy and a large int8 product reach, and
-// 1.8 for a launch):
-//   tokens x channels x k      output       floor    here   rate
-//   1 x 2048 x 2048            fp32           2.6     2.9
-//   1 x 120818 x 2048          fp32          50.8    39.4   6.3 TB/s
-//   61 x 2048 x 6144           fp32 +=        4.6     6.3   2.1 TB/s
-//   700 x 2048 x 6144          bf16          10.4    15.4   1140 TOP/s
-//   2048 x 2048 x 2048         bf16          10.1    12.0   1430
-//   2048 x 2048 x 6144         fp32          26.8    27.5   1870
-//   61 x 2 6144 x 2048         SwiGLU         6.9     7.5   3.5 TB/s
-//   2048 x 2 6144 x 2048       SwiGLU        51.9    47.6   2170 TOP/s
+// What it takes (us, in a recording, over the cards seen).  here: three sets of
+// operands in turn, whose weights stay in the 256 MB last-level cache but for the
+// 120818 channels; cold: enough sets to exceed it.  ref: the bytes at 5.05 TB/s or the
+// operations at 2058 TOP/s, what a large copy and a large int8 product of the
+// library reach, and 1.8 for a launch; no bound, since a stream that is only read
+// passes 6.3 TB/s and the SwiGLU beats that product.
+//   tokens x channels x k      output        ref    here        cold
+//   1 x 2048 x 2048            fp32          2.6    2.9-3.0     4.0
+//   1 x 120818 x 2048          fp32         50.8    39.1-39.7   39.4-39.6
+//   61 x 2048 x 6144           fp32 +=       4.6    6.3-6.5     9.0
+//   300 x 2048 x 6144          bf16          5.5   11.7        16.2
+//   700 x 2048 x 6144          bf16         10.4   15.1-16.2   20.4
+//   2048 x 2048 x 2048         bf16         10.1   11.9-13.2   14.3
+//   2048 x 2048 x 6144         fp32         26.8   27.4-30.4   34.9
+//   61 x 2 6144 x 2048         SwiGLU        6.9    7.2-7.6    10.6
+//   2048 x 2 6144 x 2048       SwiGLU       51.9   47.6-51.5   57.5
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -487,8 +491,9 @@ __global__ __launch_bounds__(128 * WT * KG, 1) void tile_kernel(Args a) {
 // streams its own quarter of the tile's W and x rows through an LDS ring of its
 // own, so there is no barrier before the end and four load streams run per
 // workgroup.  The four partial tiles meet in LDS.  Bound by the stream of W (one
-// token, 120818 channels: 39 us, 6.3 TB/s) or, where that is short, by a launch and
-// two memory round trips (one token, 2048 x 2048: 2.8 us in a recording).  Deeper
+// token, 120818 channels: 39 us, 6.3 TB/s) or, where that is short, by a launch, the
+// way of the operands and that of the scales, which are loaded after the last
+// stage (one token, 2048 x 2048: 2.9 us in a recording, 4.0 with W cold).  Deeper
 // rings and eight waves a workgroup were no faster at 1-700 tokens, nor was W
 // straight into registers.  SwiGLU: the first A / 2 row
 // blocks are gate rows, the others the same rows of up.
@@ -734,10 +739,11 @@ void launch_shape(int i, const Args &a, const KernelSpan &span, hipStream_t s) {
 
 // Whether the few-token kernel's W copies pass the caches: one token tile, so that
 // a row of W is read once, and 8 MiB of W or more.  us through the caches / past
-// them, over nine sets of weights in turn: 1 x 120818 x 2048 (64 x 16) 44.6 / 39.9, 16 x 120818
-// x 2048 51.2 / 44.5, 1 x 40000 x 4096 31.3 / 27.1, 1 x 16384 x 2048 (32 x 16) 8.3 / 7.5, 1 x 4096 x
-// 2048 (16 x 16) 4.1 / 3.5; 1 x 2048 x 6144 4.5 / 4.8 or, over three sets, 4.6 / 4.3; below
-// 8 MiB, where three sets stay in the L2s, the same or up to a quarter slower.
+// them, over sets of weights of 0.6 GB (cold) and over three sets: 1 x 2048 x 6144
+// cold 5.55 / 4.79, three 4.60 / 4.27; 16 x 2048 x 6144 cold 6.85 / 6.49, three 5.01 / 5.43;
+// 1 x 6144 x 2048 5.36 / 4.46, 4.75 / 3.90; 1 x 12288 x 2048 7.37 / 6.29, 6.24 / 5.71; 1 x
+// 120818 x 2048 44.4 / 39.2; SwiGLU 1 x 6144 x 2048 7.51 / 6.50, 6.38 / 5.88.  Below 8 MiB three
+// sets stay in the L2s and take the same either way.
 bool reads_once(int i, const Args &a, bool glu) {
     return i < 4 && a.tiles_t == 1 && (size_t)a.g.n * a.g.k * (glu ? 2 : 1) >= (8u << 20);
 }

@@ -16,7 +16,7 @@
 // whose maximum is outside [2^-90, 2^100], where fp32 could flush or overflow, take
 // the quotient throughout.  (All in fp64, 2048 x 6144 bf16 rows took 15.0 us.)
 // Of plain rows the quotient decides: 127 v is exact, and the quotient of two
-// 24-bit values is 1/2 + a whole number or 2^-25 away, more than fp64's 2^-46.
+// 24-bit values is 1/2 + a whole number or 2^-33 away, more than fp64's 2^-46.
 // Of x w, whose 127-fold has 55 bits and whose quotient may be 2^-49 away, the exact
 // remainder does where the quotient is within 2^-40 of a border (2048 x 2048 after an
 // addition: 9.7 us, as with the quotients alone; taken for every value near a border
