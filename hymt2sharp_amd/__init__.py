@@ -6,12 +6,14 @@ behind the C ABI in include/hymt_hip.h (libhymt_hip.so).
 
     from hymt2sharp_amd import HipBackend, create_backend
 """
-from ._native import BF16, F16, F32, PAGE_TOKENS  # noqa: F401
+from ._native import (BF16, F16, F32, PAGE_TOKENS, ROPE_LINEAR, ROPE_NONE, ROPE_NTK, ROPE_YARN,  # noqa: F401
+                      PagedCache, Rope, SeqBatch)
 from .backend import (ArgumentError, HipBackend, InvalidOperationError,  # noqa: F401
                       NotSupportedError, PlatformNotSupportedError, create_backend,
-                      device_count)
+                      device_count, rope_freqs)
 
 __all__ = [
     "HipBackend", "create_backend", "device_count", "F32", "F16", "BF16", "PAGE_TOKENS",
+    "PagedCache", "SeqBatch", "Rope", "rope_freqs", "ROPE_NONE", "ROPE_LINEAR", "ROPE_NTK", "ROPE_YARN",
     "ArgumentError", "NotSupportedError", "PlatformNotSupportedError", "InvalidOperationError",
 ]

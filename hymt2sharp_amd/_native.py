@@ -119,6 +119,14 @@ SIGNATURES = {
     "hymt_rows_rmsnorm_i8": [_vp, _vp, _vp, _i, _i, _i, _vp, ctypes.c_float, _vp, _vp],
     "hymt_gemm_i8": [_vp, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _i, _i],
     "hymt_gemm_i8_swiglu": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _vp, _i, _vp, _i],
+    "hymt_paged_extend": [_vp, _vp, _vp, _vp, _i],
+    "hymt_paged_fork": [_vp, _vp, _vp, _vp, _i],
+    "hymt_paged_set_len": [_vp, _vp, _vp, _vp, _i],
+    "hymt_paged_compact": [_vp, _vp],
+    "hymt_rope_freqs": [_i, ctypes.c_double, _i, ctypes.c_double, _i, _vp, ctypes.POINTER(_f)],
+    "hymt_rope_append": [_vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _f, _vp],
+    "hymt_attn_packed": [_vp, _vp, _i, _vp, _vp, _i, _f, _vp, _i],
+    "hymt_attn_shared": [_vp, _vp, _i, _vp, _i, _vp, _i, _f, _vp, _i],
     "hymt_to_bf16": [_vp, _vp, ctypes.c_size_t, _vp],
     "hymt_model_create": [_vp, _i, _i, _i, _i, ctypes.c_float, ctypes.POINTER(_vp)],
     "hymt_model_set_layer": [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
@@ -133,6 +141,35 @@ W_F32, W_F16, W_Q8_0, W_Q4_K, W_Q6_K, W_Q2_0C, W_STQ1_0 = 0, 1, 8, 12, 14, 40, 4
 GEMV_ACCUMULATE, GEMV_IN_RMSNORM, GEMV_IN_SWIGLU, GEMV_OUT_SWIGLU = 1, 2, 4, 8
 GEMM_ACCUMULATE, GEMM_OUT_BF16 = 1, 2
 PREFILL_GATE_UP_F32, PREFILL_INT8 = 1, 2
+
+ROPE_NONE, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = 0, 1, 2, 3
+PAGED_BATCH = 1024
+
+
+def paged_work(pages: int) -> int:
+    """int32 values of a multi-sequence cache's work buffer."""
+    return 4 + 3 * pages
+
+
+class PagedCache(ctypes.Structure):
+    """hymt_paged: a pool of pages that many sequences share (device addresses)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("table", _vp), ("len", _vp), ("refs", _vp), ("work", _vp),
+                ("layers", ctypes.c_int32), ("pages", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("seqs", ctypes.c_int32),
+                ("blocks", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class SeqBatch(ctypes.Structure):
+    """hymt_batch: the rows of n slots, packed (cu) or one each."""
+    _fields_ = [("slots", _vp), ("cu", _vp), ("n", ctypes.c_int32), ("rows", ctypes.c_int32),
+                ("max_len", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class Rope(ctypes.Structure):
+    """hymt_rope: rotary positions by a table of frequencies (rope_freqs)."""
+    _fields_ = [("freq", _vp), ("dim", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("scale", _f),
+                ("reserved", ctypes.c_int32)]
+
 
 _lib = None
 _synth = None

@@ -323,6 +323,79 @@ class HipBackend:
         N.check(self._lib.hymt_gemm_i8_swiglu(self._h, gate_dev, gate_scale_dev, up_dev, up_scale_dev, f, k, x_dev,
                                               x_scale_dev, m, act_dev, f if ld is None else ld))
 
+    # -- many sequences over one paged cache ---------------------------------
+    def paged_create(self, layers: int, pages: int, seqs: int, blocks: int, kv_heads: int = 4, head_dim: int = 128,
+                     dtype: int = N.BF16) -> N.PagedCache:
+        """A pool of `pages` pages, all free, and `seqs` empty slots of up to
+        blocks * 64 positions, in device memory (paged_free)."""
+        page = kv_heads * N.PAGE_TOKENS * head_dim * 2
+        c = N.PagedCache(layers=layers, pages=pages, kv_heads=kv_heads, head_dim=head_dim, dtype=dtype, seqs=seqs,
+                         blocks=blocks)
+        try:
+            c.k, c.v = self.alloc(layers * pages * page), self.alloc(layers * pages * page)
+            for name, count, fill in (("table", seqs * blocks, -1), ("len", seqs, 0), ("refs", pages, 0),
+                                      ("work", N.paged_work(pages), 0)):
+                setattr(c, name, self.alloc(4 * count))
+                self.upload(getattr(c, name), np.full(count, fill, np.int32))
+        except Exception:
+            self.paged_free(c)
+            raise
+        return c
+
+    def paged_free(self, cache: N.PagedCache):
+        for name in ("k", "v", "table", "len", "refs", "work"):
+            p = getattr(cache, name)
+            if p:
+                self.free(p)
+            setattr(cache, name, None)
+
+    def paged_work(self, cache: N.PagedCache) -> dict:
+        """What the upkeep calls left: the first status that was not 0 and the
+        last one (hymt_status), pages copied by the last, pages in use at the
+        last compact.  Waits for the stream."""
+        w = np.empty(4, np.int32)
+        self.download(w, cache.work)
+        return {"first": int(w[0]), "copies": int(w[1]), "live": int(w[2]), "status": int(w[3])}
+
+    def paged_extend(self, cache, slots_dev, n: int, cu=None):
+        """Pages for cu[i + 1] - cu[i] more positions (one without cu) of each slot."""
+        N.check(self._lib.hymt_paged_extend(self._h, ctypes.byref(cache), slots_dev, cu, n))
+
+    def paged_fork(self, cache, parent_dev, child_dev, n: int):
+        """Empty slots child[i] become copies of parent[i], sharing whole pages."""
+        N.check(self._lib.hymt_paged_fork(self._h, ctypes.byref(cache), parent_dev, child_dev, n))
+
+    def paged_set_len(self, cache, slots_dev, n: int, lens=None):
+        """Slots keep their first lens[i] positions (none without lens)."""
+        N.check(self._lib.hymt_paged_set_len(self._h, ctypes.byref(cache), slots_dev, lens, n))
+
+    def paged_compact(self, cache):
+        """The pages in use move to the front of the pool."""
+        N.check(self._lib.hymt_paged_compact(self._h, ctypes.byref(cache)))
+
+    def rope_append(self, cache, layer: int, batch, q_dev, q_ld: int, k_dev, v_dev, kv_ld: int, io_dtype: int,
+                    heads: int, rope, qnw, knw, eps: float, q_out_dev):
+        """q_out = the batch's q rows rotated and normed; k (likewise) and v into
+        the pages of `layer`."""
+        N.check(self._lib.hymt_rope_append(self._h, ctypes.byref(cache), layer, ctypes.byref(batch), q_dev, q_ld, k_dev,
+                                           v_dev, kv_ld, io_dtype, heads, ctypes.byref(rope), qnw, knw, eps, q_out_dev))
+
+    def attn_packed(self, cache, layer: int, batch, q_dev, heads: int, out_dev, scale: float | None = None,
+                    out_dtype: int | None = None):
+        """Causal attention of the batch's packed rows over their pages; scale
+        1 / sqrt(head_dim) and out of the cache's type unless given."""
+        N.check(self._lib.hymt_attn_packed(self._h, ctypes.byref(cache), layer, ctypes.byref(batch), q_dev, heads,
+                                           cache.head_dim ** -0.5 if scale is None else scale, out_dev,
+                                           cache.dtype if out_dtype is None else out_dtype))
+
+    def attn_shared(self, cache, layer: int, batch, prefix: int, q_dev, heads: int, out_dev, scale: float | None = None,
+                    out_dtype: int | None = None):
+        """Attention of one row per slot, the first `prefix` positions (slot 0's)
+        read once for all."""
+        N.check(self._lib.hymt_attn_shared(self._h, ctypes.byref(cache), layer, ctypes.byref(batch), prefix, q_dev, heads,
+                                           cache.head_dim ** -0.5 if scale is None else scale, out_dev,
+                                           cache.dtype if out_dtype is None else out_dtype))
+
     def stream(self) -> int:
         s = ctypes.c_void_p()
         N.check(self._lib.hymt_get_stream(self._h, ctypes.byref(s)))
@@ -367,6 +440,15 @@ class HipBackend:
             self.Dispose()
         except Exception:
             pass
+
+
+def rope_freqs(dim: int, base: float = 10000.0, scaling: int = N.ROPE_NONE, factor: float = 1.0, trained: int = 4096):
+    """Frequencies [dim / 2] (radians per position, fp64) and the factor on cosine
+    and sine, for Rope: N.ROPE_NONE, or contexts `factor` times longer than
+    `trained` by N.ROPE_LINEAR, N.ROPE_NTK or N.ROPE_YARN."""
+    f, s = np.empty(dim // 2, np.float64), ctypes.c_float()
+    N.check(N.lib().hymt_rope_freqs(dim, base, scaling, factor, trained, _ptr(f), ctypes.byref(s)))
+    return f, s.value
 
 
 def device_count() -> int:

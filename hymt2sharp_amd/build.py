@@ -40,6 +40,8 @@ HIP_SOURCES = {
     "gemm_skinny.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "gemm_i8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "rows_i8.hip": [],
+    "paged_ops.hip": [],
+    "paged_attn.hip": [],
     "ktimer.cpp": [],
 }
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

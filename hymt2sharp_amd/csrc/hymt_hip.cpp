@@ -21,6 +21,7 @@
 #include "int8.hpp"
 #include "ktimer.hpp"
 #include "kv_pages.hpp"
+#include "paged.hpp"
 #include "weights.hpp"
 
 using namespace hymt;
@@ -121,6 +122,7 @@ struct hymt_ctx {
     DevBuf dec_ml, dec_acc;
     // prefill workspace: split partials; q prepared by prefill_kv for the flash kernel
     DevBuf part_o, part_ml, qready;
+    DevBuf paged_ws;  // split partials of the attention over the multi-sequence cache
     // staging for host-pointer calls
     DevBuf in_q, in_k, in_v, in_qnw, in_knw, out_o, up_k, up_v;
     DevBuf rows_idx;  // token ids of hymt_embed_rows
@@ -142,7 +144,7 @@ struct hymt_ctx {
 
     hymt_ctx() {
         for (DevBuf *b : {&kpool, &vpool, &tab, &rope_cos, &rope_sin, &ones, &dec_ml, &dec_acc, &part_o, &part_ml,
-                          &qready, &in_q, &in_k, &in_v, &in_qnw, &in_knw, &out_o, &up_k, &up_v, &rows_idx})
+                          &qready, &paged_ws, &in_q, &in_k, &in_v, &in_qnw, &in_knw, &out_o, &up_k, &up_v, &rows_idx})
             b->gen = &gen;
     }
 
@@ -1517,6 +1519,182 @@ int hymt_gemm_i8_swiglu(hymt_ctx *c, const int8_t *gate, const float *gate_scale
         return map_hip(e);
     }
     return HYMT_OK;
+}
+
+// ---- many sequences over one paged cache ---------------------------------------
+
+namespace {
+int check_paged(const hymt_paged *p) {
+    if (!p) return fail(HYMT_E_ARG, "null cache");
+    if (!p->k || !p->v || !p->table || !p->len || !p->refs || !p->work) return fail(HYMT_E_ARG, "null buffer in the cache");
+    if (p->dtype != HYMT_F16 && p->dtype != HYMT_BF16) return fail(HYMT_E_UNSUPPORTED, "the cache must be fp16 or bf16");
+    if (p->head_dim != 64 && p->head_dim != 128) return fail(HYMT_E_UNSUPPORTED, "head_dim must be 64 or 128");
+    if (p->layers < 1 || p->pages < 1 || p->kv_heads < 1 || p->seqs < 1 || p->blocks < 1)
+        return fail(HYMT_E_ARG, "layers, pages, kv_heads, seqs and blocks must be positive");
+    if (p->kv_heads > 256 || p->seqs > kPagedMaxSeqs || p->blocks > kPagedMaxBlocks || p->pages > (1 << 28))
+        return fail(HYMT_E_UNSUPPORTED, "more than 256 kv heads, 65536 slots, 2^24 pages of one slot or 2^28 in all");
+    if (p->reserved != 0) return fail(HYMT_E_ARG, "reserved fields must be 0");
+    if (misaligned(p->k, 256) || misaligned(p->v, 256)) return fail(HYMT_E_ARG, "the pages must be 256-byte aligned");
+    if (misaligned(p->refs, 4) || misaligned(p->table, 4) || misaligned(p->len, 4) || misaligned(p->work, 4))
+        return fail(HYMT_E_ARG, "table, len, refs and work must be 4-byte aligned");
+    return HYMT_OK;
+}
+
+// The entries of an upkeep call: arrays of n int32, `b` only where given.
+int check_entries(const int32_t *a, const int32_t *b, int n) {
+    if (n < 0) return fail(HYMT_E_ARG, "negative entry count");
+    if (n > HYMT_PAGED_BATCH) return fail(HYMT_E_UNSUPPORTED, "more entries than HYMT_PAGED_BATCH in one call");
+    if (!a) return fail(HYMT_E_ARG, "null entries");
+    if (misaligned(a, 4) || misaligned(b, 4)) return fail(HYMT_E_ARG, "entries must be 4-byte aligned");
+    return HYMT_OK;
+}
+
+int check_batch(const hymt_batch *b) {
+    if (!b) return fail(HYMT_E_ARG, "null batch");
+    if (int r = check_entries(b->slots, b->cu, b->n)) return r;
+    if (b->rows < 0 || b->max_len < 0 || b->reserved != 0)
+        return fail(HYMT_E_ARG, "rows and max_len must not be negative, reserved fields 0");
+    if (!b->cu && b->rows != b->n) return fail(HYMT_E_ARG, "without cu a batch has as many rows as entries");
+    if (b->rows > 1 << 24) return fail(HYMT_E_UNSUPPORTED, "more than 2^24 rows");
+    return HYMT_OK;
+}
+
+int check_heads(const hymt_paged *p, int layer, int heads) {
+    if (layer < 0 || layer >= p->layers) return fail(HYMT_E_ARG, "layer outside the cache");
+    if (heads < 1 || heads % p->kv_heads != 0) return fail(HYMT_E_ARG, "heads must be a multiple of kv_heads");
+    if (heads / p->kv_heads > kPagedMaxGroup) return fail(HYMT_E_UNSUPPORTED, "more than 64 heads per kv head");
+    return HYMT_OK;
+}
+
+// Run `enqueue` on the context's device as the timed call `name`.
+template <typename F> int paged_call(hymt_ctx *c, const char *name, long arg, F enqueue) {
+    if (!c->has_device()) return fail(HYMT_E_NO_DEVICE, "context has no device");
+    TimedCall timed(call_timer(c), name, arg);
+    try {
+        HIP_TRY(hipSetDevice(c->device));
+        HIP_TRY(enqueue());
+    } catch (const HipError &e) {
+        return map_hip(e);
+    }
+    return HYMT_OK;
+}
+
+int paged_attention(hymt_ctx *c, const hymt_paged *p, int layer, const hymt_batch *b, int prefix, const void *q, int heads,
+                    float scale, void *out, int out_dtype, bool shared) {
+    if (int r = check_ctx(c, false, false)) return r;
+    if (int r = check_paged(p)) return r;
+    if (int r = check_batch(b)) return r;
+    if (int r = check_heads(p, layer, heads)) return r;
+    if (shared && b->cu) return fail(HYMT_E_ARG, "the batch must have one row per entry (cu NULL)");
+    if (prefix < 0 || prefix % kPage != 0) return fail(HYMT_E_ARG, "prefix must be a multiple of 64");
+    if (!q || !out) return fail(HYMT_E_ARG, "null q or out");
+    if (out_dtype != HYMT_F16 && out_dtype != HYMT_BF16) return fail(HYMT_E_UNSUPPORTED, "out must be fp16 or bf16");
+    if (!std::isfinite(scale)) return fail(HYMT_E_ARG, "scale must be finite");
+    if (misaligned16(q) || misaligned16(out)) return fail(HYMT_E_ARG, "q and out must be 16-byte aligned");
+    const PagedAttn a{q, heads, layer, prefix, scale, out, out_dtype};
+    if (!c->has_device()) return fail(HYMT_E_NO_DEVICE, "context has no device");
+    const size_t need = paged_attn_workspace(*p, *b, a, shared) * 4;
+    if (c->capturing && need > c->paged_ws.bytes) return fail_capture(c, "the attention's workspace would grow");
+    return paged_call(c, shared ? "attn_shared" : "attn_packed", b->rows, [&] {
+        c->paged_ws.reserve(need);
+        return shared ? launch_attn_shared(*p, *b, a, (float *)c->paged_ws.p, c->stream)
+                      : launch_attn_packed(*p, *b, a, (float *)c->paged_ws.p, c->stream);
+    });
+}
+}  // namespace
+
+int hymt_paged_extend(hymt_ctx *c, const hymt_paged *p, const int32_t *slots, const int32_t *cu, int n) {
+    if (int r = check_ctx(c, false, false)) return r;
+    if (int r = check_paged(p)) return r;
+    if (int r = check_entries(slots, cu, n)) return r;
+    return paged_call(c, "paged_extend", n, [&] { return launch_paged_extend(*p, slots, cu, n, c->stream); });
+}
+
+int hymt_paged_fork(hymt_ctx *c, const hymt_paged *p, const int32_t *parent, const int32_t *child, int n) {
+    if (int r = check_ctx(c, false, false)) return r;
+    if (int r = check_paged(p)) return r;
+    if (int r = check_entries(parent, child, n)) return r;
+    if (!child) return fail(HYMT_E_ARG, "null entries");
+    return paged_call(c, "paged_fork", n, [&] { return launch_paged_fork(*p, parent, child, n, c->stream); });
+}
+
+int hymt_paged_set_len(hymt_ctx *c, const hymt_paged *p, const int32_t *slots, const int32_t *lens, int n) {
+    if (int r = check_ctx(c, false, false)) return r;
+    if (int r = check_paged(p)) return r;
+    if (int r = check_entries(slots, lens, n)) return r;
+    return paged_call(c, "paged_set_len", n, [&] { return launch_paged_set_len(*p, slots, lens, n, c->stream); });
+}
+
+int hymt_paged_compact(hymt_ctx *c, const hymt_paged *p) {
+    if (int r = check_ctx(c, false, false)) return r;
+    if (int r = check_paged(p)) return r;
+    return paged_call(c, "paged_compact", p->pages, [&] { return launch_paged_compact(*p, c->stream); });
+}
+
+int hymt_rope_freqs(int dim, double base, int scaling, double factor, int trained, double *freq, float *scale) {
+    if (!freq || !scale) return fail(HYMT_E_ARG, "null freq or scale");
+    if (dim < 2 || dim % 2 != 0) return fail(HYMT_E_ARG, "dim must be even and positive");
+    if (!(base > 1.0) || !std::isfinite(base)) return fail(HYMT_E_ARG, "base must be above 1");
+    if (scaling < HYMT_ROPE_NONE || scaling > HYMT_ROPE_YARN) return fail(HYMT_E_UNSUPPORTED, "unknown rope scaling");
+    if (scaling != HYMT_ROPE_NONE && (!(factor >= 1.0) || !std::isfinite(factor)))
+        return fail(HYMT_E_ARG, "factor must be 1 at least");
+    if (scaling == HYMT_ROPE_YARN && trained < 1) return fail(HYMT_E_ARG, "trained must be positive");
+    const int half = dim / 2;
+    if (scaling == HYMT_ROPE_NTK && dim > 2) base *= std::pow(factor, (double)dim / (dim - 2));
+    // the pair that turns `turns` times within the trained length
+    auto pair_of = [&](double turns) { return dim * std::log(trained / (turns * 2 * M_PI)) / (2 * std::log(base)); };
+    double lo = 0, hi = 0;
+    if (scaling == HYMT_ROPE_YARN) {
+        lo = std::max(std::floor(pair_of(32.0)), 0.0);
+        hi = std::min(std::ceil(pair_of(1.0)), (double)dim - 1);
+    }
+    for (int i = 0; i < half; i++) {
+        double f = std::pow(base, -2.0 * i / dim);
+        if (scaling == HYMT_ROPE_LINEAR) f /= factor;
+        if (scaling == HYMT_ROPE_YARN) {
+            const double r = std::min(std::max((i - lo) / std::max(hi - lo, 1e-3), 0.0), 1.0);
+            f = f / factor * r + f * (1 - r);
+        }
+        freq[i] = f;
+    }
+    *scale = scaling == HYMT_ROPE_YARN ? (float)(0.1 * std::log(factor) + 1.0) : 1.0f;
+    return HYMT_OK;
+}
+
+int hymt_rope_append(hymt_ctx *c, const hymt_paged *p, int layer, const hymt_batch *b, const void *q, int q_ld,
+                     const void *k, const void *v, int kv_ld, int io_dtype, int heads, const hymt_rope *rope,
+                     const float *qnw, const float *knw, float eps, void *q_out) {
+    if (int r = check_ctx(c, false, false)) return r;
+    if (int r = check_paged(p)) return r;
+    if (int r = check_batch(b)) return r;
+    if (int r = check_heads(p, layer, heads)) return r;
+    if (!q || !k || !v || !q_out || !rope) return fail(HYMT_E_ARG, "null tensor or rope");
+    if (io_dtype != HYMT_F32 && io_dtype != HYMT_F16 && io_dtype != HYMT_BF16)
+        return fail(HYMT_E_UNSUPPORTED, "q, k and v must be fp32, fp16 or bf16");
+    if (rope->dim < 0 || rope->dim > p->head_dim || rope->dim % 16 != 0)
+        return fail(HYMT_E_UNSUPPORTED, "rope dim must be a multiple of 16 up to head_dim");
+    if (rope->dim > 0 && !rope->freq) return fail(HYMT_E_ARG, "null rope frequencies");
+    if (misaligned(rope->freq, 8)) return fail(HYMT_E_ARG, "rope frequencies must be 8-byte aligned");
+    if ((rope->interleaved != 0 && rope->interleaved != 1) || rope->reserved != 0)
+        return fail(HYMT_E_ARG, "interleaved must be 0 or 1, reserved fields 0");
+    if ((int64_t)q_ld < (int64_t)heads * p->head_dim || kv_ld < p->kv_heads * p->head_dim || q_ld % 8 || kv_ld % 8)
+        return fail(HYMT_E_ARG, "rows must be at least a row's values apart, by multiples of 8");
+    if (!(eps >= 0.f)) return fail(HYMT_E_ARG, "eps must not be negative");
+    if (misaligned16(q) || misaligned16(k) || misaligned16(v) || misaligned16(q_out) || misaligned16(qnw) || misaligned16(knw))
+        return fail(HYMT_E_ARG, "q, k, v, q_out and the norms must be 16-byte aligned");
+    const RopeAppend a{q, k, v, q_ld, kv_ld, io_dtype, heads, layer, rope->freq, rope->dim, rope->interleaved, rope->scale,
+                       qnw, knw, eps, q_out};
+    return paged_call(c, "rope_append", b->rows, [&] { return launch_rope_append(*p, *b, a, c->stream); });
+}
+
+int hymt_attn_packed(hymt_ctx *c, const hymt_paged *p, int layer, const hymt_batch *b, const void *q, int heads,
+                     float scale, void *out, int out_dtype) {
+    return paged_attention(c, p, layer, b, 0, q, heads, scale, out, out_dtype, false);
+}
+
+int hymt_attn_shared(hymt_ctx *c, const hymt_paged *p, int layer, const hymt_batch *b, int prefix, const void *q,
+                     int heads, float scale, void *out, int out_dtype) {
+    return paged_attention(c, p, layer, b, prefix, q, heads, scale, out, out_dtype, true);
 }
 
 // ---- the decode step of the model, enqueued natively -------------------------

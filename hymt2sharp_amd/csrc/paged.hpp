@@ -1,0 +1,59 @@
+// paged.hpp -- the multi-sequence cache's operators: upkeep of its pages and
+// the rotary append (paged_ops.hip), attention over it (paged_attn.hip).  The
+// structs are the C ABI's own (include/hymt_hip.h); what stands in device memory
+// is checked by the kernels, everything else by the callers of these launchers.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/hymt_hip.h"
+#include "device_common.hpp"
+
+namespace hymt {
+
+constexpr int kPagedMaxGroup = 64;      // q heads per kv head
+constexpr int kPagedMaxSeqs = 65536;    // slots (one bit each in the plan kernels' LDS)
+constexpr int kPagedMaxBlocks = 1 << 24;  // positions stay below 2^30
+
+// fp32 to an element of the cache, nearest even by the hardware's conversion (a
+// NaN stays one)
+template <typename T> __device__ __forceinline__ uint16_t bits_of(float x);
+template <> __device__ __forceinline__ uint16_t bits_of<F16>(float x) { return f32_to_f16(x); }
+template <> __device__ __forceinline__ uint16_t bits_of<BF16>(float x) {
+    return __builtin_bit_cast(uint16_t, (__bf16)x);
+}
+
+// words of hymt_paged::work
+enum { kWorkFirst = 0, kWorkCopies = 1, kWorkLive = 2, kWorkStatus = 3, kWorkLists = 4 };
+
+struct RopeAppend {
+    const void *q, *k, *v;
+    int q_ld, kv_ld, io_dtype, heads, layer;
+    const double *freq;
+    int dim, interleaved;
+    float scale;
+    const float *qnw, *knw;
+    float eps;
+    void *q_out;
+};
+
+struct PagedAttn {
+    const void *q;
+    int heads, layer, prefix;
+    float scale;
+    void *out;
+    int out_dtype;
+};
+
+hipError_t launch_paged_extend(const hymt_paged &p, const int32_t *slots, const int32_t *cu, int n, hipStream_t s);
+hipError_t launch_paged_fork(const hymt_paged &p, const int32_t *parent, const int32_t *child, int n, hipStream_t s);
+hipError_t launch_paged_set_len(const hymt_paged &p, const int32_t *slots, const int32_t *lens, int n, hipStream_t s);
+hipError_t launch_paged_compact(const hymt_paged &p, hipStream_t s);
+hipError_t launch_rope_append(const hymt_paged &p, const hymt_batch &b, const RopeAppend &a, hipStream_t s);
+// fp32 values of workspace that the two launches below need at most
+size_t paged_attn_workspace(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, bool shared);
+hipError_t launch_attn_packed(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, float *ws, hipStream_t s);
+hipError_t launch_attn_shared(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, float *ws, hipStream_t s);
+
+}  // namespace hymt

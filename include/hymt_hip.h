@@ -233,8 +233,8 @@ int hymt_sync(hymt_ctx *ctx);
  * the context does not time, HYMT_E_ARG for a kernel never timed.  Kernel
  * names: decode_attn, decode_merge, prefill_kv, prefill_flash, prefill_merge,
  * gemv_<type>, gemm_bf16_out_{f32,bf16}, gemm_i8_out_{f32,bf16},
- * gemm_i8_swiglu, to_i8, rows_*, kv_*, embed, weight_rows, tab_update, graph
- * (a whole replay).
+ * gemm_i8_swiglu, to_i8, rows_*, kv_*, paged_*, rope_append, attn_packed,
+ * attn_shared, attn_merge, embed, weight_rows, tab_update, graph (a whole replay).
  */
 /* mode 0 stops timing (the totals are kept), 1 times and prints, 2 times
  * quietly; a device context only (HYMT_E_NO_DEVICE otherwise). */
@@ -446,6 +446,149 @@ int hymt_gemm_i8(hymt_ctx *ctx, const int8_t *w, const float *w_scale, int n, in
 int hymt_gemm_i8_swiglu(hymt_ctx *ctx, const int8_t *gate, const float *gate_scale, const int8_t *up,
                         const float *up_scale, int f, int k, const int8_t *x, const float *x_scale, int m,
                         void *act, int ld);
+
+/* ---- many sequences over one paged cache -----------------------------------------
+ * The cache of hymt_kv_create holds one sequence.  A server's batch of requests
+ * shares one pool of pages instead: a sequence is a slot, a row of the page
+ * table and a length, and several slots may hold the same page (a common
+ * instruction text, the beams of one request).  Pool, table, lengths and
+ * reference counts are device memory of the caller; the calls below only enqueue
+ * work on the context's stream and may be recorded, so a recorded step follows
+ * the lengths as they grow.  They have no counterpart in the reference, whose
+ * cache has one sequence; its block store and page table are the closest
+ * (MetalBackend.cs:44-61, 224-387).
+ *
+ * A page holds 64 positions of every kv head of one layer, for K and for V:
+ * page p of layer l starts at element ((l * pages + p) * kv_heads) * 64 * head_dim,
+ * kv head h at h * 64 * head_dim further, and there (D = head_dim)
+ *   K dim d of position t at (((t/16) * D/8 + d/8) * 16 + t%16) * 8 + d%8
+ *   V dim d of position t at ((4 (t/32) + t/4%4) * D + d) * 8 + 4 (t/16%2) + t%4
+ * (16-byte chunks in the operand order of the matrix instructions, as the
+ * pages of hymt_kv_create have them).
+ *
+ * Position q of slot s is row q % 64 of page table[s * blocks + q / 64], for
+ * q < len[s]; table entries past that are not read.  refs[p] is the number of table entries
+ * that hold page p; a page with none is free.  A sequence that ends inside a
+ * page holds that page alone (fork and set_len see to it), so a position is
+ * only ever written in a page of one sequence.
+ *
+ * To start: refs 0, len 0, work 0, table anything.
+ *
+ * work[0] keeps the status (hymt_status) of the first call that found something
+ * wrong on the device, until the caller clears it: HYMT_E_ARG a slot outside the
+ * cache, a slot twice, a falling cu; HYMT_E_CAPACITY too few free pages or more
+ * than blocks * 64 positions; HYMT_E_STATE a fork into a slot that is not empty, or a table
+ * entry, length or count that the rules above exclude.  Such a call changes
+ * nothing else.  work[1] is the number of pages that the last such call copied,
+ * work[2] the number of pages in use at the last compact, work[3] the last call's own
+ * status.
+ * The other calls' reads and writes stay inside the buffers whatever these hold:
+ * slots outside the cache count as empty, positions in pages outside the pool as
+ * absent. */
+#define HYMT_PAGED_WORK(pages) (4 + 3 * (size_t)(pages)) /* int32 values of work */
+#define HYMT_PAGED_BATCH 1024                            /* entries of one call  */
+
+typedef struct hymt_paged {
+    void *k, *v;       /* [layers][pages][kv_heads][64 * head_dim], 256-byte aligned */
+    int32_t *table;    /* [seqs][blocks]                                            */
+    int32_t *len;      /* [seqs]                                                    */
+    int32_t *refs;     /* [pages]                                                   */
+    int32_t *work;     /* [HYMT_PAGED_WORK(pages)]                                  */
+    int32_t layers, pages;
+    int32_t kv_heads;  /* 1 to 256                                                  */
+    int32_t head_dim;  /* 64 or 128                                                 */
+    int32_t dtype;     /* HYMT_F16 or HYMT_BF16                                     */
+    int32_t seqs;      /* slots, up to 65536                                        */
+    int32_t blocks;    /* pages that a sequence may have, up to 2^24                */
+    int32_t reserved;  /* 0                                                         */
+} hymt_paged;
+
+/* A batch of rows: entry i is slot slots[i] and has the rows [cu[i], cu[i+1]) of
+ * the packed tensors, or with cu NULL row i alone.  They are its last positions:
+ * row j of n stands at len - n + j.  Rows from cu[n] on belong to no entry and are
+ * left as they are. */
+typedef struct hymt_batch {
+    const int32_t *slots; /* device, [n]                                            */
+    const int32_t *cu;    /* device, [n + 1], rising from 0, or NULL                */
+    int32_t n;            /* entries, up to HYMT_PAGED_BATCH                        */
+    int32_t rows;         /* rows of the packed tensors, cu[n] at least (NULL: n)   */
+    int32_t max_len;      /* about the longest len, 0 if unknown: how the work is split
+                             goes by it, and no result but for its rounding         */
+    int32_t reserved;     /* 0                                                      */
+} hymt_batch;
+
+/* len[slots[i]] += cu[i+1] - cu[i] (cu NULL: 1), with free pages for the new
+ * positions, the lowest ones first. */
+int hymt_paged_extend(hymt_ctx *ctx, const hymt_paged *cache, const int32_t *slots, const int32_t *cu, int n);
+
+/* Slot child[i], empty so far, becomes a copy of parent[i] (which is no child of
+ * the same call): the same pages, but a page that the sequence ends inside is
+ * copied, in every layer. */
+int hymt_paged_fork(hymt_ctx *ctx, const hymt_paged *cache, const int32_t *parent, const int32_t *child, int n);
+
+/* Slot slots[i] keeps its first min(len, lens[i]) positions (lens NULL: none, the
+ * slot is free again): pages past them are given up, and one that the rest ends
+ * inside is copied if another sequence holds it too.  The counterpart of
+ * hymt_kv_set_len. */
+int hymt_paged_set_len(hymt_ctx *ctx, const hymt_paged *cache, const int32_t *slots, const int32_t *lens, int n);
+
+/* The pages in use become the first ones of the pool: the k-th page in use past
+ * their number moves to the k-th free page below it, in every layer, and the
+ * table follows. */
+int hymt_paged_compact(hymt_ctx *ctx, const hymt_paged *cache);
+
+/* Rotary positions: pair t < dim / 2 of a head, (t, t + dim / 2) or with
+ * interleaved (2t, 2t + 1), turns by position * freq[t] radians (formed in fp64),
+ * cosine and sine times scale; dims from dim on stay. */
+typedef struct hymt_rope {
+    const double *freq;  /* device, [dim / 2]; NULL with dim 0                      */
+    int32_t dim;         /* a multiple of 16, 0 to head_dim                         */
+    int32_t interleaved; /* 0 or 1                                                  */
+    float scale;
+    int32_t reserved;    /* 0                                                       */
+} hymt_rope;
+
+/* freq[dim / 2] (host) and *scale for base^(-2t/dim), and with factor > 1 for
+ * contexts that much longer than the `trained` positions: HYMT_ROPE_LINEAR divides
+ * every frequency, HYMT_ROPE_NTK enlarges the base by factor^(dim/(dim-2)) (the
+ * reference's alpha, ModelConfig.cs:31-34), HYMT_ROPE_YARN divides those of pairs
+ * that turn less than once in the trained length, keeps those that turn more than
+ * 32 times, blends between, and sets *scale = 0.1 ln(factor) + 1 (else 1). */
+#define HYMT_ROPE_NONE 0
+#define HYMT_ROPE_LINEAR 1
+#define HYMT_ROPE_NTK 2
+#define HYMT_ROPE_YARN 3
+int hymt_rope_freqs(int dim, double base, int scaling, double factor, int trained, double *freq, float *scale);
+
+/* For every row of the batch: q_out[row][heads * D] = q after the rotation and, with
+ * qnw, x / sqrt(mean(x^2) + eps) * qnw per head, in the cache's type; k likewise
+ * (knw) and v as it is, rounded into layer `layer` of the pages.  q, k and v are
+ * HYMT_F32, HYMT_F16 or HYMT_BF16 as io_dtype, rows q_ld >= heads * D and kv_ld >=
+ * kv_heads * D elements apart (both multiples of 8); q, k, v, q_out, qnw and knw
+ * [D] (fp32, NULL for none) 16-byte aligned.  heads is a multiple of kv_heads, up to 64
+ * times.  A slot stands once in the batch (else which of its rows is stored is
+ * open).  Pages for the positions are there already (hymt_paged_extend).  The
+ * counterpart of what hymt_attn_prefill does before its products. */
+int hymt_rope_append(hymt_ctx *ctx, const hymt_paged *cache, int layer, const hymt_batch *batch, const void *q,
+                     int q_ld, const void *k, const void *v, int kv_ld, int io_dtype, int heads,
+                     const hymt_rope *rope, const float *qnw, const float *knw, float eps, void *q_out);
+
+/* out[row] = softmax(scale q K^T) V per head over the row's positions up to its
+ * own, of the cache's layer `layer` (q [rows][heads * D] in the cache's type, as
+ * hymt_rope_append leaves it; kv head h serves heads / kv_heads heads in turn).
+ * out is HYMT_F16 or HYMT_BF16 [rows][heads * D].  A row without positions gives 0; what stands in the
+ * pages where a row does not attend, infinities and NaN too, does not reach it.
+ * Softmax and sums in fp32, its weights rounded to the cache's type for the
+ * products with V.  q and out 16-byte aligned. */
+int hymt_attn_packed(hymt_ctx *ctx, const hymt_paged *cache, int layer, const hymt_batch *batch, const void *q,
+                     int heads, float scale, void *out, int out_dtype);
+
+/* The same for one row per entry (cu NULL) where every entry's first `prefix`
+ * positions (a multiple of 64, 0 for none) are those of slots[0], as far as its
+ * whole pages go: they are read from its pages, once for all entries, the others from
+ * each one's own.  (After a fork the pages are the same.) */
+int hymt_attn_shared(hymt_ctx *ctx, const hymt_paged *cache, int layer, const hymt_batch *batch, int prefix,
+                     const void *q, int heads, float scale, void *out, int out_dtype);
 
 /* ---- the model's decode step, enqueued natively ---------------------------------
  * IComputeBackend.ForwardStep for one token (IComputeBackend.cs:40-47) in one
