@@ -1555,14 +1555,15 @@ int check_batch(const hymt_batch *b) {
     if (b->rows < 0 || b->max_len < 0 || b->reserved != 0)
         return fail(HYMT_E_ARG, "rows and max_len must not be negative, reserved fields 0");
     if (!b->cu && b->rows != b->n) return fail(HYMT_E_ARG, "without cu a batch has as many rows as entries");
-    if (b->rows > 1 << 24) return fail(HYMT_E_UNSUPPORTED, "more than 2^24 rows");
+    if (b->rows > 1 << 22) return fail(HYMT_E_UNSUPPORTED, "more than 2^22 rows");
     return HYMT_OK;
 }
 
-int check_heads(const hymt_paged *p, int layer, int heads) {
+int check_heads(const hymt_paged *p, const hymt_batch *b, int layer, int heads) {
     if (layer < 0 || layer >= p->layers) return fail(HYMT_E_ARG, "layer outside the cache");
     if (heads < 1 || heads % p->kv_heads != 0) return fail(HYMT_E_ARG, "heads must be a multiple of kv_heads");
     if (heads / p->kv_heads > kPagedMaxGroup) return fail(HYMT_E_UNSUPPORTED, "more than 64 heads per kv head");
+    if ((int64_t)b->rows * heads > 1 << 30) return fail(HYMT_E_UNSUPPORTED, "more than 2^30 rows of all heads");
     return HYMT_OK;
 }
 
@@ -1584,7 +1585,7 @@ int paged_attention(hymt_ctx *c, const hymt_paged *p, int layer, const hymt_batc
     if (int r = check_ctx(c, false, false)) return r;
     if (int r = check_paged(p)) return r;
     if (int r = check_batch(b)) return r;
-    if (int r = check_heads(p, layer, heads)) return r;
+    if (int r = check_heads(p, b, layer, heads)) return r;
     if (shared && b->cu) return fail(HYMT_E_ARG, "the batch must have one row per entry (cu NULL)");
     if (prefix < 0 || prefix % kPage != 0) return fail(HYMT_E_ARG, "prefix must be a multiple of 64");
     if (!q || !out) return fail(HYMT_E_ARG, "null q or out");
@@ -1667,7 +1668,7 @@ int hymt_rope_append(hymt_ctx *c, const hymt_paged *p, int layer, const hymt_bat
     if (int r = check_ctx(c, false, false)) return r;
     if (int r = check_paged(p)) return r;
     if (int r = check_batch(b)) return r;
-    if (int r = check_heads(p, layer, heads)) return r;
+    if (int r = check_heads(p, b, layer, heads)) return r;
     if (!q || !k || !v || !q_out || !rope) return fail(HYMT_E_ARG, "null tensor or rope");
     if (io_dtype != HYMT_F32 && io_dtype != HYMT_F16 && io_dtype != HYMT_BF16)
         return fail(HYMT_E_UNSUPPORTED, "q, k and v must be fp32, fp16 or bf16");
