@@ -438,26 +438,27 @@ hipError_t launch_paged_compact(const hymt_paged &p, hipStream_t s) {
 
 namespace {
 
-// Entry of row r: the last i with cu[i] <= r.  Lanes of a wave look at 64
-// entries at a time (one load each, no chain of dependent ones).
-__device__ __forceinline__ int entry_of_row(const int32_t *cu, int n, int r) {
-    const int lane = threadIdx.x & 63;
-    int below = 0;  // entries whose end is at or before r
-    for (int base = 0; base < n; base += 64) {
-        const int i = base + lane;
-        below += __popcll(__ballot(i < n && cu[i + 1] <= r));
-    }
-    return below;
+// 8 values of a row as loaded (16 bytes, fp32 32), and in fp32.
+template <typename IO> struct Raw8 {
+    uint4 u[IO::kBytes / 2];
+};
+template <typename IO> __device__ __forceinline__ Raw8<IO> load8(const void *base, size_t i) {
+    Raw8<IO> r;
+#pragma unroll
+    for (int k = 0; k < IO::kBytes / 2; k++) r.u[k] = *(const uint4 *)((const char *)base + i * IO::kBytes + 16 * k);
+    return r;
 }
-
-template <typename IO> __device__ __forceinline__ void load8(const void *base, size_t i, float *o) {
+template <typename IO> __device__ __forceinline__ void values8(const Raw8<IO> &r, float *o) {
     if constexpr (IO::kBytes == 4) {
-        const float4 a = *(const float4 *)((const float *)base + i), b = *(const float4 *)((const float *)base + i + 4);
-        o[0] = a.x; o[1] = a.y; o[2] = a.z; o[3] = a.w;
-        o[4] = b.x; o[5] = b.y; o[6] = b.z; o[7] = b.w;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            o[4 * k] = __uint_as_float(r.u[k].x);
+            o[4 * k + 1] = __uint_as_float(r.u[k].y);
+            o[4 * k + 2] = __uint_as_float(r.u[k].z);
+            o[4 * k + 3] = __uint_as_float(r.u[k].w);
+        }
     } else {
-        const uint4 u = *(const uint4 *)((const uint16_t *)base + i);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        const uint32_t w[4] = {r.u[0].x, r.u[0].y, r.u[0].z, r.u[0].w};
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             o[2 * e] = from_elem<IO>((uint16_t)w[e]);
@@ -465,104 +466,310 @@ template <typename IO> __device__ __forceinline__ void load8(const void *base, s
         }
     }
 }
+template <typename T> __device__ __forceinline__ uint4 pack8(const float *x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) w[e] = bits_of<T>(x[2 * e]) | (uint32_t)bits_of<T>(x[2 * e + 1]) << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
-// One workgroup per row: cosines and sines of the row's position once into
-// LDS, then D / 8 lanes per head (8 dims each) over q, k and v heads.
-template <typename T, typename IO, int D>
-__global__ __launch_bounds__(256) void rope_append_kernel(hymt_paged p, hymt_batch b, RopeAppend a) {
+// (cosine, sine) of position * freq, times scale.  The angle is formed in
+// revolutions in fp64, where the product is good to 2^-53 of itself at any
+// position, and only its fraction goes on in fp32.
+__device__ __forceinline__ float2 turn_of(int pos, double freq, float scale) {
+    const double turn = (double)pos * freq * 0.15915494309189535;
+    float sn, cs;
+    sincospif((float)(turn - rint(turn)) * 2.0f, &sn, &cs);
+    return make_float2(cs * scale, sn * scale);
+}
+
+// What a lane (8 dims from d0 = 8 c of a head) needs of its row's turns: the pairs of
+// its dims, interleaved the 4 it holds whole, else the 8 that it holds one half of.
+struct Turns {
+    float cs[8], sn[8];
+};
+__device__ __forceinline__ Turns turns_of(const float2 *row, int c, const RopeAppend &a) {
+    const int d0 = 8 * c, half = a.dim / 2;
+    Turns t;
+    const float2 *at = row + (d0 >= a.dim ? 0 : a.interleaved ? d0 / 2 : d0 < half ? d0 : d0 - half);
+    const int n = d0 >= a.dim ? 0 : a.interleaved ? 4 : 8;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float2 x = e < n ? at[e] : make_float2(1.f, 0.f);
+        t.cs[e] = x.x;
+        // the second of a pair adds what the first takes away
+        t.sn[e] = !a.interleaved && d0 < half ? -x.y : x.y;
+    }
+    return t;
+}
+
+// y = x of lane c +- hc (half / 8) of the head's lanes: by DPP at the usual sizes
+template <int CTRL> __device__ __forceinline__ float dpp_from(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ void partners(const float *x, float *y, int c, int hc, int other) {
+    if (hc == 8) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = dpp_from<0x128>(x[e]);  // turned by 8
+    } else if (hc == 4) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float up = dpp_from<0x104>(x[e]), dn = dpp_from<0x114>(x[e]);  // from lanes + 4 and - 4
+            y[e] = c & 4 ? dn : up;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = __shfl(x[e], other);
+    }
+}
+
+// Sum over the L = 8 or 16 neighbouring lanes of a head.
+template <int L> __device__ __forceinline__ float lanes_sum(float v) {
+    if constexpr (L == 16) return dpp_sum16(v);
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, false));
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, false));
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, false));
+    return v;
+}
+
+// 8 dims of a head, L = D / 8 neighbouring lanes holding it whole: rotation,
+// then RMSNorm with the lane's weights g where the head has one.
+template <int D>
+__device__ __forceinline__ void rotate_norm(float *x, int c, const Turns &t, const RopeAppend &a, bool norm, const float *g) {
     constexpr int L = D / 8;
-    __shared__ float s_cos[64], s_sin[64];
+    const int d0 = 8 * c;
+    if (a.interleaved) {
+        if (d0 < a.dim)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float y0 = x[2 * e], y1 = x[2 * e + 1];
+                x[2 * e] = y0 * t.cs[e] - y1 * t.sn[e];
+                x[2 * e + 1] = y1 * t.cs[e] + y0 * t.sn[e];
+            }
+    } else if (a.dim) {
+        const int hc = a.dim / 16;
+        const int other = (int)(threadIdx.x & 63) + (d0 >= a.dim ? 0 : c < hc ? hc : -hc);
+        float y[8];
+        partners(x, y, c, hc, other);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = d0 < a.dim ? x[e] * t.cs[e] + y[e] * t.sn[e] : x[e];
+    }
+    if (norm) {
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) ss += x[e] * x[e];
+        const float r = __builtin_amdgcn_rsqf(lanes_sum<L>(ss) * (1.0f / D) + a.eps);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = x[e] * r * g[e];
+    }
+}
+
+// The norm's weights of a lane's dims.
+__device__ __forceinline__ void weights8(const float *w, int d0, float *g) {
+    if (!w) return;
+    const float4 w0 = *(const float4 *)(w + d0), w1 = *(const float4 *)(w + d0 + 4);
+    g[0] = w0.x; g[1] = w0.y; g[2] = w0.z; g[3] = w0.w;
+    g[4] = w1.x; g[5] = w1.y; g[6] = w1.z; g[7] = w1.w;
+}
+
+__device__ __forceinline__ int slot_length(const hymt_paged &p, int slot) {
+    return (unsigned)slot < (unsigned)p.seqs ? max(0, min(p.len[slot], 1 << 30)) : 0;
+}
+
+// The entry of row r, its slot and its rows from r on.  Lanes look at 64 entries
+// at a time, end and slot in one round trip.
+struct RowEntry {
+    int slot, behind;
+};
+__device__ __forceinline__ bool entry_of_row(const hymt_batch &b, int r, RowEntry &out) {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0; base < b.n; base += 64) {
+        const int i = min(base + lane, b.n - 1);
+        const int end = b.cu[i + 1], slot = b.slots[i];
+        const uint64_t hit = __ballot(base + lane < b.n && end > r);
+        if (hit) {
+            const int k = __ffsll((unsigned long long)hit) - 1;
+            out = {__builtin_amdgcn_readlane(slot, k), __builtin_amdgcn_readlane(end, k) - r};
+            return true;
+        }
+    }
+    return false;
+}
+
+// A workgroup a row, for batches of few rows an entry.  q, k and v do not wait for the
+// row's position, so they are loaded first.
+template <typename T, typename IO, int D>
+__global__ __launch_bounds__(256) void rope_row_kernel(hymt_paged p, hymt_batch b, RopeAppend a) {
+    constexpr int L = D / 8, U = 256 / L;
+    __shared__ float2 s_cs[D / 2];
     const int row = blockIdx.x;
-    int entry = row;
-    int n_rows = 1, j = 0;
-    if (b.cu) {
-        entry = entry_of_row(b.cu, b.n, row);
-        if (entry >= b.n) return;
-        n_rows = b.cu[entry + 1] - b.cu[entry];
-        j = row - b.cu[entry];
-    }
-    if (entry >= b.n) return;
-    const int slot = b.slots[entry];
-    const bool known = (unsigned)slot < (unsigned)p.seqs;
-    const int pos = (known ? p.len[slot] : 0) - n_rows + j;
-    const int half = a.dim / 2;
-    if ((int)threadIdx.x < half) {
-        // revolutions in fp64, whose fraction is what counts at far positions
-        const double turn = (double)pos * a.freq[threadIdx.x] * 0.15915494309189535;
-        const float x = (float)(turn - rint(turn)) * 2.0f;
-        float sn, cs;
-        sincospif(x, &sn, &cs);
-        s_cos[threadIdx.x] = cs * a.scale;
-        s_sin[threadIdx.x] = sn * a.scale;
-    }
-    __syncthreads();
-    const bool stored = known && pos >= 0 && pos < (long)p.blocks * kPage;
-    int page = stored ? p.table[(size_t)slot * p.blocks + pos / kPage] : -1;
-    const bool in_pool = (unsigned)page < (unsigned)p.pages;
-    const int t = pos & (kPage - 1);
     const int c = threadIdx.x & (L - 1), d0 = 8 * c;
     const int units = a.heads + 2 * p.kv_heads;
-    for (int base = 0; base < units; base += 256 / L) {
-        const int u = base + threadIdx.x / L;
-        const bool on = u < units;
-        const int uc = on ? u : units - 1;
-        const bool isq = uc < a.heads, isv = uc >= a.heads + p.kv_heads;
-        const int h = isq ? uc : isv ? uc - a.heads - p.kv_heads : uc - a.heads;
-        float x[8];
-        load8<IO>(isq ? a.q : isv ? a.v : a.k, (size_t)row * (isq ? a.q_ld : a.kv_ld) + (size_t)h * D + d0, x);
-        if (!isv) {
-            if (a.interleaved) {
-                if (d0 < a.dim)
+    auto load = [&](int u) __attribute__((always_inline)) {
+        u = min(u, units - 1);
+        const bool isq = u < a.heads, isv = u >= a.heads + p.kv_heads;
+        const int h = isq ? u : isv ? u - a.heads - p.kv_heads : u - a.heads;
+        return load8<IO>(isq ? a.q : isv ? a.v : a.k, (size_t)row * (isq ? a.q_ld : a.kv_ld) + (size_t)h * D + d0);
+    };
+    const int u0 = threadIdx.x / L;
+    Raw8<IO> next = load(u0), after = load(u0 + U);
+    const double freq = (int)threadIdx.x < a.dim / 2 ? a.freq[threadIdx.x] : 0.0;
+    RowEntry e{0, 1};
+    if (!b.cu) e.slot = b.slots[row];
+    else if (!entry_of_row(b, row, e)) return;
+    const int slot = e.slot, pos = slot_length(p, slot) - e.behind;
+    if ((int)threadIdx.x < a.dim / 2) s_cs[threadIdx.x] = turn_of(pos, freq, a.scale);
+    const bool stored = pos >= 0 && pos < (long)p.blocks * kPage;
+    const int page = stored ? p.table[(size_t)slot * p.blocks + pos / kPage] : -1;
+    const bool in_pool = (unsigned)page < (unsigned)p.pages;
+    const int t = pos & (kPage - 1);
+    float gq[8] = {}, gk[8] = {};
+    weights8(a.qnw, d0, gq);
+    weights8(a.knw, d0, gk);
+    __syncthreads();
+    const Turns turns = turns_of(s_cs, c, a);
+    for (int base = 0; base < units; base += U) {
+        const int u = base + u0;
+        const bool isq = u < a.heads, isv = u >= a.heads + p.kv_heads;
+        float x[8], y[8];
+        values8<IO>(next, x);
+        next = after;
+        if (base + 2 * U < units) after = load(u + 2 * U);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float cs = s_cos[d0 / 2 + e], sn = s_sin[d0 / 2 + e], y0 = x[2 * e], y1 = x[2 * e + 1];
-                        x[2 * e] = y0 * cs - y1 * sn;
-                        x[2 * e + 1] = y1 * cs + y0 * sn;
-                    }
-            } else {
-                const bool low = d0 < half;
-                const int other = (int)(threadIdx.x & 63) + (d0 >= a.dim ? 0 : low ? half / 8 : -(half / 8));
+        for (int e = 0; e < 8; e++) y[e] = x[e];
+        float g[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float y = __shfl(x[e], other);
-                    if (d0 < a.dim) {
-                        const int i = low ? d0 + e : d0 - half + e;
-                        x[e] = low ? x[e] * s_cos[i] - y * s_sin[i] : x[e] * s_cos[i] + y * s_sin[i];
-                    }
-                }
-            }
-            const float *w = isq ? a.qnw : a.knw;
-            if (w) {
-                float ss = 0.f;
+        for (int e = 0; e < 8; e++) g[e] = isq ? gq[e] : gk[e];
+        rotate_norm<D>(y, c, turns, a, (isq ? a.qnw : a.knw) != nullptr, g);
+        if (u >= units) continue;
+        const int h = isq ? u : isv ? u - a.heads - p.kv_heads : u - a.heads;
+        const size_t at = (((size_t)a.layer * p.pages + page) * p.kv_heads + h) * (size_t)(kPage * D);
+        if (isq) {
+            *(uint4 *)((uint16_t *)a.q_out + (size_t)row * a.heads * D + (size_t)h * D + d0) = pack8<T>(y);
+        } else if (in_pool && !isv) {
+            *(uint4 *)((uint16_t *)p.k + at + ((((size_t)(t >> 4) * L + c) * 16 + (t & 15)) << 3)) = pack8<T>(y);
+        } else if (in_pool) {
+            const int pc = 4 * (t >> 5) + ((t >> 2) & 3), e0 = 4 * ((t >> 4) & 1) + (t & 3);
+            uint16_t *vp = (uint16_t *)p.v + at + ((size_t)pc * D + d0) * 8 + e0;
 #pragma unroll
-                for (int e = 0; e < 8; e++) ss += x[e] * x[e];
-#pragma unroll
-                for (int m = 1; m < L; m <<= 1) ss += __shfl_xor(ss, m);
-                const float r = 1.0f / sqrtf(ss / (float)D + a.eps);
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = x[e] * r * w[d0 + e];
-            }
+            for (int e = 0; e < 8; e++) vp[8 * e] = bits_of<T>(x[e]);
         }
-        uint16_t y[8];
+    }
+}
+
+// Packed rows: a workgroup takes the rows of one entry that lie in one block of 32
+// positions, for one kv head with its q heads.  A V chunk holds 8 of the block's
+// positions, so the block writes its chunks whole, 16 bytes a thread, after a
+// turn through LDS; row by row each chunk was written in 8 pieces, by
+// workgroups on 8 XCDs.
+constexpr int kRopeRows = 32;
+constexpr int kRopeFew = 8;  // fewer rows an entry than this: row by row
+
+template <typename T, typename IO, int D>
+__global__ __launch_bounds__(256) void rope_block_kernel(hymt_paged p, hymt_batch b, RopeAppend a) {
+    constexpr int L = D / 8, RP = 256 / L, PASSES = kRopeRows / RP;
+    __shared__ float2 s_cs[kRopeRows][D / 2];
+    __shared__ __attribute__((aligned(16))) uint16_t s_v[kRopeRows][D + 8];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int h = blockIdx.x % p.kv_heads, w = blockIdx.x / p.kv_heads;
+    // ---- the block's entry: 64 entries at a time, one a lane
+    int slot = -1, row0 = 0, n = 0, p0 = 0, index = -1;  // first row, rows, their first position, block of it
+    for (int base = 0, before = 0; base < b.n; base += 64) {
+        const int i = base + lane;
+        int lo = 0, cnt = 0, sl = -1;
+        if (i < b.n) {
+            lo = max(0, min(b.cu[i], b.rows));
+            cnt = max(lo, min(b.cu[i + 1], b.rows)) - lo;
+            sl = b.slots[i];
+        }
+        const int at = slot_length(p, sl) - cnt;
+        const int blocks = cnt ? ((at + cnt - 1) >> 5) - (at >> 5) + 1 : 0;
+        int x = blocks;
 #pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = bits_of<T>(x[e]);
-        if (!on) continue;
-        if (isv) {
-            if (in_pool) {
-                uint16_t *vp = (uint16_t *)p.v + (((size_t)a.layer * p.pages + page) * p.kv_heads + h) * (kPage * D);
-                const int pc = 4 * (t >> 5) + ((t >> 2) & 3), e0 = 4 * ((t >> 4) & 1) + (t & 3);
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl_up(x, d);
+            if (lane >= d) x += y;
+        }
+        const uint64_t hit = __ballot(w < before + x);
+        if (hit) {
+            const int k = __ffsll((unsigned long long)hit) - 1;
+            slot = __builtin_amdgcn_readlane(sl, k);
+            row0 = __builtin_amdgcn_readlane(lo, k);
+            n = __builtin_amdgcn_readlane(cnt, k);
+            p0 = __builtin_amdgcn_readlane(at, k);
+            index = w - before - (__builtin_amdgcn_readlane(x, k) - __builtin_amdgcn_readlane(blocks, k));
+            break;
+        }
+        before += __builtin_amdgcn_readlane(x, 63);
+    }
+    if (index < 0) return;
+    const int pb = ((p0 >> 5) + index) * 32;  // position of the block's first row
+    const int r_lo = max(0, p0 - pb), r_hi = min(kRopeRows, p0 + n - pb);
+    const bool stored = slot >= 0 && slot < p.seqs && pb >= 0 && pb < (long)p.blocks * kPage;
+    const int page = stored ? p.table[(size_t)slot * p.blocks + pb / kPage] : -1;
+    const bool in_pool = (unsigned)page < (unsigned)p.pages;
+    const int c = tid & (L - 1), d0 = 8 * c, r0 = tid / L;
+    const int group = a.heads / p.kv_heads, items = (group + 2) * PASSES;
+    auto load = [&](int item) __attribute__((always_inline)) {
+        const int u = item / PASSES, r = r0 + item % PASSES * RP;
+        const size_t row = row0 + max(0, min(pb + r - p0, n - 1));  // rows outside are loaded for nothing, from inside
+        const bool isq = u < group;
+        return load8<IO>(isq ? a.q : u == group ? a.k : a.v,
+                         row * (isq ? a.q_ld : a.kv_ld) + (size_t)(isq ? h * group + u : h) * D + d0);
+    };
+    Raw8<IO> next = load(0), after = load(1);
+    const int half = a.dim / 2;
+    for (int i = tid; i < (r_hi - r_lo) * half; i += 256) {
+        const int r = r_lo + i / half, k = i % half;
+        s_cs[r][k] = turn_of(pb + r, a.freq[k], a.scale);
+    }
+    float gq[8] = {}, gk[8] = {};
+    weights8(a.qnw, d0, gq);
+    weights8(a.knw, d0, gk);
+    __syncthreads();
+    const size_t at = (((size_t)a.layer * p.pages + page) * p.kv_heads + h) * (size_t)(kPage * D);
+    Turns turns[PASSES];
 #pragma unroll
-                for (int e = 0; e < 8; e++) vp[((size_t)pc * D + d0 + e) * 8 + e0] = y[e];
-            }
+    for (int k = 0; k < PASSES; k++) turns[k] = turns_of(s_cs[r0 + k * RP], c, a);
+    for (int first = 0; first < items; first += PASSES)
+#pragma unroll
+    for (int pass = 0; pass < PASSES; pass++) {
+        const int item = first + pass, u = item / PASSES, r = r0 + pass * RP, t = (pb + r) & (kPage - 1);
+        float x[8];
+        values8<IO>(next, x);
+        next = after;
+        if (item + 2 < items) after = load(item + 2);
+        if (u > group) {
+            *(uint4 *)&s_v[r][d0] = pack8<T>(x);
             continue;
         }
-        const uint4 w = make_uint4(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16, y[4] | (uint32_t)y[5] << 16,
-                                   y[6] | (uint32_t)y[7] << 16);
-        if (isq) {
-            *(uint4 *)((uint16_t *)a.q_out + (size_t)row * a.heads * D + (size_t)h * D + d0) = w;
-        } else if (in_pool) {
-            uint16_t *kp = (uint16_t *)p.k + (((size_t)a.layer * p.pages + page) * p.kv_heads + h) * (kPage * D);
-            *(uint4 *)(kp + ((((size_t)(t >> 4) * L + c) * 16 + (t & 15)) << 3)) = w;
+        if (u < group) rotate_norm<D>(x, c, turns[pass], a, a.qnw != nullptr, gq);
+        else rotate_norm<D>(x, c, turns[pass], a, a.knw != nullptr, gk);
+        if (r < r_lo || r >= r_hi) continue;
+        if (u < group)
+            *(uint4 *)((uint16_t *)a.q_out + (size_t)(row0 + pb + r - p0) * a.heads * D + (size_t)(h * group + u) * D + d0) =
+                pack8<T>(x);
+        else if (in_pool)
+            *(uint4 *)((uint16_t *)p.k + at + ((((size_t)(t >> 4) * L + c) * 16 + (t & 15)) << 3)) = pack8<T>(x);
+    }
+    __syncthreads();
+    if (!in_pool) return;
+    // ---- V chunks (4 m + g, d), m the block's half of the page
+    for (int i = tid; i < 4 * D; i += 256) {
+        const int g = i / D, d = i - g * D;
+        uint16_t *vp = (uint16_t *)p.v + at + ((size_t)(4 * ((pb >> 5) & 1) + g) * D + d) * 8;
+        uint16_t y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = s_v[v_chunk_pos(g, e)][d];
+        if (v_chunk_pos(g, 0) >= r_lo && v_chunk_pos(g, 7) < r_hi) {
+            *(uint4 *)vp = make_uint4(y[0] | (uint32_t)y[1] << 16, y[2] | (uint32_t)y[3] << 16, y[4] | (uint32_t)y[5] << 16,
+                                      y[6] | (uint32_t)y[7] << 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int r = v_chunk_pos(g, e);
+                if (r >= r_lo && r < r_hi) vp[e] = y[e];
+            }
         }
     }
 }
@@ -570,8 +777,15 @@ __global__ __launch_bounds__(256) void rope_append_kernel(hymt_paged p, hymt_bat
 template <typename T, typename IO>
 void launch_rope(const hymt_paged &p, const hymt_batch &b, const RopeAppend &a, hipStream_t s) {
     KernelSpan span("rope_append", s, true);
-    if (p.head_dim == 64) launch(span, rope_append_kernel<T, IO, 64>, dim3(b.rows), dim3(256), 0, s, p, b, a);
-    else launch(span, rope_append_kernel<T, IO, 128>, dim3(b.rows), dim3(256), 0, s, p, b, a);
+    if (!b.cu || b.rows < kRopeFew * b.n) {
+        if (p.head_dim == 64) launch(span, rope_row_kernel<T, IO, 64>, dim3(b.rows), dim3(256), 0, s, p, b, a);
+        else launch(span, rope_row_kernel<T, IO, 128>, dim3(b.rows), dim3(256), 0, s, p, b, a);
+        return;
+    }
+    // an entry's rows touch at most two blocks more than they fill
+    const dim3 grid((unsigned)(((b.rows + kRopeRows - 1) / kRopeRows + 2 * b.n) * p.kv_heads));
+    if (p.head_dim == 64) launch(span, rope_block_kernel<T, IO, 64>, grid, dim3(256), 0, s, p, b, a);
+    else launch(span, rope_block_kernel<T, IO, 128>, grid, dim3(256), 0, s, p, b, a);
 }
 
 }  // namespace
