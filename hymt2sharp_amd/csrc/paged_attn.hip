@@ -25,7 +25,6 @@
 // Weights are rounded to the cache's type for the product with V and
 // summed as rounded, so they sum to 1.
 #include <algorithm>
-
 #include "attn_kernels.hpp"
 #include "device_common.hpp"
 #include "ktimer.hpp"
@@ -89,14 +88,25 @@ __device__ __forceinline__ float rows_sum(float v) {
     r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v = min(v, __shfl_xor(v, m));
-    return v;
+// Wave-wide steps by DPP: within rows of 16 lanes, then row 15 -> the next row and lane
+// 31 -> the upper half.  Lane 63 has seen all 64 lanes.
+template <typename F> __device__ __forceinline__ int dpp_scan(int x, int none, F f) {
+    x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x111, 0xF, 0xF, false));  // row_shr:1, 2, 4, 8
+    x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x112, 0xF, 0xF, false));
+    x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x114, 0xF, 0xF, false));
+    x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x118, 0xF, 0xF, false));
+    x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x142, 0xA, 0xF, false));  // row_bcast:15 into rows 1 and 3
+    x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x143, 0xC, 0xF, false));  // row_bcast:31 into rows 2 and 3
+    return x;
+}
+__device__ __forceinline__ int wave_sums(int x) {  // of the lanes up to each
+    return dpp_scan(x, 0, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ int wave_min(int x) {  // in a scalar register
+    return __builtin_amdgcn_readlane(dpp_scan(x, 0x7FFFFFFF, [](int a, int b) { return min(a, b); }), 63);
 }
 
 constexpr int kRows = 128;         // rows of a tile
-constexpr int kMinPages = 4;       // pages that a part of a split range has at least
 constexpr int kMaxParts = 64;      // parts of a split range
 constexpr float kLazyMax = 8.0f;   // weights stay below 2^8 of the running maximum's
 constexpr float kNoMax = -1e30f;   // the maximum before any score: finite, so that -inf - m is -inf
@@ -109,8 +119,9 @@ struct Plan {
     int heads, group, layer, prefix, out_f16;
     float c;          // |scale| log2 e; 0 is replaced by a number that makes every weight 1
     uint32_t flip;    // sign bits flipped in q where scale is negative
-    int parts;        // parts that a kv range is cut into at most (prefix: of it)
-    int own_parts;    // shared: parts of an entry's own range at most
+    int parts, span;  // a kv range (shared: the prefix) is cut into parts of about `span` pages, `parts` at most
+    int own_parts, own_span;  // shared: the same of an entry's own range
+    int tiles;        // tiles of one kv head, at most
     int direct;       // shared: no prefix and no split, the row part writes the output
     float *o, *ml;    // partials: [part][rows * heads][D], [part][rows * heads][2]
 };
@@ -119,8 +130,10 @@ __device__ __forceinline__ int slot_len(const hymt_paged &p, int slot) {
     return (unsigned)slot < (unsigned)p.seqs ? max(0, min(p.len[slot], p.blocks * kPage)) : 0;
 }
 __device__ __forceinline__ int pages_of(int positions) { return (positions + kPage - 1) / kPage; }
-// Parts that a range of `pages` is cut into, at most `most`.
-__device__ __forceinline__ int parts_of(int pages, int most) { return max(1, min(most, pages / kMinPages)); }
+// Parts of about `span` pages that a range of `pages` is cut into, at most `most`.
+__device__ __forceinline__ int parts_of(int pages, int span, int most) {
+    return max(1, min(most, (pages + span - 1) / span));
+}
 
 // An entry's rows in the packed tensors, whatever cu holds: inside [0, rows).
 struct Span {
@@ -161,35 +174,52 @@ template <int READS> __device__ __forceinline__ void read_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x008, 2 * DEPTH, 0);
 }
 
-template <int D> struct TileLds {
-    uint16_t kv[2][2][kPage * D];  // [buffer][K, V][page]
-    int flag[2];                   // a value that is not finite was seen in V, by buffer
-    int low[4];                    // lowest limit of each wave's rows
+// Pages of a slot's table: lane i holds that of tile at + i.  The first 64 are loaded by
+// whoever knows the slot, beside the length that the tiles hang on, and others as
+// they come up.
+struct Ids {
+    const int32_t *table;  // the slot's row, null for a slot outside the cache
+    int blocks, at, v;
+    __device__ __forceinline__ void load(int first) {
+        const int i = first + (int)(threadIdx.x & 63);
+        at = first;
+        v = table && i < blocks ? table[i] : -1;
+    }
+    // -1: absent.  t is the same in all lanes and below `blocks`.
+    __device__ __forceinline__ int page(const hymt_paged &p, int t) {
+        if ((unsigned)(t - at) >= 64u) load(t);
+        const int x = __builtin_amdgcn_readlane(v, t - at);
+        return (unsigned)x < (unsigned)p.pages ? x : -1;
+    }
+};
+__device__ __forceinline__ Ids ids_of(const hymt_paged &p, int slot, int first) {
+    Ids r;
+    r.table = (unsigned)slot < (unsigned)p.seqs ? p.table + (size_t)slot * p.blocks : nullptr;
+    r.blocks = p.blocks;
+    r.load(first);
+    return r;
+}
+
+// KS: groups of four waves that take the rows' pages in turn.
+template <int D, int KS> struct TileLds {
+    uint16_t kv[KS][2][2][kPage * D];  // [group][buffer][K, V][page]; later what the groups hand over
+    int flag[2];                       // a value that is not finite was seen in V, by buffer
+    int low[4];                        // lowest limit of each wave's rows
 };
 
-// 128 rows of kv head h over pages [t0, t1) of `slot`.  PREFIX: row r is entry
+// 128 rows of kv head h over pages [t0, t1) of a slot.  PREFIX: row r is entry
 // r / G's, its limit min(common, that entry's length), the result a partial.
-template <typename T, int D, bool PREFIX>
-__device__ __forceinline__ void tile_part(const Plan &a, TileLds<D> &s, int h, int slot, int slot_positions, Rows rows,
+template <typename T, int D, int KS, bool PREFIX>
+__device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int h, Ids ids, int slot_positions, Rows rows,
                                           int r0, int t0, int t1, int part, bool partial) {
     typedef typename Mma<T>::vec vec;
-    constexpr int KS = D / 32, DB = D / 16, kPageBytes = kPage * D * 2;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int DS = D / 32, DB = D / 16, kPageBytes = kPage * D * 2;
+    const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int half = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8);
     const int grp = lane >> 4, c = lane & 15;
 
-    // ---- pages: lane i has the page of tile (base & ~63) + i
-    const int32_t *table = a.p.table + (size_t)slot * a.p.blocks;
-    int ids = -1, ids_at = -1;
-    auto page_of = [&](int t) __attribute__((always_inline)) {
-        if ((t & ~63) != ids_at) {  // uniform
-            ids_at = t & ~63;
-            ids = ids_at + lane < t1 ? table[ids_at + lane] : -1;
-        }
-        const int page = __builtin_amdgcn_readlane(ids, t & 63);
-        return (unsigned)page < (unsigned)a.p.pages ? page : -1;
-    };
     const uint32_t off = (wave * 64 + lane) * 16;
-    const uint32_t lds0 = lds_addr(&s.kv[0][0][0]) + wave * 1024;
+    const uint32_t lds0 = lds_addr(&s.kv[half][0][0][0]) + wave * 1024;
     auto fetch = [&](int page, int buf, int v) __attribute__((always_inline)) {
         const char *base = (const char *)(v ? a.p.v : a.p.k) +
                            (((size_t)a.layer * a.p.pages + page) * a.p.kv_heads + h) * (size_t)kPageBytes;
@@ -198,39 +228,39 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D> &s, int h, i
             lds_dma16_sv(base + i * 4096, off, lds0 + (buf * 2 + v) * kPageBytes + i * 4096);
     };
 
-    int page = t0 < t1 ? page_of(t0) : -1;
-    if (page >= 0) {
-        fetch(page, 0, 0);
-        fetch(page, 0, 1);
-    }
-
     // ---- the wave's rows: q as the S^T B operand, lane (grp, c) has dims
     // 32 ks + 8 grp + [0, 8) of row c; rows past the end repeat the last one
     int limit[2];
     size_t at[2];  // element of (row, head) in q and out
-    uint4 qu[2][KS];
+    uint4 qu[2][DS];
 #pragma unroll
     for (int qq = 0; qq < 2; qq++) {
         const int r = min(r0 + wave * 32 + qq * 16 + c, rows.n - 1);
         const int token = r / a.group, g = r - token * a.group;
         at[qq] = ((size_t)(rows.first + token) * a.heads + h * a.group + g) * D;
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) qu[qq][ks] = *(const uint4 *)((const uint16_t *)a.q + at[qq] + 32 * ks + 8 * grp);
+        for (int ks = 0; ks < DS; ks++) qu[qq][ks] = *(const uint4 *)((const uint16_t *)a.q + at[qq] + 32 * ks + 8 * grp);
         if constexpr (PREFIX) limit[qq] = min(slot_positions, slot_len(a.p, a.b.slots[token]));
         else limit[qq] = min(rows.seen + token, slot_positions);
     }
-    vec qf[2][KS];
+    int page = t0 + half < t1 ? ids.page(a.p, t0 + half) : -1;
+    if (page >= 0) {
+        fetch(page, 0, 0);
+        fetch(page, 0, 1);
+    }
+
+    vec qf[2][DS];
 #pragma unroll
     for (int qq = 0; qq < 2; qq++)
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++)
+        for (int ks = 0; ks < DS; ks++)
             qf[qq][ks] = __builtin_bit_cast(vec, make_uint4(qu[qq][ks].x ^ a.flip, qu[qq][ks].y ^ a.flip,
                                                             qu[qq][ks].z ^ a.flip, qu[qq][ks].w ^ a.flip));
     // lowest limits: of the wave's blocks, and of the tile
     int low[2];
 #pragma unroll
-    for (int qq = 0; qq < 2; qq++) low[qq] = __builtin_amdgcn_readfirstlane(wave_min(limit[qq]));
-    if (lane == 0) s.low[wave] = min(low[0], low[1]);
+    for (int qq = 0; qq < 2; qq++) low[qq] = wave_min(limit[qq]);
+    if (lane == 0) s.low[wave] = min(low[0], low[1]);  // the groups have the same rows
     if (tid < 2) s.flag[tid] = 0;
 
     const bool live = r0 + wave * 32 < rows.n;  // the wave has a row
@@ -245,22 +275,26 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D> &s, int h, i
     __syncthreads();
     const int tile_low = min(min(s.low[0], s.low[1]), min(s.low[2], s.low[3]));
 
-    for (int t = t0; t < t1; t++) {
-        const int buf = (t - t0) & 1, base = t * kPage;
-        const int next = t + 1 < t1 ? page_of(t + 1) : -1;
-        const uint16_t *kt = s.kv[buf][0] + lane * 8, *vt = s.kv[buf][1] + grp * (D * 8) + c * 8;
-        if (next >= 0) fetch(next, buf ^ 1, 0);
+    for (int step = t0; step < t1; step += KS) {
+        const int t = step + half, buf = KS == 1 ? (step - t0) & 1 : (step - t0) >> 1 & 1, base = t * kPage;
+        const int next = t + KS < t1 ? ids.page(a.p, t + KS) : -1;
+        const uint16_t *kt = s.kv[half][buf][0] + lane * 8, *vt = s.kv[half][buf][1] + grp * (D * 8) + c * 8;
+        if (next >= 0) {
+            fetch(next, buf ^ 1, 0);
+            fetch(next, buf ^ 1, 1);
+        }
         bool odd = false;
-        if (page >= 0 && base + kPage > tile_low) {
+        if (min(step + KS, t1) * kPage > tile_low) {  // the same for both groups
             // Some row does not see some position of this page.  Its weight is 0
             // there, and 0 times an infinity or a NaN is none: values past the
             // sequence's end (anything may stand there) become 0 in LDS, and
             // if others are not finite the products leave them out (below).
             uint32_t top = 0;
+            if (page >= 0)
 #pragma unroll
             for (int i = 0; i < kPage * D / 8 / 256; i++) {
                 const int ch = tid + 256 * i, pc = ch / D;
-                uint4 *at_v = (uint4 *)s.kv[buf][1] + ch;
+                uint4 *at_v = (uint4 *)s.kv[half][buf][1] + ch;
                 uint4 u = *at_v;
                 uint32_t w[4] = {u.x, u.y, u.z, u.w};
                 if (!PREFIX && base + kPage > slot_positions) {
@@ -279,23 +313,23 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D> &s, int h, i
             __syncthreads();
             odd = s.flag[buf] != 0;
         }
-        if (page >= 0 && live) {
+        const bool on = page >= 0 && live;
+        pa_f32x4 sc[4][2];
+        if (on) {
             // ---- S^T = K Q^T, 64 positions x 16 rows a block
-            pa_f32x4 sc[4][2];
 #pragma unroll
             for (int kb = 0; kb < 4; kb++)
 #pragma unroll
                 for (int qq = 0; qq < 2; qq++) sc[kb][qq] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++)
+            for (int ks = 0; ks < DS; ks++)
 #pragma unroll
                 for (int kb = 0; kb < 4; kb++) {
                     const vec kf = __builtin_bit_cast(vec, *(const uint4 *)(kt + kb * (16 * D) + ks * 512));
 #pragma unroll
                     for (int qq = 0; qq < 2; qq++) sc[kb][qq] = Mma<T>::mma(kf, qf[qq][ks], sc[kb][qq]);
                 }
-            read_ahead<4 * KS>();
-            if (next >= 0) fetch(next, buf ^ 1, 1);
+            read_ahead<4 * DS>();
 
             // ---- softmax
             float mx[2];
@@ -326,77 +360,113 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D> &s, int h, i
                     for (int db = 0; db < DB; db++) o[db][qq] *= al;
                 }
             }
-#pragma unroll
-            for (int kb = 0; kb < 4; kb++)
-#pragma unroll
-                for (int qq = 0; qq < 2; qq++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        sc[kb][qq][i] = __builtin_amdgcn_exp2f(fmaf(sc[kb][qq][i], a.c, -m[qq]));
-
-            // ---- O^T += V^T P^T
-            vec pf[2][2];
-#pragma unroll
-            for (int k2 = 0; k2 < 2; k2++)
-#pragma unroll
-                for (int qq = 0; qq < 2; qq++) {
-                    const pa_f32x4 x = sc[2 * k2][qq], y = sc[2 * k2 + 1][qq];
-                    const uint4 u = make_uint4(Mma<T>::pack(x[0], x[1]), Mma<T>::pack(x[2], x[3]),
-                                               Mma<T>::pack(y[0], y[1]), Mma<T>::pack(y[2], y[3]));
-                    l[qq] = Mma<T>::sum(u.w, Mma<T>::sum(u.z, Mma<T>::sum(u.y, Mma<T>::sum(u.x, l[qq]))));
-                    pf[k2][qq] = __builtin_bit_cast(vec, u);
-                }
-            if (!odd) {
-#pragma unroll
-                for (int k2 = 0; k2 < 2; k2++)
-#pragma unroll
-                    for (int db = 0; db < DB; db++) {
-                        const vec vf = __builtin_bit_cast(vec, *(const uint4 *)(vt + k2 * (4 * D * 8) + db * 128));
-#pragma unroll
-                        for (int qq = 0; qq < 2; qq++) o[db][qq] = Mma<T>::mma(vf, pf[k2][qq], o[db][qq]);
-                    }
-                read_ahead<2 * DB>();
-            } else {
-                // the products without the values that are not finite ...
-#pragma unroll
-                for (int k2 = 0; k2 < 2; k2++)
-#pragma unroll
-                    for (int db = 0; db < DB; db++) {
-                        const uint4 u = *(const uint4 *)(vt + k2 * (4 * D * 8) + db * 128);
-                        uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            if ((w[e] & 0x7FFFu) >= Mma<T>::kInf) w[e] &= 0xFFFF0000u;
-                            if ((w[e] >> 16 & 0x7FFFu) >= Mma<T>::kInf) w[e] &= 0xFFFFu;
-                        }
-                        const vec vf = __builtin_bit_cast(vec, make_uint4(w[0], w[1], w[2], w[3]));
-#pragma unroll
-                        for (int qq = 0; qq < 2; qq++) o[db][qq] = Mma<T>::mma(vf, pf[k2][qq], o[db][qq]);
-                    }
-                // ... and those to the rows that see them (their weight is
-                // positive, so the result is the value)
+        }
+        if (odd) {
+            // Rare: the values that are not finite go to the rows that see them by
+            // themselves (their weight is positive, so the result is the value)
+            // and are then 0 for the products.
+            if (on)
                 for (int pos = 0; pos < kPage; pos++) {
                     const int pc = 4 * (pos >> 5) + ((pos >> 2) & 3), e = 4 * ((pos >> 4) & 1) + (pos & 3);
-                    const uint16_t *v = s.kv[buf][1] + (size_t)pc * (D * 8) + e;
+                    const uint16_t *v = s.kv[half][buf][1] + (size_t)pc * (D * 8) + e;
 #pragma unroll
                     for (int db = 0; db < DB; db++)
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const uint16_t x = v[(16 * db + 4 * grp + i) * 8];
-                            if ((x & 0x7FFFu) >= Mma<T>::kInf)
+                            const float y = (x & 0x7FFFu) >= Mma<T>::kInf ? from_elem<T>(x) : 0.f;
 #pragma unroll
-                                for (int qq = 0; qq < 2; qq++)
-                                    if (base + pos < limit[qq]) o[db][qq][i] += from_elem<T>(x);
+                            for (int qq = 0; qq < 2; qq++) o[db][qq][i] += base + pos < limit[qq] ? y : 0.f;
                         }
                 }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kPage * D / 8 / 256; i++) {
+                uint32_t *w = (uint32_t *)((uint4 *)s.kv[half][buf][1] + tid + 256 * i);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint32_t x = w[e];
+                    if ((x & 0x7FFFu) >= Mma<T>::kInf) x &= 0xFFFF0000u;
+                    if ((x >> 16 & 0x7FFFu) >= Mma<T>::kInf) x &= 0xFFFFu;
+                    w[e] = x;
+                }
             }
-        } else if (next >= 0) {
-            fetch(next, buf ^ 1, 1);
+            __syncthreads();
+        }
+        if (on) {
+            // ---- weights, and O^T += V^T P^T: the second half's weights between the
+            // first half's products
+            vec pf[2], vf[DB], vg[DB];
+            auto weights = [&](int k2) __attribute__((always_inline)) {
+#pragma unroll
+                for (int qq = 0; qq < 2; qq++) {
+                    pa_f32x4 x = sc[2 * k2][qq], y = sc[2 * k2 + 1][qq];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], a.c, -m[qq]));
+                        y[i] = __builtin_amdgcn_exp2f(fmaf(y[i], a.c, -m[qq]));
+                    }
+                    const uint4 u = make_uint4(Mma<T>::pack(x[0], x[1]), Mma<T>::pack(x[2], x[3]),
+                                               Mma<T>::pack(y[0], y[1]), Mma<T>::pack(y[2], y[3]));
+                    l[qq] = Mma<T>::sum(u.w, Mma<T>::sum(u.z, Mma<T>::sum(u.y, Mma<T>::sum(u.x, l[qq]))));
+                    pf[qq] = __builtin_bit_cast(vec, u);
+                }
+            };
+#pragma unroll
+            for (int db = 0; db < DB; db++) vf[db] = __builtin_bit_cast(vec, *(const uint4 *)(vt + db * 128));
+            weights(0);
+            __builtin_amdgcn_sched_barrier(0);
+            const vec p0 = pf[0], p1 = pf[1];
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                o[db][0] = Mma<T>::mma(vf[db], p0, o[db][0]);
+                o[db][1] = Mma<T>::mma(vf[db], p1, o[db][1]);
+                vg[db] = __builtin_bit_cast(vec, *(const uint4 *)(vt + 4 * D * 8 + db * 128));
+            }
+            weights(1);
+#pragma unroll
+            for (int i = 0; i < DB; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 56 / DB, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int db = 0; db < DB; db++) {
+                o[db][0] = Mma<T>::mma(vg[db], pf[0], o[db][0]);
+                o[db][1] = Mma<T>::mma(vg[db], pf[1], o[db][1]);
+            }
         }
         page = next;
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         if (odd && tid == 0) s.flag[buf] = 0;  // every wave has read it; the next that sets it does so two steps on
+    }
+
+    if constexpr (KS == 2) {
+        // the second group hands its (m, l, O) to the first (the last barrier is
+        // behind every read of the pages)
+        pa_f32x4 *x = (pa_f32x4 *)&s.kv[0][0][0][0] + (wave * (2 * DB + 1)) * 64 + lane;
+        static_assert(4 * (2 * DB + 1) * 64 * 16 <= (int)sizeof(s.kv), "hand-over");
+        if (half) {
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int qq = 0; qq < 2; qq++) x[(2 * db + qq) * 64] = o[db][qq];
+            x[2 * DB * 64] = pa_f32x4{m[0], m[1], l[0], l[1]};
+        }
+        __syncthreads();
+        if (half) return;
+        const pa_f32x4 ml = x[2 * DB * 64];
+#pragma unroll
+        for (int qq = 0; qq < 2; qq++) {
+            const float now = fmaxf(m[qq], ml[qq]);
+            const float w0 = __builtin_amdgcn_exp2f(m[qq] - now), w1 = __builtin_amdgcn_exp2f(ml[qq] - now);
+            m[qq] = now;
+            l[qq] = l[qq] * w0 + ml[2 + qq] * w1;
+#pragma unroll
+            for (int db = 0; db < DB; db++) o[db][qq] = o[db][qq] * w0 + x[(2 * db + qq) * 64] * w1;
+        }
     }
 
 #pragma unroll
@@ -420,13 +490,20 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D> &s, int h, i
     }
 }
 
-// The tile that work index w is of: its entry, place and number there.  Tiles of
-// an entry come last first, so that the longest kv ranges start first.
+// Pages that a tile of an entry attends to.
+__device__ __forceinline__ int tile_pages(int len, Span sp, int index, int group) {
+    const int last = min(sp.n - 1, (min((index + 1) * kRows, sp.n * group) - 1) / group);
+    return pages_of(max(0, min(len, len - sp.n + last + 1)));
+}
+
+// The tile that work index w is of.  Tiles of an entry come last first, so that the
+// longest kv ranges start first; SPLIT: only those that are cut into parts count (the
+// last ones of an entry).
 struct Tile {
-    int entry, index, slot, len;
+    int index, slot, len;
     Span span;
 };
-__device__ __forceinline__ bool find_tile(const Plan &a, int w, Tile &out) {
+template <bool SPLIT> __device__ __forceinline__ bool find_tile(const Plan &a, int w, Tile &out) {
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int base = 0; base < a.b.n; base += 64) {
@@ -439,19 +516,19 @@ __device__ __forceinline__ bool find_tile(const Plan &a, int w, Tile &out) {
         }
         const int len = slot_len(a.p, slot);  // for every entry: one load deep, not one more after the search
         const int tiles = (sp.n * a.group + kRows - 1) / kRows;
-        int x = tiles;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int y = __shfl_up(x, d);
-            if (lane >= d) x += y;
+        int count = tiles;
+        if constexpr (SPLIT) {
+            // tile_pages(index) > span from the token on that sees span * 64 + 1 positions
+            const long token = max(0L, (long)a.span * kPage - (len - sp.n));
+            // the first tile whose last token is that one or a later one
+            count = len > a.span * kPage && token < sp.n ? tiles - (int)(token * a.group / kRows) : 0;
         }
+        const int x = wave_sums(count);
         const uint64_t hit = __ballot(w < before + x);
         if (hit) {
             const int at = __ffsll((unsigned long long)hit) - 1;
-            out.entry = base + at;
-            const int count = __builtin_amdgcn_readlane(tiles, at);
-            const int first = before + __builtin_amdgcn_readlane(x, at) - count;
-            out.index = count - 1 - (w - first);
+            const int first = before + __builtin_amdgcn_readlane(x, at) - __builtin_amdgcn_readlane(count, at);
+            out.index = __builtin_amdgcn_readlane(tiles, at) - 1 - (w - first);
             out.slot = __builtin_amdgcn_readlane(slot, at);
             out.len = __builtin_amdgcn_readlane(len, at);
             out.span = {__builtin_amdgcn_readlane(sp.first, at), __builtin_amdgcn_readlane(sp.n, at)};
@@ -462,25 +539,19 @@ __device__ __forceinline__ bool find_tile(const Plan &a, int w, Tile &out) {
     return false;
 }
 
-// Pages that a tile of an entry attends to.
-__device__ __forceinline__ int tile_pages(int len, Span sp, int index, int group) {
-    const int last = min(sp.n - 1, (min((index + 1) * kRows, sp.n * group) - 1) / group);
-    return pages_of(max(0, min(len, len - sp.n + last + 1)));
-}
-
-template <typename T, int D> __global__ __launch_bounds__(256, 2) void attn_packed_kernel(Plan a) {
-    __shared__ __attribute__((aligned(256))) TileLds<D> s;
+template <typename T, int D, int KS> __global__ __launch_bounds__(256 * KS, 2) void attn_packed_kernel(Plan a) {
+    __shared__ __attribute__((aligned(256))) TileLds<D, KS> s;
     // workgroups of one kv head on the same XCDs (workgroup b runs on XCD
     // b % 8), whose L2 then holds that head's pages
     const int h = blockIdx.x % a.p.kv_heads, rest = blockIdx.x / a.p.kv_heads;
-    const int part = rest % a.parts;
+    const int part = rest / a.tiles;  // second parts, which not every tile has, come after all first ones
     Tile t;
-    if (!find_tile(a, rest / a.parts, t)) return;
-    const int pages = tile_pages(t.len, t.span, t.index, a.group), parts = parts_of(pages, a.parts);
+    if (!find_tile<false>(a, rest - part * a.tiles, t)) return;
+    const Ids ids = ids_of(a.p, t.slot, 0);
+    const int pages = tile_pages(t.len, t.span, t.index, a.group), parts = parts_of(pages, a.span, a.parts);
     if (part >= parts) return;
     const Rows rows{t.span.first, t.span.n * a.group, t.len - t.span.n + 1};
-    const int slot = max(0, t.slot);  // an unknown slot has no pages
-    tile_part<T, D, false>(a, s, h, slot, t.len, rows, t.index * kRows, (int)((long)part * pages / parts),
+    tile_part<T, D, KS, false>(a, s, h, ids, t.len, rows, t.index * kRows, (int)((long)part * pages / parts),
                            (int)((long)(part + 1) * pages / parts), part, parts > 1);
 }
 
@@ -492,50 +563,64 @@ template <int D> struct RowLds {
 };
 
 // Up to 16 rows (heads g0 ..) of one entry over pages [t0, t1) of its slot, a page to
-// a wave: K and V go from memory into operand registers.
+// a wave: K and V go from memory into operand registers, those of the wave's next
+// page as soon as the products have read these.
 template <typename T, int D>
-__device__ __forceinline__ void row_part(const Plan &a, RowLds<D> &s, int entry, int h, int g0, int slot, int len, int t0,
+__device__ __forceinline__ void row_part(const Plan &a, RowLds<D> &s, int entry, int h, int g0, Ids ids, int len, int t0,
                                          int t1, int part, bool partial) {
     typedef typename Mma<T>::vec vec;
-    constexpr int KS = D / 32, DB = D / 16;
+    constexpr int DS = D / 32, DB = D / 16;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int grp = lane >> 4, c = lane & 15;
     const int g = min(g0 + c, a.group - 1);
     const size_t at = ((size_t)entry * a.heads + h * a.group + g) * D;
-    vec qf[KS];
+    uint4 qu[DS], ku[DS][4], vu[2][DB];
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) {
-        const uint4 u = *(const uint4 *)((const uint16_t *)a.q + at + 32 * ks + 8 * grp);
-        qf[ks] = __builtin_bit_cast(vec, make_uint4(u.x ^ a.flip, u.y ^ a.flip, u.z ^ a.flip, u.w ^ a.flip));
-    }
-    pa_f32x4 o[DB];
+    for (int ks = 0; ks < DS; ks++) qu[ks] = *(const uint4 *)((const uint16_t *)a.q + at + 32 * ks + 8 * grp);
+    // an absent page is read as page 0 and masked whole
+    auto base_of = [&](int page) {
+        return (((size_t)a.layer * a.p.pages + max(page, 0)) * a.p.kv_heads + h) * (size_t)(kPage * D);
+    };
+    auto load_k = [&](int page) __attribute__((always_inline)) {
+        const uint16_t *kp = (const uint16_t *)a.p.k + base_of(page) + lane * 8;
 #pragma unroll
-    for (int db = 0; db < DB; db++) o[db] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = kNoMax, l = 0.f;
-    const int32_t *table = a.p.table + (size_t)slot * a.p.blocks;
-    for (int t = t0 + wave; t < t1; t += 4) {
-        const int page = __builtin_amdgcn_readfirstlane(table[t]);
-        if ((unsigned)page >= (unsigned)a.p.pages) continue;
-        const size_t base = (((size_t)a.layer * a.p.pages + page) * a.p.kv_heads + h) * (size_t)(kPage * D);
-        const uint16_t *kp = (const uint16_t *)a.p.k + base + lane * 8;
-        const uint16_t *vp = (const uint16_t *)a.p.v + base + grp * (D * 8) + c * 8;
-        uint4 ku[KS][4], vu[2][DB];
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++)
+        for (int ks = 0; ks < DS; ks++)
 #pragma unroll
             for (int kb = 0; kb < 4; kb++) ku[ks][kb] = *(const uint4 *)(kp + kb * (16 * D) + ks * 512);
+    };
+    auto load_v = [&](int page) __attribute__((always_inline)) {
+        const uint16_t *vp = (const uint16_t *)a.p.v + base_of(page) + grp * (D * 8) + c * 8;
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++)
 #pragma unroll
             for (int db = 0; db < DB; db++) vu[k2][db] = *(const uint4 *)(vp + k2 * (4 * D * 8) + db * 128);
+    };
+    int t = t0 + wave, page = -1;
+    if (t < t1) {
+        page = ids.page(a.p, t);
+        load_k(page);
+        load_v(page);
+    }
+    vec qf[DS];
+#pragma unroll
+    for (int ks = 0; ks < DS; ks++)
+        qf[ks] = __builtin_bit_cast(vec, make_uint4(qu[ks].x ^ a.flip, qu[ks].y ^ a.flip, qu[ks].z ^ a.flip,
+                                                    qu[ks].w ^ a.flip));
+    pa_f32x4 o[DB];
+#pragma unroll
+    for (int db = 0; db < DB; db++) o[db] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = kNoMax, l = 0.f;
+    while (t < t1) {
         pa_f32x4 sc[4];
 #pragma unroll
         for (int kb = 0; kb < 4; kb++) sc[kb] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++)
+        for (int ks = 0; ks < DS; ks++)
 #pragma unroll
             for (int kb = 0; kb < 4; kb++) sc[kb] = Mma<T>::mma(__builtin_bit_cast(vec, ku[ks][kb]), qf[ks], sc[kb]);
-        const int left = len - t * kPage;  // positions of this page
+        const int left = page < 0 ? 0 : len - t * kPage;  // positions of this page
+        const int next = t + 4 < t1 ? ids.page(a.p, t + 4) : -1;
+        if (t + 4 < t1) load_k(next);
         if (left < kPage) {
 #pragma unroll
             for (int kb = 0; kb < 4; kb++)
@@ -577,6 +662,9 @@ __device__ __forceinline__ void row_part(const Plan &a, RowLds<D> &s, int entry,
             for (int db = 0; db < DB; db++)
                 o[db] = Mma<T>::mma(__builtin_bit_cast(vec, vu[k2][db]), __builtin_bit_cast(vec, u), o[db]);
         }
+        if (t + 4 < t1) load_v(next);
+        page = next;
+        t += 4;
     }
     l = rows_sum(l);
     // ---- the four waves' results meet in LDS
@@ -620,16 +708,19 @@ __device__ __forceinline__ int common_of(const Plan &a) {
 // Workgroups [0, tile_wgs) the prefix, the others the entries' own positions.
 template <typename T, int D> __global__ __launch_bounds__(256, 2) void attn_shared_kernel(Plan a, int tile_wgs) {
     __shared__ __attribute__((aligned(256))) union {
-        TileLds<D> tile;
+        TileLds<D, 1> tile;
         RowLds<D> row;
     } s;
-    const int common = common_of(a);
+    // the table's part is loaded where the range begins if slots[0] is as long as the
+    // prefix, as it should be, beside the length that decides
+    const int pages_expected = min(a.prefix / kPage, a.p.blocks), slot0 = a.b.slots[0];
     if ((int)blockIdx.x < tile_wgs) {
-        const int h = blockIdx.x % a.p.kv_heads, rest = blockIdx.x / a.p.kv_heads;
-        const int pages = common / kPage, parts = parts_of(pages, a.parts), part = rest % a.parts;
+        const int h = blockIdx.x % a.p.kv_heads, rest = blockIdx.x / a.p.kv_heads, part = rest % a.parts;
+        const Ids ids = ids_of(a.p, slot0, (int)((long)part * pages_expected / parts_of(pages_expected, a.span, a.parts)));
+        const int common = common_of(a), pages = common / kPage, parts = parts_of(pages, a.span, a.parts);
         if (part >= parts || pages == 0) return;
-        tile_part<T, D, true>(a, s.tile, h, a.b.slots[0], common, Rows{0, a.b.n * a.group, 0}, rest / a.parts * kRows,
-                              (int)((long)part * pages / parts), (int)((long)(part + 1) * pages / parts), part, true);
+        tile_part<T, D, 1, true>(a, s.tile, h, ids, common, Rows{0, a.b.n * a.group, 0}, rest / a.parts * kRows,
+                                 (int)((long)part * pages / parts), (int)((long)(part + 1) * pages / parts), part, true);
         return;
     }
     int w = blockIdx.x - tile_wgs;
@@ -638,102 +729,175 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void attn_shar
     const int blocks16 = (a.group + 15) / 16;
     const int g0 = w % blocks16 * 16;
     w /= blocks16;
-    const int part = w % a.own_parts, entry = w / a.own_parts;
-    const int slot = a.b.slots[entry], len = slot_len(a.p, slot);
-    const int first = common / kPage, pages = max(0, pages_of(len) - first), parts = parts_of(pages, a.own_parts);
+    const int part = w % a.own_parts, entry = w / a.own_parts, slot = a.b.slots[entry];
+    const Ids ids = ids_of(a.p, slot, pages_expected);
+    const int common = common_of(a), len = slot_len(a.p, slot);
+    const int first = common / kPage, pages = max(0, pages_of(len) - first),
+              parts = parts_of(pages, a.own_span, a.own_parts);
     if (part >= parts) return;
-    row_part<T, D>(a, s.row, entry, h, g0, max(0, slot), len, first + (int)((long)part * pages / parts),
+    row_part<T, D>(a, s.row, entry, h, g0, ids, len, first + (int)((long)part * pages / parts),
                    first + (int)((long)(part + 1) * pages / parts), a.parts + part, !a.direct);
 }
 
 // ---- joining -----------------------------------------------------------------------
 
-// A wave a row of one head: the parts' sums, weighed by their maxima.
-template <typename T, int D, bool SHARED> __global__ __launch_bounds__(256) void attn_merge_kernel(Plan a) {
-    const int lane = threadIdx.x & 63;
-    const int rh = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row = rh / a.heads;
-    if (row >= a.b.rows) return;
-    int n0 = 0, n1 = 0;  // parts [0, n0) and [a.parts, a.parts + n1)
-    if constexpr (SHARED) {
-        const int common = common_of(a), len = slot_len(a.p, a.b.slots[row]);
-        if (common) n0 = parts_of(common / kPage, a.parts);
-        n1 = parts_of(max(0, pages_of(len) - common / kPage), a.own_parts);
-    } else {
-        int below = 0;
-        if (a.b.cu) {
-            for (int base = 0; base < a.b.n; base += 64) {
-                const int i = base + lane;
-                below += __popcll(__ballot(i < a.b.n && a.b.cu[i + 1] <= row));
-            }
-        } else {
-            below = row;
-        }
-        if (below >= a.b.n) return;
-        const Span sp = a.b.cu ? span_of(a.b, below) : Span{row, 1};
-        if (row < sp.first || row >= sp.first + sp.n) return;
-        const int index = ((row - sp.first) * a.group + rh % a.heads % a.group) / kRows;
-        n0 = parts_of(tile_pages(slot_len(a.p, a.b.slots[below]), sp, index, a.group), a.parts);
-        if (n0 == 1) return;  // written by its tile
-    }
+// Joining: out = sum_k 2^(m_k - m) O_k / sum_k 2^(m_k - m) l_k.
+
+
+// The split tiles of attn_packed: a group of D / 4 lanes a row of one head.  The grid
+// walks over them, as their number is only known here.
+constexpr int kJoinGrid = 1024;
+template <typename T, int D> __global__ __launch_bounds__(256) void attn_join_tiles_kernel(Plan a) {
+    constexpr int L = D / 4, G = 256 / L, K = kMaxParts / L;
+    __shared__ float s_w[G][kMaxParts];
+    const int g = threadIdx.x / L, lane = threadIdx.x % L;
     const size_t stride = (size_t)a.b.rows * a.heads;
-    const int total = n0 + n1;
+    for (int u = blockIdx.x;; u += gridDim.x) {
+        const int h = u % a.p.kv_heads, rest = u / a.p.kv_heads;
+        Tile t;
+        if (!find_tile<true>(a, rest / (kRows / G), t)) return;
+        const int n = parts_of(tile_pages(t.len, t.span, t.index, a.group), a.span, a.parts);
+        const int r = t.index * kRows + rest % (kRows / G) * G + g;
+        const bool on = r < t.span.n * a.group;
+        const int token = min(r, t.span.n * a.group - 1) / a.group;
+        const size_t at = (size_t)(t.span.first + token) * a.heads + h * a.group + (on ? r - token * a.group : 0);
+        float2 ml[K];
+        float top = kNoMax, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int i = lane + L * k;
+            ml[k] = i < n ? *(const float2 *)(a.ml + (i * stride + at) * 2) : make_float2(kNoMax, 0.f);
+            top = fmaxf(top, ml[k].x);
+        }
+#pragma unroll
+        for (int x = 1; x < L; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const float w = __builtin_amdgcn_exp2f(ml[k].x - top);
+            sum += w * ml[k].y;
+            s_w[g][lane + L * k] = w;
+        }
+#pragma unroll
+        for (int x = 1; x < L; x <<= 1) sum += __shfl_xor(sum, x);
+        __syncthreads();
+        pa_f32x4 acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int k = 0; k < n; k++) acc += *(const pa_f32x4 *)(a.o + (k * stride + at) * D + 4 * lane) * s_w[g][k];
+        const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+        if (on) put4<T>(a, at * D + 4 * lane, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+        __syncthreads();
+    }
+}
+
+// attn_shared: the first n0 parts of the prefix, then n1 of the entry's own.  WHOLE: a
+// workgroup takes one row of one head, its groups of D / 4 lanes the parts in
+// turn; else a group takes a row by itself (up to D / 4 parts).  The (m, l) are
+// read before it is known how many parts the row has (what lies past them is left
+// out): one round trip less between the lengths and the sums.
+template <typename T, int D, bool WHOLE> __global__ __launch_bounds__(256) void attn_join_rows_kernel(Plan a) {
+    constexpr int L = D / 4, G = 256 / L, K = WHOLE ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) float s_o[WHOLE ? G : 1][D];
+    __shared__ float s_w[WHOLE ? 1 : G][WHOLE ? 2 * kMaxParts : L];
+    const int tid = threadIdx.x, g = tid / L, lane = tid % L, d = 4 * lane;
+    const size_t stride = (size_t)a.b.rows * a.heads;
+    const size_t rh = WHOLE ? blockIdx.x : (size_t)blockIdx.x * G + g, at = min(rh, stride - 1);
+    const int row = (int)(at / a.heads), most = a.parts + a.own_parts;
+    constexpr int W = WHOLE ? 64 : L;  // lanes that hold a row's weights, K parts each
+    const int mine = WHOLE ? tid & 63 : lane;
+    float2 ml[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) ml[k] = *(const float2 *)(a.ml + (min(mine + W * k, most - 1) * stride + at) * 2);
+    const int common = common_of(a), len = slot_len(a.p, a.b.slots[row]);
+    const int n0 = common ? parts_of(common / kPage, a.span, a.parts) : 0;
+    const int n1 = parts_of(max(0, pages_of(len) - common / kPage), a.own_span, a.own_parts);
     float top = kNoMax, sum = 0.f;
-    auto index_of = [&](int k) { return (size_t)(k < n0 ? k : a.parts + k - n0) * stride + rh; };
-    for (int base = 0; base < total; base += 64) {
-        float2 x = make_float2(kNoMax, 0.f);
-        if (base + lane < total) x = *(const float2 *)(a.ml + index_of(base + lane) * 2);
-        float mx = x.x;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
-        const float now = fmaxf(top, mx);
-        float w = x.y * __builtin_amdgcn_exp2f(x.x - now);
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) w += __shfl_xor(w, d);
-        sum = sum * __builtin_amdgcn_exp2f(top - now) + w;
-        top = now;
+    for (int k = 0; k < K; k++) {
+        const int i = mine + W * k;
+        if (i >= most || !(i < n0 || (i >= a.parts && i < a.parts + n1))) ml[k] = make_float2(kNoMax, 0.f);
+        top = fmaxf(top, ml[k].x);
     }
-    // 4 dims a lane, D / 4 lanes a part, several parts at a time
-    constexpr int L = D / 4, S = 64 / L;
+#pragma unroll
+    for (int x = 1; x < W; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const float w = __builtin_amdgcn_exp2f(ml[k].x - top);
+        sum += w * ml[k].y;
+        if (!WHOLE || tid < 64) s_w[WHOLE ? 0 : g][mine + W * k] = w;
+    }
+#pragma unroll
+    for (int x = 1; x < W; x <<= 1) sum += __shfl_xor(sum, x);
+    __syncthreads();
+    const int total = n0 + n1;
     pa_f32x4 acc{0.f, 0.f, 0.f, 0.f};
-    for (int k = lane / L; k < total; k += S) {
-        const size_t i = index_of(k);
-        const float w = __builtin_amdgcn_exp2f(a.ml[i * 2] - top);
-        acc += *(const pa_f32x4 *)(a.o + i * D + 4 * (lane % L)) * w;
+#pragma unroll 4
+    for (int k = WHOLE ? g : 0; k < total; k += WHOLE ? G : 1) {
+        const int part = k < n0 ? k : a.parts + k - n0;
+        acc += *(const pa_f32x4 *)(a.o + (part * stride + at) * D + d) * s_w[WHOLE ? 0 : g][part];
     }
-#pragma unroll
-    for (int d = L; d < 64; d <<= 1)
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], d);
+    if constexpr (WHOLE) {
+        *(pa_f32x4 *)&s_o[g][d] = acc;
+        __syncthreads();
+        if (tid >= L) return;
+        for (int k = 1; k < G; k++) acc += *(const pa_f32x4 *)&s_o[k][d];
+    }
+    if (rh >= stride) return;
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-    if (lane < L) put4<T>(a, (size_t)rh * D + 4 * lane, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+    put4<T>(a, at * D + d, acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
 }
 
 // ---- host --------------------------------------------------------------------------
 
-constexpr int kSlots = 512;  // tile workgroups that the chip holds at once, two a CU
+constexpr int kCus = 256;
 
 struct Shape {
-    int tiles, parts, own, blocks16;
+    int tiles, parts, span, own, own_span, blocks16;
+    int groups;  // of waves in a tile workgroup
 };
 int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
+// Cut ranges of up to `longest` pages, `average` on average, of `wgs` workgroups so
+// that every one of `slots` gets its share, `least` pages at least, unless that saves
+// less than `worth` pages' time on the longest.
+void cut(long wgs, int longest, long average, int slots, int least, int worth, int &parts, int &span) {
+    span = std::max({least, ceil_div(wgs * average, slots), ceil_div(longest, kMaxParts), 1});
+    if (longest <= span + worth) span = std::max(longest, 1);
+    parts = std::max(1, ceil_div(longest, span));
+}
+
 Shape shape_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, bool shared) {
     const int group = a.heads / p.kv_heads;
-    const int longest = b.max_len > 0 ? std::min<long>(b.max_len, (long)p.blocks * kPage) : p.blocks * kPage;
-    Shape s{0, 1, 1, (group + 15) / 16};
-    auto cut = [&](int wgs, int pages) {  // parts that fill the chip
-        return std::max(1, std::min({kSlots / std::max(wgs, 1), pages / kMinPages, kMaxParts}));
-    };
+    const long longest = b.max_len > 0 ? std::min<long>(b.max_len, (long)p.blocks * kPage) : (long)p.blocks * kPage;
+    const int pages = ceil_div(longest, kPage);
+    Shape s{0, 1, 1, 1, 1, (group + 15) / 16, 1};
     if (shared) {
-        const int common = std::min(a.prefix, longest) / kPage;
+        const int common = (int)std::min<long>(a.prefix, longest) / kPage;
         s.tiles = a.prefix ? ceil_div((long)b.n * group, kRows) : 0;
-        if (s.tiles) s.parts = cut(s.tiles * p.kv_heads, common);
-        s.own = cut(b.n * p.kv_heads * s.blocks16, ceil_div(longest, kPage) - common);
+        const long rows = (long)b.n * p.kv_heads * s.blocks16;
+        // One tile a CU, beside it the rows: at 256 rows behind 16384 positions 75 us
+        // (tiles in both places first, rows after them, 94).  Short parts, as
+        // a page is 1.5 us of one tile's time and the join is launched anyway, yet
+        // not one page each of a longer prefix, which moves more partials than it saves
+        // (64 rows behind 1024: one page 17.4 us, two 16.2; behind 4096: two 21.1, three
+        // 20.2, four 20.8; 8 behind 512: one 9.4, two 10.1).
+        if (s.tiles)
+            cut((long)s.tiles * p.kv_heads, common, common, kCus, common <= 8 ? 1 : common < 48 ? 2 : 3, 0, s.parts, s.span);
+        cut(rows, pages - common, pages - common, kCus, 4, s.tiles ? 0 : 4, s.own, s.own_span);
     } else {
-        const long rows = b.cu ? (long)b.rows * group / kRows + b.n : (long)b.n * ceil_div(group, kRows);
-        s.tiles = (int)rows;
-        s.parts = cut(s.tiles * p.kv_heads, ceil_div(longest, kPage));
+        s.tiles = (int)(b.cu ? (long)b.rows * group / kRows + b.n : (long)b.n * ceil_div(group, kRows));
+        // the rows are an entry's last ones: the first of them attend to less
+        const int average = pages - (int)(std::min<long>(b.rows, longest) / kPage / 2);
+        const long wgs = (long)s.tiles * p.kv_heads;
+        // Two groups of waves, which halve a tile's own time, where the longest
+        // tile takes about as long as the chip needs for all: one prompt of 2048
+        // 48 -> 38 us, of 4096 93 -> 80; three of 2048 would go from 73 to 84, one of
+        // 8192 from 262 to 277.
+        if (pages >= 8 && 5L * pages * kCus >= 4 * wgs * average) s.groups = 2;
+        // Few tiles of long ranges are cut besides (two chunks of 256 over 8192: 68
+        // us with two parts, 50 with four); 260 tiles of one prompt of 2048 are not
+        // (38 us, cut 47: the partials cost what the balance gains).
+        if (wgs <= kCus / 2) cut(wgs, pages, average, 2 * kCus / s.groups, 4, 8, s.parts, s.span);
+        else s.span = pages;
     }
     return s;
 }
@@ -752,24 +916,26 @@ Plan plan_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, const
     r.c = std::max(std::abs(a.scale) * 1.4426950408889634f, 1e-30f);
     r.flip = a.scale < 0 ? 0x80008000u : 0u;
     r.parts = s.parts;
+    r.span = s.span;
     r.own_parts = s.own;
+    r.own_span = s.own_span;
+    r.tiles = s.tiles;
     const size_t rh = (size_t)b.rows * a.heads;
     r.o = ws;
     r.ml = ws + (size_t)(s.parts + s.own) * rh * p.head_dim;
     return r;
 }
 
-template <typename K> void launch_merge(K k, const Plan &a, hipStream_t s) {
-    KernelSpan span("attn_merge", s, true);
-    launch(span, k, dim3((unsigned)(((size_t)a.b.rows * a.heads + 3) / 4)), dim3(256), 0, s, a);
-}
-
 template <typename T, int D> void packed(const Plan &a, const Shape &s, hipStream_t st) {
     {
         KernelSpan span("attn_packed", st, true);
-        launch(span, attn_packed_kernel<T, D>, dim3(s.tiles * s.parts * a.p.kv_heads), dim3(256), 0, st, a);
+        const dim3 grid(s.tiles * s.parts * a.p.kv_heads);
+        if (s.groups == 2) launch(span, attn_packed_kernel<T, D, 2>, grid, dim3(512), 0, st, a);
+        else launch(span, attn_packed_kernel<T, D, 1>, grid, dim3(256), 0, st, a);
     }
-    if (s.parts > 1) launch_merge(attn_merge_kernel<T, D, false>, a, st);
+    if (s.parts == 1) return;
+    KernelSpan span("attn_merge", st, true);
+    launch(span, attn_join_tiles_kernel<T, D>, dim3(std::min<long>((long)s.tiles * (kRows * D / 1024) * a.p.kv_heads, kJoinGrid)), dim3(256), 0, st, a);
 }
 
 template <typename T, int D> void shared(Plan a, const Shape &s, hipStream_t st) {
@@ -780,7 +946,15 @@ template <typename T, int D> void shared(Plan a, const Shape &s, hipStream_t st)
         KernelSpan span("attn_shared", st, true);
         launch(span, attn_shared_kernel<T, D>, dim3(tile_wgs + row_wgs), dim3(256), 0, st, a, tile_wgs);
     }
-    if (!a.direct) launch_merge(attn_merge_kernel<T, D, true>, a, st);
+    if (a.direct) return;
+    constexpr int L = D / 4, G = 256 / L;
+    const long rows = (long)a.b.rows * a.heads;
+    KernelSpan span("attn_merge", st, true);
+    // many parts of few rows: a workgroup a row
+    if (a.parts + a.own_parts > L || (rows < 2048 && a.parts + a.own_parts >= G))
+        launch(span, attn_join_rows_kernel<T, D, true>, dim3((unsigned)rows), dim3(256), 0, st, a);
+    else
+        launch(span, attn_join_rows_kernel<T, D, false>, dim3(ceil_div(rows, G)), dim3(256), 0, st, a);
 }
 
 }  // namespace
