@@ -106,7 +106,6 @@ __device__ __forceinline__ int wave_min(int x) {  // in a scalar register
     return __builtin_amdgcn_readlane(dpp_scan(x, 0x7FFFFFFF, [](int a, int b) { return min(a, b); }), 63);
 }
 
-constexpr int kRows = 128;         // rows of a tile
 constexpr int kMaxParts = 64;      // parts of a split range
 constexpr float kLazyMax = 8.0f;   // weights stay below 2^8 of the running maximum's
 constexpr float kNoMax = -1e30f;   // the maximum before any score: finite, so that -inf - m is -inf
@@ -122,6 +121,7 @@ struct Plan {
     int parts, span;  // a kv range (shared: the prefix) is cut into parts of about `span` pages, `parts` at most
     int own_parts, own_span;  // shared: the same of an entry's own range
     int tiles;        // tiles of one kv head, at most
+    int tile_rows;    // 64 or 128
     int direct;       // shared: no prefix and no split, the row part writes the output
     float *o, *ml;    // partials: [part][rows * heads][D], [part][rows * heads][2]
 };
@@ -162,16 +162,16 @@ __device__ __forceinline__ void put4(const Plan &a, size_t at, float x, float y,
 }
 
 // LDS reads ahead of the products that use them: DEPTH in flight, then one more
-// after every operand's two products.
-template <int READS> __device__ __forceinline__ void read_ahead() {
+// after every operand's products.
+template <int READS, int EACH> __device__ __forceinline__ void read_ahead() {
     constexpr int DEPTH = 6;
     __builtin_amdgcn_sched_group_barrier(0x100, DEPTH, 0);
 #pragma unroll
     for (int i = 0; i < READS - DEPTH; i++) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, 2 * DEPTH, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, EACH * DEPTH, 0);
 }
 
 // Pages of a slot's table: lane i holds that of tile at + i.  The first 64 are loaded by
@@ -207,9 +207,9 @@ template <int D, int KS> struct TileLds {
     int low[4];                        // lowest limit of each wave's rows
 };
 
-// 128 rows of kv head h over pages [t0, t1) of a slot.  PREFIX: row r is entry
+// 64 QB rows of kv head h over pages [t0, t1) of a slot.  PREFIX: row r is entry
 // r / G's, its limit min(common, that entry's length), the result a partial.
-template <typename T, int D, int KS, bool PREFIX>
+template <typename T, int D, int KS, int QB, bool PREFIX>
 __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int h, Ids ids, int slot_positions, Rows rows,
                                           int r0, int t0, int t1, int part, bool partial) {
     typedef typename Mma<T>::vec vec;
@@ -230,12 +230,12 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
 
     // ---- the wave's rows: q as the S^T B operand, lane (grp, c) has dims
     // 32 ks + 8 grp + [0, 8) of row c; rows past the end repeat the last one
-    int limit[2];
-    size_t at[2];  // element of (row, head) in q and out
-    uint4 qu[2][DS];
+    int limit[QB];
+    size_t at[QB];  // element of (row, head) in q and out
+    uint4 qu[QB][DS];
 #pragma unroll
-    for (int qq = 0; qq < 2; qq++) {
-        const int r = min(r0 + wave * 32 + qq * 16 + c, rows.n - 1);
+    for (int qq = 0; qq < QB; qq++) {
+        const int r = min(r0 + wave * (16 * QB) + qq * 16 + c, rows.n - 1);
         const int token = r / a.group, g = r - token * a.group;
         at[qq] = ((size_t)(rows.first + token) * a.heads + h * a.group + g) * D;
 #pragma unroll
@@ -249,27 +249,32 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
         fetch(page, 0, 1);
     }
 
-    vec qf[2][DS];
+    vec qf[QB][DS];
 #pragma unroll
-    for (int qq = 0; qq < 2; qq++)
+    for (int qq = 0; qq < QB; qq++)
 #pragma unroll
         for (int ks = 0; ks < DS; ks++)
             qf[qq][ks] = __builtin_bit_cast(vec, make_uint4(qu[qq][ks].x ^ a.flip, qu[qq][ks].y ^ a.flip,
                                                             qu[qq][ks].z ^ a.flip, qu[qq][ks].w ^ a.flip));
     // lowest limits: of the wave's blocks, and of the tile
-    int low[2];
+    int low[QB];
 #pragma unroll
-    for (int qq = 0; qq < 2; qq++) low[qq] = wave_min(limit[qq]);
-    if (lane == 0) s.low[wave] = min(low[0], low[1]);  // the groups have the same rows
+    for (int qq = 0; qq < QB; qq++) low[qq] = wave_min(limit[qq]);
+    if (lane == 0) s.low[wave] = min(low[0], low[QB - 1]);  // the groups have the same rows
     if (tid < 2) s.flag[tid] = 0;
 
-    const bool live = r0 + wave * 32 < rows.n;  // the wave has a row
-    pa_f32x4 o[DB][2];
+    const bool live = r0 + wave * (16 * QB) < rows.n;  // the wave has a row
+    pa_f32x4 o[DB][QB];
 #pragma unroll
     for (int db = 0; db < DB; db++)
 #pragma unroll
-        for (int qq = 0; qq < 2; qq++) o[db][qq] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
-    float m[2] = {kNoMax, kNoMax}, l[2] = {0.f, 0.f};  // m in units of c s; l this lane's share
+        for (int qq = 0; qq < QB; qq++) o[db][qq] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
+    float m[QB], l[QB];  // m in units of c s; l this lane's share
+#pragma unroll
+    for (int qq = 0; qq < QB; qq++) {
+        m[qq] = kNoMax;
+        l[qq] = 0.f;
+    }
 
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
@@ -314,27 +319,27 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
             odd = s.flag[buf] != 0;
         }
         const bool on = page >= 0 && live;
-        pa_f32x4 sc[4][2];
+        pa_f32x4 sc[4][QB];
         if (on) {
             // ---- S^T = K Q^T, 64 positions x 16 rows a block
 #pragma unroll
             for (int kb = 0; kb < 4; kb++)
 #pragma unroll
-                for (int qq = 0; qq < 2; qq++) sc[kb][qq] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int qq = 0; qq < QB; qq++) sc[kb][qq] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < DS; ks++)
 #pragma unroll
                 for (int kb = 0; kb < 4; kb++) {
                     const vec kf = __builtin_bit_cast(vec, *(const uint4 *)(kt + kb * (16 * D) + ks * 512));
 #pragma unroll
-                    for (int qq = 0; qq < 2; qq++) sc[kb][qq] = Mma<T>::mma(kf, qf[qq][ks], sc[kb][qq]);
+                    for (int qq = 0; qq < QB; qq++) sc[kb][qq] = Mma<T>::mma(kf, qf[qq][ks], sc[kb][qq]);
                 }
-            read_ahead<4 * DS>();
+            read_ahead<4 * DS, QB>();
 
             // ---- softmax
-            float mx[2];
+            float mx[QB];
 #pragma unroll
-            for (int qq = 0; qq < 2; qq++) {
+            for (int qq = 0; qq < QB; qq++) {
                 if (base + kPage > low[qq]) {
 #pragma unroll
                     for (int kb = 0; kb < 4; kb++)
@@ -349,9 +354,9 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
                     for (int i = 0; i < 4; i++) v = fmaxf(v, sc[kb][qq][i]);
                 mx[qq] = v * a.c;
             }
-            if (__any(mx[0] > m[0] + kLazyMax || mx[1] > m[1] + kLazyMax)) {
+            if (__any(mx[0] > m[0] + kLazyMax || mx[QB - 1] > m[QB - 1] + kLazyMax)) {
 #pragma unroll
-                for (int qq = 0; qq < 2; qq++) {
+                for (int qq = 0; qq < QB; qq++) {
                     const float now = fmaxf(m[qq], rows_max(mx[qq]));
                     const float al = __builtin_amdgcn_exp2f(m[qq] - now);
                     m[qq] = now;
@@ -376,7 +381,7 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
                             const uint16_t x = v[(16 * db + 4 * grp + i) * 8];
                             const float y = (x & 0x7FFFu) >= Mma<T>::kInf ? from_elem<T>(x) : 0.f;
 #pragma unroll
-                            for (int qq = 0; qq < 2; qq++) o[db][qq][i] += base + pos < limit[qq] ? y : 0.f;
+                            for (int qq = 0; qq < QB; qq++) o[db][qq][i] += base + pos < limit[qq] ? y : 0.f;
                         }
                 }
             __syncthreads();
@@ -396,10 +401,10 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
         if (on) {
             // ---- weights, and O^T += V^T P^T: the second half's weights between the
             // first half's products
-            vec pf[2], vf[DB], vg[DB];
+            vec pf[QB], vf[DB], vg[DB];
             auto weights = [&](int k2) __attribute__((always_inline)) {
 #pragma unroll
-                for (int qq = 0; qq < 2; qq++) {
+                for (int qq = 0; qq < QB; qq++) {
                     pa_f32x4 x = sc[2 * k2][qq], y = sc[2 * k2 + 1][qq];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
@@ -416,26 +421,27 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
             for (int db = 0; db < DB; db++) vf[db] = __builtin_bit_cast(vec, *(const uint4 *)(vt + db * 128));
             weights(0);
             __builtin_amdgcn_sched_barrier(0);
-            const vec p0 = pf[0], p1 = pf[1];
+            vec first[QB];
+#pragma unroll
+            for (int qq = 0; qq < QB; qq++) first[qq] = pf[qq];
 #pragma unroll
             for (int db = 0; db < DB; db++) {
-                o[db][0] = Mma<T>::mma(vf[db], p0, o[db][0]);
-                o[db][1] = Mma<T>::mma(vf[db], p1, o[db][1]);
+#pragma unroll
+                for (int qq = 0; qq < QB; qq++) o[db][qq] = Mma<T>::mma(vf[db], first[qq], o[db][qq]);
                 vg[db] = __builtin_bit_cast(vec, *(const uint4 *)(vt + 4 * D * 8 + db * 128));
             }
             weights(1);
 #pragma unroll
             for (int i = 0; i < DB; i++) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, QB, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 56 / DB, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 28 * QB / DB, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int db = 0; db < DB; db++) {
-                o[db][0] = Mma<T>::mma(vg[db], pf[0], o[db][0]);
-                o[db][1] = Mma<T>::mma(vg[db], pf[1], o[db][1]);
-            }
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int qq = 0; qq < QB; qq++) o[db][qq] = Mma<T>::mma(vg[db], pf[qq], o[db][qq]);
         }
         page = next;
         __builtin_amdgcn_s_waitcnt(0);
@@ -446,33 +452,33 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
     if constexpr (KS == 2) {
         // the second group hands its (m, l, O) to the first (the last barrier is
         // behind every read of the pages)
-        pa_f32x4 *x = (pa_f32x4 *)&s.kv[0][0][0][0] + (wave * (2 * DB + 1)) * 64 + lane;
-        static_assert(4 * (2 * DB + 1) * 64 * 16 <= (int)sizeof(s.kv), "hand-over");
+        pa_f32x4 *x = (pa_f32x4 *)&s.kv[0][0][0][0] + (wave * (QB * DB + 1)) * 64 + lane;
+        static_assert(4 * (QB * DB + 1) * 64 * 16 <= (int)sizeof(s.kv), "hand-over");
         if (half) {
 #pragma unroll
             for (int db = 0; db < DB; db++)
 #pragma unroll
-                for (int qq = 0; qq < 2; qq++) x[(2 * db + qq) * 64] = o[db][qq];
-            x[2 * DB * 64] = pa_f32x4{m[0], m[1], l[0], l[1]};
+                for (int qq = 0; qq < QB; qq++) x[(QB * db + qq) * 64] = o[db][qq];
+            x[QB * DB * 64] = pa_f32x4{m[0], m[QB - 1], l[0], l[QB - 1]};
         }
         __syncthreads();
         if (half) return;
-        const pa_f32x4 ml = x[2 * DB * 64];
+        const pa_f32x4 ml = x[QB * DB * 64];
 #pragma unroll
-        for (int qq = 0; qq < 2; qq++) {
+        for (int qq = 0; qq < QB; qq++) {
             const float now = fmaxf(m[qq], ml[qq]);
             const float w0 = __builtin_amdgcn_exp2f(m[qq] - now), w1 = __builtin_amdgcn_exp2f(ml[qq] - now);
             m[qq] = now;
             l[qq] = l[qq] * w0 + ml[2 + qq] * w1;
 #pragma unroll
-            for (int db = 0; db < DB; db++) o[db][qq] = o[db][qq] * w0 + x[(2 * db + qq) * 64] * w1;
+            for (int db = 0; db < DB; db++) o[db][qq] = o[db][qq] * w0 + x[(QB * db + qq) * 64] * w1;
         }
     }
 
 #pragma unroll
-    for (int qq = 0; qq < 2; qq++) {
+    for (int qq = 0; qq < QB; qq++) {
         l[qq] = rows_sum(l[qq]);
-        if (r0 + wave * 32 + qq * 16 + c >= rows.n) continue;
+        if (r0 + wave * (16 * QB) + qq * 16 + c >= rows.n) continue;
         if (partial) {
             const size_t rh = at[qq] / D + (size_t)part * a.b.rows * a.heads;
             float *po = a.o + rh * D + 4 * grp;
@@ -491,8 +497,8 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
 }
 
 // Pages that a tile of an entry attends to.
-__device__ __forceinline__ int tile_pages(int len, Span sp, int index, int group) {
-    const int last = min(sp.n - 1, (min((index + 1) * kRows, sp.n * group) - 1) / group);
+__device__ __forceinline__ int tile_pages(const Plan &a, int len, Span sp, int index) {
+    const int last = min(sp.n - 1, (min((index + 1) * a.tile_rows, sp.n * a.group) - 1) / a.group);
     return pages_of(max(0, min(len, len - sp.n + last + 1)));
 }
 
@@ -515,13 +521,13 @@ template <bool SPLIT> __device__ __forceinline__ bool find_tile(const Plan &a, i
             slot = a.b.slots[i];
         }
         const int len = slot_len(a.p, slot);  // for every entry: one load deep, not one more after the search
-        const int tiles = (sp.n * a.group + kRows - 1) / kRows;
+        const int tiles = (sp.n * a.group + a.tile_rows - 1) / a.tile_rows;
         int count = tiles;
         if constexpr (SPLIT) {
             // tile_pages(index) > span from the token on that sees span * 64 + 1 positions
             const long token = max(0L, (long)a.span * kPage - (len - sp.n));
             // the first tile whose last token is that one or a later one
-            count = len > a.span * kPage && token < sp.n ? tiles - (int)(token * a.group / kRows) : 0;
+            count = len > a.span * kPage && token < sp.n ? tiles - (int)(token * a.group / a.tile_rows) : 0;
         }
         const int x = wave_sums(count);
         const uint64_t hit = __ballot(w < before + x);
@@ -539,7 +545,7 @@ template <bool SPLIT> __device__ __forceinline__ bool find_tile(const Plan &a, i
     return false;
 }
 
-template <typename T, int D, int KS> __global__ __launch_bounds__(256 * KS, 2) void attn_packed_kernel(Plan a) {
+template <typename T, int D, int KS, int QB> __global__ __launch_bounds__(256 * KS, 2) void attn_packed_kernel(Plan a) {
     __shared__ __attribute__((aligned(256))) TileLds<D, KS> s;
     // workgroups of one kv head on the same XCDs (workgroup b runs on XCD
     // b % 8), whose L2 then holds that head's pages
@@ -548,10 +554,10 @@ template <typename T, int D, int KS> __global__ __launch_bounds__(256 * KS, 2) v
     Tile t;
     if (!find_tile<false>(a, rest - part * a.tiles, t)) return;
     const Ids ids = ids_of(a.p, t.slot, 0);
-    const int pages = tile_pages(t.len, t.span, t.index, a.group), parts = parts_of(pages, a.span, a.parts);
+    const int pages = tile_pages(a, t.len, t.span, t.index), parts = parts_of(pages, a.span, a.parts);
     if (part >= parts) return;
     const Rows rows{t.span.first, t.span.n * a.group, t.len - t.span.n + 1};
-    tile_part<T, D, KS, false>(a, s, h, ids, t.len, rows, t.index * kRows, (int)((long)part * pages / parts),
+    tile_part<T, D, KS, QB, false>(a, s, h, ids, t.len, rows, t.index * (64 * QB), (int)((long)part * pages / parts),
                            (int)((long)(part + 1) * pages / parts), part, parts > 1);
 }
 
@@ -719,7 +725,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void attn_shar
         const Ids ids = ids_of(a.p, slot0, (int)((long)part * pages_expected / parts_of(pages_expected, a.span, a.parts)));
         const int common = common_of(a), pages = common / kPage, parts = parts_of(pages, a.span, a.parts);
         if (part >= parts || pages == 0) return;
-        tile_part<T, D, 1, true>(a, s.tile, h, ids, common, Rows{0, a.b.n * a.group, 0}, rest / a.parts * kRows,
+        tile_part<T, D, 1, 2, true>(a, s.tile, h, ids, common, Rows{0, a.b.n * a.group, 0}, rest / a.parts * 128,
                                  (int)((long)part * pages / parts), (int)((long)(part + 1) * pages / parts), part, true);
         return;
     }
@@ -755,9 +761,10 @@ template <typename T, int D> __global__ __launch_bounds__(256) void attn_join_ti
     for (int u = blockIdx.x;; u += gridDim.x) {
         const int h = u % a.p.kv_heads, rest = u / a.p.kv_heads;
         Tile t;
-        if (!find_tile<true>(a, rest / (kRows / G), t)) return;
-        const int n = parts_of(tile_pages(t.len, t.span, t.index, a.group), a.span, a.parts);
-        const int r = t.index * kRows + rest % (kRows / G) * G + g;
+        const int chunks = a.tile_rows / G;
+        if (!find_tile<true>(a, rest / chunks, t)) return;
+        const int n = parts_of(tile_pages(a, t.len, t.span, t.index), a.span, a.parts);
+        const int r = t.index * a.tile_rows + rest % chunks * G + g;
         const bool on = r < t.span.n * a.group;
         const int token = min(r, t.span.n * a.group - 1) / a.group;
         const size_t at = (size_t)(t.span.first + token) * a.heads + h * a.group + (on ? r - token * a.group : 0);
@@ -853,6 +860,7 @@ constexpr int kCus = 256;
 struct Shape {
     int tiles, parts, span, own, own_span, blocks16;
     int groups;  // of waves in a tile workgroup
+    int rows;    // of a tile
 };
 int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
@@ -869,10 +877,10 @@ Shape shape_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, boo
     const int group = a.heads / p.kv_heads;
     const long longest = b.max_len > 0 ? std::min<long>(b.max_len, (long)p.blocks * kPage) : (long)p.blocks * kPage;
     const int pages = ceil_div(longest, kPage);
-    Shape s{0, 1, 1, 1, 1, (group + 15) / 16, 1};
+    Shape s{0, 1, 1, 1, 1, (group + 15) / 16, 1, 128};
     if (shared) {
         const int common = (int)std::min<long>(a.prefix, longest) / kPage;
-        s.tiles = a.prefix ? ceil_div((long)b.n * group, kRows) : 0;
+        s.tiles = a.prefix ? ceil_div((long)b.n * group, s.rows) : 0;
         const long rows = (long)b.n * p.kv_heads * s.blocks16;
         // One tile a CU, beside it the rows: at 256 rows behind 16384 positions 75 us
         // (tiles in both places first, rows after them, 94).  Short parts, as
@@ -884,7 +892,10 @@ Shape shape_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, boo
             cut((long)s.tiles * p.kv_heads, common, common, kCus, common <= 8 ? 1 : common < 48 ? 2 : 3, 0, s.parts, s.span);
         cut(rows, pages - common, pages - common, kCus, 4, s.tiles ? 0 : 4, s.own, s.own_span);
     } else {
-        s.tiles = (int)(b.cu ? (long)b.rows * group / kRows + b.n : (long)b.n * ceil_div(group, kRows));
+        auto tiles = [&](int rows) {
+            return (int)(b.cu ? (long)b.rows * group / rows + b.n : (long)b.n * ceil_div(group, rows));
+        };
+        s.tiles = tiles(s.rows);
         // the rows are an entry's last ones: the first of them attend to less
         const int average = pages - (int)(std::min<long>(b.rows, longest) / kPage / 2);
         const long wgs = (long)s.tiles * p.kv_heads;
@@ -894,10 +905,18 @@ Shape shape_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, boo
         // 8192 from 262 to 277.
         if (pages >= 8 && 5L * pages * kCus >= 4 * wgs * average) s.groups = 2;
         // Few tiles of long ranges are cut besides (two chunks of 256 over 8192: 68
-        // us with two parts, 50 with four); 260 tiles of one prompt of 2048 are not
-        // (38 us, cut 47: the partials cost what the balance gains).
-        if (wgs <= kCus / 2) cut(wgs, pages, average, 2 * kCus / s.groups, 4, 8, s.parts, s.span);
+        // us with two parts, 50 with four).  Shorter ranges or more tiles are not: one
+        // prompt of 1000 cut in four 34 us, whole 17; of 2048 47 and 38.
+        if (wgs <= kCus / 2) cut(wgs, pages, average, 2 * kCus / s.groups, 4, 24, s.parts, s.span);
         else s.span = pages;
+        // Tiles of half the rows, as a tile's time is mostly its own chain of reads
+        // and products, as long as they do not queue for the CUs (128 rows and 64: one
+        // sentence 8.6 and 6.6 us, 32 of them 11.0 and 10.0, one prompt of 700 18.8 and
+        // 13.5, of 2048 37.6 and 34.2; but 12 of 200 16.0 and 17.1, 64 of 61 16.1 and 18.2).
+        if (s.parts == 1 && 8 * wgs <= 9 * kCus) {
+            s.rows = 64;
+            s.tiles = tiles(s.rows);
+        }
     }
     return s;
 }
@@ -920,6 +939,7 @@ Plan plan_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, const
     r.own_parts = s.own;
     r.own_span = s.own_span;
     r.tiles = s.tiles;
+    r.tile_rows = s.rows;
     const size_t rh = (size_t)b.rows * a.heads;
     r.o = ws;
     r.ml = ws + (size_t)(s.parts + s.own) * rh * p.head_dim;
@@ -930,12 +950,17 @@ template <typename T, int D> void packed(const Plan &a, const Shape &s, hipStrea
     {
         KernelSpan span("attn_packed", st, true);
         const dim3 grid(s.tiles * s.parts * a.p.kv_heads);
-        if (s.groups == 2) launch(span, attn_packed_kernel<T, D, 2>, grid, dim3(512), 0, st, a);
-        else launch(span, attn_packed_kernel<T, D, 1>, grid, dim3(256), 0, st, a);
+        if (s.rows == 64) {
+            if (s.groups == 2) launch(span, attn_packed_kernel<T, D, 2, 1>, grid, dim3(512), 0, st, a);
+            else launch(span, attn_packed_kernel<T, D, 1, 1>, grid, dim3(256), 0, st, a);
+        } else {
+            if (s.groups == 2) launch(span, attn_packed_kernel<T, D, 2, 2>, grid, dim3(512), 0, st, a);
+            else launch(span, attn_packed_kernel<T, D, 1, 2>, grid, dim3(256), 0, st, a);
+        }
     }
     if (s.parts == 1) return;
     KernelSpan span("attn_merge", st, true);
-    launch(span, attn_join_tiles_kernel<T, D>, dim3(std::min<long>((long)s.tiles * (kRows * D / 1024) * a.p.kv_heads, kJoinGrid)), dim3(256), 0, st, a);
+    launch(span, attn_join_tiles_kernel<T, D>, dim3(std::min<long>((long)s.tiles * (s.rows * D / 1024) * a.p.kv_heads, kJoinGrid)), dim3(256), 0, st, a);
 }
 
 template <typename T, int D> void shared(Plan a, const Shape &s, hipStream_t st) {
