@@ -712,7 +712,7 @@ __device__ __forceinline__ int common_of(const Plan &a) {
 }
 
 // Workgroups [0, tile_wgs) the prefix, the others the entries' own positions.
-template <typename T, int D> __global__ __launch_bounds__(256, 2) void attn_shared_kernel(Plan a, int tile_wgs) {
+template <typename T, int D, int QB> __global__ __launch_bounds__(256, 2) void attn_shared_kernel(Plan a, int tile_wgs) {
     __shared__ __attribute__((aligned(256))) union {
         TileLds<D, 1> tile;
         RowLds<D> row;
@@ -725,7 +725,7 @@ template <typename T, int D> __global__ __launch_bounds__(256, 2) void attn_shar
         const Ids ids = ids_of(a.p, slot0, (int)((long)part * pages_expected / parts_of(pages_expected, a.span, a.parts)));
         const int common = common_of(a), pages = common / kPage, parts = parts_of(pages, a.span, a.parts);
         if (part >= parts || pages == 0) return;
-        tile_part<T, D, 1, 2, true>(a, s.tile, h, ids, common, Rows{0, a.b.n * a.group, 0}, rest / a.parts * 128,
+        tile_part<T, D, 1, QB, true>(a, s.tile, h, ids, common, Rows{0, a.b.n * a.group, 0}, rest / a.parts * (64 * QB),
                                  (int)((long)part * pages / parts), (int)((long)(part + 1) * pages / parts), part, true);
         return;
     }
@@ -880,16 +880,18 @@ Shape shape_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, boo
     Shape s{0, 1, 1, 1, 1, (group + 15) / 16, 1, 128};
     if (shared) {
         const int common = (int)std::min<long>(a.prefix, longest) / kPage;
+        // tiles of 64 rows until a CU has more than 8 pages of them (128 rows and 64: 8
+        // rows behind 512 positions 9.4 and 8.6 us, 64 behind 4096 20.3 and 18.3, 128 22.1 and
+        // 21.3; 256 behind 16384 73 and 88)
+        if ((long)ceil_div((long)b.n * group, 64) * p.kv_heads * common <= 8 * kCus) s.rows = 64;
         s.tiles = a.prefix ? ceil_div((long)b.n * group, s.rows) : 0;
         const long rows = (long)b.n * p.kv_heads * s.blocks16;
         // One tile a CU, beside it the rows: at 256 rows behind 16384 positions 75 us
         // (tiles in both places first, rows after them, 94).  Short parts, as
-        // a page is 1.5 us of one tile's time and the join is launched anyway, yet
-        // not one page each of a longer prefix, which moves more partials than it saves
-        // (64 rows behind 1024: one page 17.4 us, two 16.2; behind 4096: two 21.1, three
-        // 20.2, four 20.8; 8 behind 512: one 9.4, two 10.1).
-        if (s.tiles)
-            cut((long)s.tiles * p.kv_heads, common, common, kCus, common <= 8 ? 1 : common < 48 ? 2 : 3, 0, s.parts, s.span);
+        // the join is launched anyway, yet not one page each of a longer prefix,
+        // which moves more partials than it saves (64 rows behind 1024: one page 15.6 us,
+        // three 13.9; 16 behind 8192: two 16.8, three 15.5; 8 behind 512: one 9.4, two 10.1).
+        if (s.tiles) cut((long)s.tiles * p.kv_heads, common, common, kCus, common <= 8 ? 1 : 3, 0, s.parts, s.span);
         cut(rows, pages - common, pages - common, kCus, 4, s.tiles ? 0 : 4, s.own, s.own_span);
     } else {
         auto tiles = [&](int rows) {
@@ -969,7 +971,8 @@ template <typename T, int D> void shared(Plan a, const Shape &s, hipStream_t st)
     if (s.tiles == 0) a.parts = 0;
     {
         KernelSpan span("attn_shared", st, true);
-        launch(span, attn_shared_kernel<T, D>, dim3(tile_wgs + row_wgs), dim3(256), 0, st, a, tile_wgs);
+        if (s.rows == 64) launch(span, attn_shared_kernel<T, D, 1>, dim3(tile_wgs + row_wgs), dim3(256), 0, st, a, tile_wgs);
+        else launch(span, attn_shared_kernel<T, D, 2>, dim3(tile_wgs + row_wgs), dim3(256), 0, st, a, tile_wgs);
     }
     if (a.direct) return;
     constexpr int L = D / 4, G = 256 / L;
