@@ -24,6 +24,24 @@ template <> __device__ __forceinline__ uint16_t bits_of<BF16>(float x) {
     return __builtin_bit_cast(uint16_t, (__bf16)x);
 }
 
+// Wave-wide steps by DPP: within rows of 16 lanes, then row 15 -> the next row and lane
+// 31 -> the upper half.  Lane 63 has seen all 64 lanes.
+template <typename F> __device__ __forceinline__ int dpp_scan(int x, int none, F f) {
+    x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x111, 0xF, 0xF, false));  // row_shr:1, 2, 4, 8
+    x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x112, 0xF, 0xF, false));
+    x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x114, 0xF, 0xF, false));
+    x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x118, 0xF, 0xF, false));
+    x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x142, 0xA, 0xF, false));  // row_bcast:15 into rows 1 and 3
+    x = f(x, __builtin_amdgcn_update_dpp(none, x, 0x143, 0xC, 0xF, false));  // row_bcast:31 into rows 2 and 3
+    return x;
+}
+__device__ __forceinline__ int wave_sums(int x) {  // of the lanes up to each
+    return dpp_scan(x, 0, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ int wave_min(int x) {  // in a scalar register
+    return __builtin_amdgcn_readlane(dpp_scan(x, 0x7FFFFFFF, [](int a, int b) { return min(a, b); }), 63);
+}
+
 // words of hymt_paged::work
 enum { kWorkFirst = 0, kWorkCopies = 1, kWorkLive = 2, kWorkStatus = 3, kWorkLists = 4 };
 

@@ -27,53 +27,32 @@ __device__ __forceinline__ int32_t *work_map(const hymt_paged &p) { return p.wor
 
 __device__ __forceinline__ int blocks_of(int len) { return (len + kPage - 1) / kPage; }
 
-// Exclusive prefix sum over the workgroup's threads, and the total.
-__device__ int block_scan(int v, int *s_wave, int &total) {
+// Exclusive prefix sums of two values over the workgroup's threads, and their totals.
+struct Sums {
+    int a, b, all_a, all_b;
+};
+__device__ __forceinline__ Sums block_scan(int va, int vb, int2 *s_wave) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
+    const int xa = wave_sums(va), xb = wave_sums(vb);
     __syncthreads();  // s_wave's last readers
-    if (lane == 63) s_wave[wave] = x;
+    if (lane == 63) s_wave[wave] = make_int2(xa, xb);
     __syncthreads();
-    int base = 0, sum = 0;
+    Sums r{xa - va, xb - vb, 0, 0};
 #pragma unroll
     for (int w = 0; w < kPlanWaves; w++) {
-        const int t = s_wave[w];
-        if (w < wave) base += t;
-        sum += t;
+        const int2 t = s_wave[w];
+        if (w == wave) {
+            r.a += r.all_a;
+            r.b += r.all_b;
+        }
+        r.all_a += t.x;
+        r.all_b += t.y;
     }
-    total = sum;
-    return base + x - v;
+    return r;
 }
 
-// The pages [lo, hi) in ascending order, 1024 at a time: f(page, refs, valid) for
-// every thread of the workgroup alike.
-template <typename F> __device__ __forceinline__ void for_pages(const hymt_paged &p, int lo, int hi, F f) {
-    for (int base = lo; base < hi; base += kPlanThreads) {
-        const int i = base + (int)threadIdx.x;
-        const bool ok = i < hi;
-        f(i, ok ? p.refs[i] : 0, ok);
-    }
-}
-
-// The `need` lowest free pages into list[0 .. need); false if there are fewer.
-__device__ bool find_free(const hymt_paged &p, int need, int32_t *list, int *s_wave) {
-    int found = 0;
-    for (int base = 0; base < p.pages && found < need; base += kPlanThreads) {
-        const int i = base + (int)threadIdx.x;
-        const int free = i < p.pages && p.refs[i] <= 0;
-        int total;
-        const int at = found + block_scan(free, s_wave, total);
-        if (free && at < need) list[at] = i;
-        found += total;
-    }
-    __syncthreads();
-    return found >= need;
-}
+// Whether page `page` of the pool can be had; a page past the end cannot.
+__device__ __forceinline__ int is_free(const hymt_paged &p, int page) { return page < p.pages && p.refs[page] <= 0; }
 
 // One thread ends a call: its status, and the first that was not good.
 __device__ void finish(const hymt_paged &p, int status, int copies) {
@@ -83,12 +62,10 @@ __device__ void finish(const hymt_paged &p, int status, int copies) {
 }
 
 // Pages in use (all threads get the number).
-__device__ int count_live(const hymt_paged &p, int *s_wave) {
+__device__ int count_live(const hymt_paged &p, int2 *s_wave) {
     int mine = 0;
     for (int i = threadIdx.x; i < p.pages; i += kPlanThreads) mine += p.refs[i] > 0;
-    int total;
-    block_scan(mine, s_wave, total);
-    return total;
+    return block_scan(mine, 0, s_wave).all_a;
 }
 
 // A slot's place in a bit per slot; true if it was set already.
@@ -99,8 +76,9 @@ __device__ __forceinline__ bool mark(uint32_t *bits, int slot) {
 
 struct PlanShared {
     uint32_t bits[kPagedMaxSeqs / 32];
-    int wave[kPlanWaves];
+    int2 wave[kPlanWaves];
     int status;
+    int free[kPlanThreads];  // the lowest free pages handed out
     int slot[HYMT_PAGED_BATCH], first[HYMT_PAGED_BATCH], count[HYMT_PAGED_BATCH], rank[HYMT_PAGED_BATCH];
 };
 
@@ -116,18 +94,49 @@ __device__ __forceinline__ void plan_fail(PlanShared &sh, int code) {
     while (old != HYMT_OK && code < old) old = atomicCAS(&sh.status, old, code);
 }
 
+// Ranks of the entries' `need` free pages, lowest pages first: entry i gets
+// [rank, rank + need) of list, of which the first 1024 are in sh.free too.  free0 is
+// is_free of page threadIdx.x, loaded before it was known how many are needed.
+// False if there are too few.
+__device__ bool hand_out(const hymt_paged &p, PlanShared &sh, int need, int free0, int32_t *list, int &rank, int &total) {
+    const int tid = threadIdx.x;
+    Sums s = block_scan(need, free0, sh.wave);
+    rank = s.a;
+    total = s.all_a;
+    int at = s.b, found = s.all_b, page = tid, free = free0;
+    for (int base = kPlanThreads;; base += kPlanThreads) {
+        if (free && at < total) {
+            list[at] = page;
+            if (at < kPlanThreads) sh.free[at] = page;
+        }
+        if (found >= total || base >= p.pages) break;
+        page = base + tid;
+        free = is_free(p, page);
+        s = block_scan(0, free, sh.wave);
+        at = found + s.b;
+        found += s.all_b;
+    }
+    __syncthreads();
+    return found >= total;
+}
+
 __global__ __launch_bounds__(kPlanThreads) void paged_extend_kernel(hymt_paged p, const int32_t *slots,
                                                                     const int32_t *cu, int n) {
     __shared__ PlanShared sh;
-    plan_begin(sh, p.seqs);
-    const int i = threadIdx.x;
-    int slot = -1, len = 0, add = 0, need = 0;
+    const int i = threadIdx.x, free0 = is_free(p, i);
+    int slot = -1, from = 0, to = 0;
     if (i < n) {
         slot = slots[i];
-        add = cu ? cu[i + 1] - cu[i] : 1;
-        if ((unsigned)slot >= (unsigned)p.seqs || add < 0 || (cu && i == 0 && cu[0] != 0) || mark(sh.bits, slot)) {
+        from = cu ? cu[i] : i;
+        to = cu ? cu[i + 1] : i + 1;
+    }
+    plan_begin(sh, p.seqs);
+    int len = 0, add = 0, need = 0;
+    if (i < n) {
+        if ((unsigned)slot >= (unsigned)p.seqs || to < from || (i == 0 && from != 0) || mark(sh.bits, slot)) {
             plan_fail(sh, HYMT_E_ARG);
         } else {
+            add = to - from;  // offsets that rise from 0 on: all together below 2^31
             len = p.len[slot];
             const long cap = (long)p.blocks * kPage;
             if (len < 0 || len > cap) plan_fail(sh, HYMT_E_STATE);
@@ -141,13 +150,9 @@ __global__ __launch_bounds__(kPlanThreads) void paged_extend_kernel(hymt_paged p
             }
         }
     }
-    int total;
-    const int rank = block_scan(need, sh.wave, total);
     int32_t *list = work_src(p);
-    bool enough = true;
-    if (total > p.pages) enough = false;
-    else if (total > 0) enough = find_free(p, total, list, sh.wave);
-    if (!enough && i == 0) plan_fail(sh, HYMT_E_CAPACITY);
+    int rank, total;
+    if (!hand_out(p, sh, need, free0, list, rank, total) && i == 0) plan_fail(sh, HYMT_E_CAPACITY);
     __syncthreads();
     if (sh.status != HYMT_OK) {
         if (i == 0) finish(p, sh.status, 0);
@@ -160,33 +165,33 @@ __global__ __launch_bounds__(kPlanThreads) void paged_extend_kernel(hymt_paged p
         sh.rank[i] = rank;
         p.len[slot] = len + add;
     }
-    __syncthreads();
-    if (total > 0)
+    if (total > 0) {
+        __syncthreads();
         for (int e = threadIdx.x >> 6; e < n; e += kPlanWaves)
             for (int j = threadIdx.x & 63; j < sh.count[e]; j += 64) {
-                const int page = list[sh.rank[e] + j];
+                const int at = sh.rank[e] + j, page = at < kPlanThreads ? sh.free[at] : list[at];
                 p.table[(size_t)sh.slot[e] * p.blocks + sh.first[e] + j] = page;
                 p.refs[page] = 1;
             }
-    __syncthreads();
+    }
     if (i == 0) finish(p, HYMT_OK, 0);
 }
 
 __global__ __launch_bounds__(kPlanThreads) void paged_fork_plan_kernel(hymt_paged p, const int32_t *parent,
                                                                        const int32_t *child, int n) {
     __shared__ PlanShared sh;
-    plan_begin(sh, p.seqs);
-    const int i = threadIdx.x;
+    const int i = threadIdx.x, free0 = is_free(p, i);
     int from = 0, to = 0, len = 0, need = 0, src = 0;
+    bool known = false;
     if (i < n) {
         from = parent[i];
         to = child[i];
-        if ((unsigned)from >= (unsigned)p.seqs || (unsigned)to >= (unsigned)p.seqs || mark(sh.bits, to))
-            plan_fail(sh, HYMT_E_ARG);
+        known = (unsigned)from < (unsigned)p.seqs && (unsigned)to < (unsigned)p.seqs;
     }
-    __syncthreads();
-    if (i < n && (unsigned)from < (unsigned)p.seqs && (unsigned)to < (unsigned)p.seqs) {
-        if (sh.bits[from >> 5] >> (from & 31) & 1) plan_fail(sh, HYMT_E_ARG);
+    plan_begin(sh, p.seqs);
+    if (i < n && (!known || mark(sh.bits, to))) plan_fail(sh, HYMT_E_ARG);
+    if (i < n) sh.count[i] = 0;
+    if (known) {
         len = p.len[from];
         if (len < 0 || len > (long)p.blocks * kPage || p.len[to] != 0) {
             plan_fail(sh, HYMT_E_STATE);
@@ -200,17 +205,15 @@ __global__ __launch_bounds__(kPlanThreads) void paged_fork_plan_kernel(hymt_page
         sh.slot[i] = from;
         sh.count[i] = len / kPage;
     }
-    int total;
-    const int rank = block_scan(need, sh.wave, total);
-    int32_t *list = work_dst(p);
-    const bool enough = total <= p.pages && (total == 0 || find_free(p, total, list, sh.wave));
-    if (!enough && i == 0) plan_fail(sh, HYMT_E_CAPACITY);
     __syncthreads();
+    if (known && (sh.bits[from >> 5] >> (from & 31) & 1)) plan_fail(sh, HYMT_E_ARG);
     // whole pages have to be in the pool before one of them is counted again
-    if (sh.status == HYMT_OK)
-        for (int e = threadIdx.x >> 6; e < n; e += kPlanWaves)
-            for (int j = threadIdx.x & 63; j < sh.count[e]; j += 64)
-                if ((unsigned)p.table[(size_t)sh.slot[e] * p.blocks + j] >= (unsigned)p.pages) plan_fail(sh, HYMT_E_STATE);
+    for (int e = threadIdx.x >> 6; e < n; e += kPlanWaves)
+        for (int j = threadIdx.x & 63; j < sh.count[e]; j += 64)
+            if ((unsigned)p.table[(size_t)sh.slot[e] * p.blocks + j] >= (unsigned)p.pages) plan_fail(sh, HYMT_E_STATE);
+    int32_t *list = work_dst(p);
+    int rank, total;
+    if (!hand_out(p, sh, need, free0, list, rank, total) && i == 0) plan_fail(sh, HYMT_E_CAPACITY);
     __syncthreads();
     if (sh.status != HYMT_OK) {
         if (i == 0) finish(p, sh.status, 0);
@@ -219,7 +222,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_fork_plan_kernel(hymt_page
     if (i < n) {
         p.len[to] = len;
         if (need) {
-            const int dst = list[rank];
+            const int dst = sh.free[rank];
             work_src(p)[rank] = src;
             p.table[(size_t)to * p.blocks + len / kPage] = dst;
             p.refs[dst] = 1;
@@ -231,12 +234,15 @@ __global__ __launch_bounds__(kPlanThreads) void paged_fork_plan_kernel(hymt_page
 __global__ __launch_bounds__(kPlanThreads) void paged_set_len_plan_kernel(hymt_paged p, const int32_t *slots,
                                                                           const int32_t *lens, int n) {
     __shared__ PlanShared sh;
-    plan_begin(sh, p.seqs);
-    const int i = threadIdx.x;
+    const int i = threadIdx.x, free0 = is_free(p, i);
     int slot = 0, len = 0, want = 0, need = 0, src = 0;
     if (i < n) {
         slot = slots[i];
         want = lens ? lens[i] : 0;
+    }
+    plan_begin(sh, p.seqs);
+    if (i < n) {
+        sh.count[i] = 0;
         if ((unsigned)slot >= (unsigned)p.seqs || want < 0 || mark(sh.bits, slot)) plan_fail(sh, HYMT_E_ARG);
         else {
             len = p.len[slot];
@@ -255,17 +261,14 @@ __global__ __launch_bounds__(kPlanThreads) void paged_set_len_plan_kernel(hymt_p
             sh.count[i] = blocks_of(len) - blocks_of(want);
         }
     }
-    int total;
-    const int rank = block_scan(need, sh.wave, total);
-    int32_t *list = work_dst(p);
-    const bool enough = total <= p.pages && (total == 0 || find_free(p, total, list, sh.wave));
-    if (!enough && i == 0) plan_fail(sh, HYMT_E_CAPACITY);
     __syncthreads();
-    if (sh.status == HYMT_OK)
-        for (int e = threadIdx.x >> 6; e < n; e += kPlanWaves)
-            for (int j = threadIdx.x & 63; j < sh.count[e]; j += 64)
-                if ((unsigned)p.table[(size_t)sh.slot[e] * p.blocks + sh.first[e] + j] >= (unsigned)p.pages)
-                    plan_fail(sh, HYMT_E_STATE);
+    for (int e = threadIdx.x >> 6; e < n; e += kPlanWaves)
+        for (int j = threadIdx.x & 63; j < sh.count[e]; j += 64)
+            if ((unsigned)p.table[(size_t)sh.slot[e] * p.blocks + sh.first[e] + j] >= (unsigned)p.pages)
+                plan_fail(sh, HYMT_E_STATE);
+    int32_t *list = work_dst(p);
+    int rank, total;
+    if (!hand_out(p, sh, need, free0, list, rank, total) && i == 0) plan_fail(sh, HYMT_E_CAPACITY);
     __syncthreads();
     if (sh.status != HYMT_OK) {
         if (i == 0) finish(p, sh.status, 0);
@@ -274,7 +277,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_set_len_plan_kernel(hymt_p
     if (i < n) {
         p.len[slot] = want;
         if (need) {
-            const int dst = list[rank];
+            const int dst = sh.free[rank];
             work_src(p)[rank] = src;
             p.table[(size_t)slot * p.blocks + want / kPage] = dst;
             p.refs[dst] = 1;
@@ -291,23 +294,20 @@ __global__ __launch_bounds__(kPlanThreads) void paged_set_len_plan_kernel(hymt_p
 }
 
 __global__ __launch_bounds__(kPlanThreads) void paged_compact_plan_kernel(hymt_paged p) {
-    __shared__ int s_wave[kPlanWaves];
+    __shared__ int2 s_wave[kPlanWaves];
     const int live = count_live(p, s_wave);
-    int holes = 0, movers = 0, total;
-    for_pages(p, 0, live, [&](int i, int refs, bool ok) {
-        const int free = ok && refs <= 0;
-        const int at = holes + block_scan(free, s_wave, total);
-        if (free) work_dst(p)[at] = i;
-        holes += total;
-    });
-    for_pages(p, live, p.pages, [&](int i, int refs, bool ok) {
-        const int used = ok && refs > 0;
-        const int at = movers + block_scan(used, s_wave, total);
-        if (used) work_src(p)[at] = i;
-        movers += total;
-    });
-    __syncthreads();  // as many holes below `live` as pages in use above
-    for (int i = live + (int)threadIdx.x; i < p.pages; i += kPlanThreads) work_map(p)[i] = i;
+    // as many holes below `live` as pages in use from there on
+    int holes = 0, movers = 0;
+    for (int base = 0; base < p.pages; base += kPlanThreads) {
+        const int i = base + (int)threadIdx.x, refs = i < p.pages ? p.refs[i] : 0;
+        const int hole = i < live && refs <= 0, mover = i >= live && refs > 0;
+        const Sums s = block_scan(hole, mover, s_wave);
+        if (hole) work_dst(p)[holes + s.a] = i;
+        if (mover) work_src(p)[movers + s.b] = i;
+        if (i >= live && i < p.pages) work_map(p)[i] = i;
+        holes += s.all_a;
+        movers += s.all_b;
+    }
     __syncthreads();
     for (int k = threadIdx.x; k < movers; k += kPlanThreads) {
         const int src = work_src(p)[k], dst = work_dst(p)[k];
@@ -684,12 +684,7 @@ __global__ __launch_bounds__(256) void rope_block_kernel(hymt_paged p, hymt_batc
         }
         const int at = slot_length(p, sl) - cnt;
         const int blocks = cnt ? ((at + cnt - 1) >> 5) - (at >> 5) + 1 : 0;
-        int x = blocks;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int y = __shfl_up(x, d);
-            if (lane >= d) x += y;
-        }
+        const int x = wave_sums(blocks);
         const uint64_t hit = __ballot(w < before + x);
         if (hit) {
             const int k = __ffsll((unsigned long long)hit) - 1;

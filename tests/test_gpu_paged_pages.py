@@ -241,6 +241,7 @@ A, CAP, ST = N.HYMT_E_ARG, N.HYMT_E_CAPACITY, N.HYMT_E_STATE
     ([1, 0], [64, 200], {}, CAP),                 # more than blocks * 64 positions
     ([0, 1, 3], [29, 65, 64], {}, CAP),           # four pages, two free
     ([0], [2 ** 30], {}, CAP),
+    ([0, 1, 2], [2 ** 30, 2 ** 30, 2 ** 30], {}, A),  # offsets past 2^31
     ([0], [1], {"len": (0, 257)}, ST), ([0], [1], {"len": (0, -1)}, ST),
     ([0], [1], {"table": ((0, 1), 8)}, ST), ([0], [1], {"table": ((0, 1), -1)}, ST),
 ])
@@ -289,6 +290,26 @@ def test_no_entries(be):
     be.paged_set_len(dev, s, 0)
     equal(c, room, dev)
     room.close()
+
+
+def test_a_million_pages_for_one_slot(be):
+    need = (1 << 20) + 7
+    dev = be.paged_create(1, 2 * need + 3, 2, need + 1, kv_heads=1, head_dim=64)
+    room = Room(be)
+    try:
+        be.paged_extend(dev, ints(room, [1, 0]), 2, cu=ints(room, [0, 64 * need, 64 * need + 64 * need - 63]))
+        assert be.paged_work(dev) == {"first": 0, "copies": 0, "live": 0, "status": 0}
+        table = be.download(np.empty((2, need + 1), np.int32), dev.table)
+        refs = be.download(np.empty(2 * need + 3, np.int32), dev.refs)
+        np.testing.assert_array_equal(table, [[*range(need, 2 * need), -1], [*range(need), -1]])
+        np.testing.assert_array_equal(refs, [1] * (2 * need) + [0] * 3)
+        be.paged_set_len(dev, ints(room, [1]), 1)
+        be.paged_compact(dev)
+        table = be.download(np.empty((2, need + 1), np.int32), dev.table)
+        assert sorted(table[0, :need]) == [*range(need)] and (table[1] == -1).all()
+    finally:
+        room.close()
+        be.paged_free(dev)
 
 
 def test_pools_past_2_32_bytes(be):
