@@ -25,6 +25,8 @@
 // Weights are rounded to the cache's type for the product with V and
 // summed as rounded, so they sum to 1.
 #include <algorithm>
+#include <limits>
+
 #include "attn_kernels.hpp"
 #include "device_common.hpp"
 #include "ktimer.hpp"
@@ -90,7 +92,15 @@ __device__ __forceinline__ float rows_sum(float v) {
 }
 constexpr int kMaxParts = 64;      // parts of a split range
 constexpr float kLazyMax = 8.0f;   // weights stay below 2^8 of the running maximum's
-constexpr float kNoMax = -1e30f;   // the maximum before any score: finite, so that -inf - m is -inf
+constexpr float kNoMax = -3.4028234e38f;  // the maximum before any score: finite, so that -inf - m is -inf
+// c s - m in one fma has the rounding of m = c max s left over, |m| 2^-25 of a power of
+// 2: from here on (2^-13) the product is rounded first, so that it is 0 where s is the
+// maximum, in every part of a range
+constexpr float kFarMax = 4096.f;
+__device__ __forceinline__ float product_less(float x, float y, float z) {
+#pragma clang fp contract(off)
+    return x * y - z;
+}
 
 struct Plan {
     hymt_paged p;
@@ -252,6 +262,7 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
 #pragma unroll
         for (int qq = 0; qq < QB; qq++) o[db][qq] = pa_f32x4{0.f, 0.f, 0.f, 0.f};
     float m[QB], l[QB];  // m in units of c s; l this lane's share
+    bool far = false;    // some |m| of the wave is beyond kFarMax
 #pragma unroll
     for (int qq = 0; qq < QB; qq++) {
         m[qq] = kNoMax;
@@ -303,7 +314,9 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
         const bool on = page >= 0 && live;
         pa_f32x4 sc[4][QB];
         if (on) {
-            // ---- S^T = K Q^T, 64 positions x 16 rows a block
+            // ---- S^T = K Q^T, 64 positions x 16 rows a block.  Of two workgroups on
+            // a CU the one at its products goes first (four prompts of 8192 512 -> 497 us)
+            if constexpr (KS == 1) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int kb = 0; kb < 4; kb++)
 #pragma unroll
@@ -317,6 +330,7 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
                     for (int qq = 0; qq < QB; qq++) sc[kb][qq] = Mma<T>::mma(kf, qf[qq][ks], sc[kb][qq]);
                 }
             read_ahead<4 * DS, QB>();
+            if constexpr (KS == 1) __builtin_amdgcn_s_setprio(0);
 
             // ---- softmax
             float mx[QB];
@@ -346,7 +360,17 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
 #pragma unroll
                     for (int db = 0; db < DB; db++) o[db][qq] *= al;
                 }
+                far = false;
+#pragma unroll
+                for (int qq = 0; qq < QB; qq++) far |= __any(m[qq] != kNoMax && fabsf(m[qq]) > kFarMax) != 0;
             }
+            if (far)
+#pragma unroll
+                for (int qq = 0; qq < QB; qq++)
+#pragma unroll
+                    for (int kb = 0; kb < 4; kb++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) sc[kb][qq][i] = product_less(sc[kb][qq][i], a.c, m[qq]);
         }
         if (odd) {
             // Rare: the values that are not finite go to the rows that see them by
@@ -384,14 +408,16 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
             // ---- weights, and O^T += V^T P^T: the second half's weights between the
             // first half's products
             vec pf[QB], vf[DB], vg[DB];
+            const float by = far ? 1.0f : a.c;
             auto weights = [&](int k2) __attribute__((always_inline)) {
 #pragma unroll
                 for (int qq = 0; qq < QB; qq++) {
                     pa_f32x4 x = sc[2 * k2][qq], y = sc[2 * k2 + 1][qq];
+                    const float less = far ? 0.f : -m[qq];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], a.c, -m[qq]));
-                        y[i] = __builtin_amdgcn_exp2f(fmaf(y[i], a.c, -m[qq]));
+                        x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], by, less));
+                        y[i] = __builtin_amdgcn_exp2f(fmaf(y[i], by, less));
                     }
                     const uint4 u = make_uint4(Mma<T>::pack(x[0], x[1]), Mma<T>::pack(x[2], x[3]),
                                                Mma<T>::pack(y[0], y[1]), Mma<T>::pack(y[2], y[3]));
@@ -403,6 +429,7 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
             for (int db = 0; db < DB; db++) vf[db] = __builtin_bit_cast(vec, *(const uint4 *)(vt + db * 128));
             weights(0);
             __builtin_amdgcn_sched_barrier(0);
+            if constexpr (KS == 1) __builtin_amdgcn_s_setprio(1);
             vec first[QB];
 #pragma unroll
             for (int qq = 0; qq < QB; qq++) first[qq] = pf[qq];
@@ -424,6 +451,7 @@ __device__ __forceinline__ void tile_part(const Plan &a, TileLds<D, KS> &s, int 
             for (int db = 0; db < DB; db++)
 #pragma unroll
                 for (int qq = 0; qq < QB; qq++) o[db][qq] = Mma<T>::mma(vg[db], pf[qq], o[db][qq]);
+            if constexpr (KS == 1) __builtin_amdgcn_s_setprio(0);
         }
         page = next;
         __builtin_amdgcn_s_waitcnt(0);
@@ -639,7 +667,7 @@ __device__ __forceinline__ void row_part(const Plan &a, RowLds<D> &s, int entry,
 #pragma unroll
         for (int kb = 0; kb < 4; kb++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) sc[kb][i] = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], a.c, -m));
+            for (int i = 0; i < 4; i++) sc[kb][i] = __builtin_amdgcn_exp2f(product_less(sc[kb][i], a.c, m));
 #pragma unroll
         for (int k2 = 0; k2 < 2; k2++) {
             const pa_f32x4 x = sc[2 * k2], y = sc[2 * k2 + 1];
@@ -916,7 +944,7 @@ Plan plan_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, const
     r.layer = a.layer;
     r.prefix = a.prefix;
     r.out_f16 = a.out_dtype == HYMT_F16;
-    r.c = std::max(std::abs(a.scale) * 1.4426950408889634f, 1e-30f);
+    r.c = std::max(std::abs(a.scale) * 1.4426950408889634f, std::numeric_limits<float>::denorm_min());
     r.flip = a.scale < 0 ? 0x80008000u : 0u;
     r.parts = s.parts;
     r.span = s.span;

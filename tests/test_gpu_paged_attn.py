@@ -162,6 +162,47 @@ def test_large_and_lopsided_scores(be, dt):
     run(be, c, slots, [0, 500], 2, q=q)
 
 
+@pytest.mark.parametrize("form", ["packed", "few_rows", "single", "shared"])
+@pytest.mark.parametrize("dt,qv,kv", [(N.BF16, 2.0 ** 60, -2.0 ** 62), (N.BF16, 2.0 ** 60, 2.0 ** 61), (N.BF16, 3.0, 2.0 ** 20),
+                                      (N.F16, 60000.0, 30000.0), (N.F16, 60000.0, -30000.0)])
+@pytest.mark.parametrize("scale", [None, 0.0])
+def test_scores_far_from_zero(be, form, dt, qv, kv, scale):
+    """Equal scores of up to +-2^126: every weight is 1 and the result the mean of
+    V, to the fp32 sums' (n + 8) 2^-24 of the mean of |v| and one rounding; and a position
+    that stands out by half a score takes all."""
+    lens = [300, 90] if form != "few_rows" else [3000, 90]
+    c, slots = held(11, lens, kv_heads=1, d=64, dt=dt)
+    c.k[:] = to_bits(np.full(1, kv / 8), dt)[0]
+    new = {"packed": lens, "few_rows": [20, 7], "single": [1, 1], "shared": [1, 1]}[form]
+    prefix = 64 if form == "shared" else 0 if form == "single" else None
+    if form == "shared":
+        c.refs[c.table[slots[0], 0]] += 1
+        c.table[slots[1], 0] = c.table[slots[0], 0]
+    q = np.full((sum(new), 2 * 64), qv / 8)
+    cu = None if prefix is not None else cu_of(new)
+    got = call(be, c, slots, cu, 2, q=q, scale=scale, prefix=prefix)[1]
+    got = from_bits(got, dt).astype(np.float64).reshape(-1, 2, 64)
+    u = 2.0 ** -11 if dt == N.F16 else 2.0 ** -8
+    r = 0
+    for s, n, length in zip(slots, new, lens):
+        v = c.rows(0, s, length)[1][0]
+        for j in range(n):
+            x = v[:length - n + 1 + j]
+            tol = (len(x) + 8) * 2.0 ** -24 * np.abs(x).mean(0) + u * np.abs(x.mean(0)) + 2.0 ** -25
+            assert (np.abs(got[r] - x.mean(0)) <= tol).all(), (r, j)
+            r += 1
+    if scale is None:
+        for s in slots:
+            c.k[0, c.table[s, 0], 0, c.ko[5]] = to_bits(np.full(1, kv / 8 * (1.5 if kv > 0 else 0.5)), dt)[0]
+        got = call(be, c, slots, cu, 2, q=q, prefix=prefix)[1].reshape(-1, 2, 64)
+        r = 0
+        for s, n, length in zip(slots, new, lens):
+            for j in range(n):
+                if length - n + j >= 5:
+                    assert (got[r] == c.v[0, c.table[s, 0], 0, c.vo[5]]).all(), (r, j)
+                r += 1
+
+
 def test_rows_have_the_same_bits_twice(be):
     c, slots = held(9, [700, 64, 1500], dt=N.F16)
     a = call(be, c, slots, cu_of([100, 64, 20]), 16)[1]
