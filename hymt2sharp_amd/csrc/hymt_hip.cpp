@@ -1678,6 +1678,7 @@ int hymt_rope_append(hymt_ctx *c, const hymt_paged *p, int layer, const hymt_bat
     if (misaligned(rope->freq, 8)) return fail(HYMT_E_ARG, "rope frequencies must be 8-byte aligned");
     if ((rope->interleaved != 0 && rope->interleaved != 1) || rope->reserved != 0)
         return fail(HYMT_E_ARG, "interleaved must be 0 or 1, reserved fields 0");
+    if (!std::isfinite(rope->scale)) return fail(HYMT_E_ARG, "rope scale must be finite");
     if ((int64_t)q_ld < (int64_t)heads * p->head_dim || kv_ld < p->kv_heads * p->head_dim || q_ld % 8 || kv_ld % 8)
         return fail(HYMT_E_ARG, "rows must be at least a row's values apart, by multiples of 8");
     if (!(eps >= 0.f)) return fail(HYMT_E_ARG, "eps must not be negative");

@@ -596,7 +596,7 @@ __device__ __forceinline__ bool entry_of_row(const hymt_batch &b, int r, RowEntr
     return false;
 }
 
-// A workgroup a row, for batches of few rows an entry.  q, k and v do not wait for the
+// A workgroup a row, for batches of few rows.  q, k and v do not wait for the
 // row's position, so they are loaded first.
 template <typename T, typename IO, int D>
 __global__ __launch_bounds__(256) void rope_row_kernel(hymt_paged p, hymt_batch b, RopeAppend a) {
@@ -663,7 +663,13 @@ __global__ __launch_bounds__(256) void rope_row_kernel(hymt_paged p, hymt_batch 
 // turn through LDS; row by row each chunk was written in 8 pieces, by
 // workgroups on 8 XCDs.
 constexpr int kRopeRows = 32;
-constexpr int kRopeFew = 8;  // fewer rows an entry than this: row by row
+// Row by row for batches of few rows, or of few an entry.  A row alone takes a round of
+// loads less than a block, whose workgroups first look for their entry and do 32 rows
+// in turn; blocks win once the chip has several rows a CU.  bf16 cache, 16 q heads,
+// fp32 rows, by rows and by blocks, us: one entry of 64 rows 4.9 and 11.7, of 1024 10.8
+// and 12.8, of 1536 15.0 and 13.5, of 2048 17.1 and 13.7; 256 entries of 12 25.5 and 26.3, of 16
+// 34.5 and 31.7; 128 of 12 15.8 and 15.4.
+constexpr int kRopeFew = 1536, kRopeFewEach = 14;
 
 template <typename T, typename IO, int D>
 __global__ __launch_bounds__(256) void rope_block_kernel(hymt_paged p, hymt_batch b, RopeAppend a) {
@@ -772,7 +778,7 @@ __global__ __launch_bounds__(256) void rope_block_kernel(hymt_paged p, hymt_batc
 template <typename T, typename IO>
 void launch_rope(const hymt_paged &p, const hymt_batch &b, const RopeAppend &a, hipStream_t s) {
     KernelSpan span("rope_append", s, true);
-    if (!b.cu || b.rows < kRopeFew * b.n) {
+    if (!b.cu || b.rows < kRopeFew || b.rows < kRopeFewEach * b.n) {
         if (p.head_dim == 64) launch(span, rope_row_kernel<T, IO, 64>, dim3(b.rows), dim3(256), 0, s, p, b, a);
         else launch(span, rope_row_kernel<T, IO, 128>, dim3(b.rows), dim3(256), 0, s, p, b, a);
         return;

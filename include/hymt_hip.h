@@ -467,7 +467,7 @@ int hymt_gemm_i8_swiglu(hymt_ctx *ctx, const int8_t *gate, const float *gate_sca
  * pages of hymt_kv_create have them).
  *
  * Position q of slot s is row q % 64 of page table[s * blocks + q / 64], for
- * q < len[s]; table entries past that are not read.  refs[p] is the number of table entries
+ * q < len[s]; table entries past that mean nothing.  refs[p] is the number of table entries
  * that hold page p; a page with none is free.  A sequence that ends inside a
  * page holds that page alone (fork and set_len see to it), so a position is
  * only ever written in a page of one sequence.
@@ -494,7 +494,7 @@ typedef struct hymt_paged {
     int32_t *len;      /* [seqs]                                                    */
     int32_t *refs;     /* [pages]                                                   */
     int32_t *work;     /* [HYMT_PAGED_WORK(pages)]                                  */
-    int32_t layers, pages;
+    int32_t layers, pages; /* up to 2^28 pages                                      */
     int32_t kv_heads;  /* 1 to 256                                                  */
     int32_t head_dim;  /* 64 or 128                                                 */
     int32_t dtype;     /* HYMT_F16 or HYMT_BF16                                     */
@@ -511,7 +511,8 @@ typedef struct hymt_batch {
     const int32_t *slots; /* device, [n]                                            */
     const int32_t *cu;    /* device, [n + 1], rising from 0, or NULL                */
     int32_t n;            /* entries, up to HYMT_PAGED_BATCH                        */
-    int32_t rows;         /* rows of the packed tensors, cu[n] at least (NULL: n)   */
+    int32_t rows;         /* rows of the packed tensors, cu[n] at least (NULL: n); up to
+                             2^22, and 2^30 times the q heads                       */
     int32_t max_len;      /* about the longest len, 0 if unknown: how the work is split
                              goes by it, and no result but for its rounding         */
     int32_t reserved;     /* 0                                                      */
@@ -544,7 +545,7 @@ typedef struct hymt_rope {
     const double *freq;  /* device, [dim / 2]; NULL with dim 0                      */
     int32_t dim;         /* a multiple of 16, 0 to head_dim                         */
     int32_t interleaved; /* 0 or 1                                                  */
-    float scale;
+    float scale;         /* finite                                                  */
     int32_t reserved;    /* 0                                                       */
 } hymt_rope;
 
@@ -567,8 +568,8 @@ int hymt_rope_freqs(int dim, double base, int scaling, double factor, int traine
  * kv_heads * D elements apart (both multiples of 8); q, k, v, q_out, qnw and knw
  * [D] (fp32, NULL for none) 16-byte aligned.  heads is a multiple of kv_heads, up to 64
  * times.  A slot stands once in the batch (else which of its rows is stored is
- * open).  Pages for the positions are there already (hymt_paged_extend).  The
- * counterpart of what hymt_attn_prefill does before its products. */
+ * open), and q_out overlaps none of the others.  Pages for the positions are there
+ * already (hymt_paged_extend).  The counterpart of what hymt_attn_prefill does before its products. */
 int hymt_rope_append(hymt_ctx *ctx, const hymt_paged *cache, int layer, const hymt_batch *batch, const void *q,
                      int q_ld, const void *k, const void *v, int kv_ld, int io_dtype, int heads,
                      const hymt_rope *rope, const float *qnw, const float *knw, float eps, void *q_out);
@@ -577,9 +578,10 @@ int hymt_rope_append(hymt_ctx *ctx, const hymt_paged *cache, int layer, const hy
  * own, of the cache's layer `layer` (q [rows][heads * D] in the cache's type, as
  * hymt_rope_append leaves it; kv head h serves heads / kv_heads heads in turn).
  * out is HYMT_F16 or HYMT_BF16 [rows][heads * D].  A row without positions gives 0; what stands in the
- * pages where a row does not attend, infinities and NaN too, does not reach it.
+ * pages where a row does not attend, infinities and NaN too, does not reach it (where
+ * it does attend they make its result infinite or NaN).
  * Softmax and sums in fp32, its weights rounded to the cache's type for the
- * products with V.  q and out 16-byte aligned. */
+ * products with V.  q and out 16-byte aligned; out may be q, else they do not overlap. */
 int hymt_attn_packed(hymt_ctx *ctx, const hymt_paged *cache, int layer, const hymt_batch *batch, const void *q,
                      int heads, float scale, void *out, int out_dtype);
 

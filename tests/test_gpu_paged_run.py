@@ -10,7 +10,7 @@ import pytest
 from hymt2sharp_amd import HipBackend, Rope, rope_freqs
 from hymt2sharp_amd import _native as N
 from tests.i8_cases import Room
-from tests.paged_cases import PAGE, TINY, U, Cache, attention, batch, check_rows, from_bits, rotated, to_bits
+from tests.paged_cases import PAGE, TINY, U, Cache, attention, batch, blocks_of, check_rows, from_bits, rotated, to_bits
 from tests.test_gpu_paged_pages import Model, equal, ints, offsets_of
 
 pytestmark = pytest.mark.gpu
@@ -200,6 +200,74 @@ def test_a_recording_that_would_have_to_grow(be):
     finally:
         room.close()
         fresh.Dispose()
+
+
+def test_a_recording_whose_workspace_was_replaced(be):
+    """Two recordings share the workspace and give the eager bits in any order; once
+    an eager call has made it grow, they are refused."""
+    fresh = HipBackend(0)
+    room = Room(fresh)
+    try:
+        c = Cache(1, pages=300, kv_heads=1, d=D, seqs=3, blocks=200)
+        c.give(0, 3000)
+        c.give(1, 12000)
+        dev = c.put(room)
+        rng = np.random.default_rng(0)
+        q = room.put(to_bits(rng.standard_normal((40, 2 * D)), N.BF16))
+        zero = np.zeros((40, 2 * D), np.uint16)
+        outs = [room.put(zero) for _ in range(4)]
+        one = batch(room, [0], max_len=3000)
+        rows = batch(room, [0], [0, 40], max_len=3000)
+        calls = [lambda o: fresh.attn_shared(dev, 0, one, 0, q, 2, o), lambda o: fresh.attn_packed(dev, 0, rows, q, 2, o)]
+        for f, o in zip(calls, outs):
+            f(o)
+        graphs = []
+        for f, o in zip(calls, outs[2:]):
+            fresh.graph_begin()
+            f(o)
+            graphs.append(fresh.graph_end())
+        for order in ([0, 1, 0], [1, 1, 0], [0, 1]):
+            for o in outs[2:]:
+                fresh.upload(o, zero)
+            for k in order:
+                fresh.graph_launch(graphs[k])
+            fresh.sync()
+            for k in range(2):
+                np.testing.assert_array_equal(room.get(outs[2 + k], zero), room.get(outs[k], zero))
+        fresh.attn_packed(dev, 0, batch(room, [0, 1], [0, 1, 40], max_len=12000), q, 2, outs[0])
+        for g in graphs:
+            with pytest.raises(N.InvalidOperationError):
+                fresh.graph_launch(g)
+            fresh.graph_destroy(g)
+    finally:
+        room.close()
+        fresh.Dispose()
+
+
+@pytest.mark.parametrize("new,lens,prefix", [([70, 3], [300, 900], None), ([2000], [2000], None), ([5] * 3, [4000] * 3, None),
+                                             ([1] * 5, [100, 1, 64, 700, 9], 0), ([1] * 2, [3000, 5000], 0),
+                                             ([1] * 40, [700] * 40, 640)])
+def test_out_may_be_q(be, new, lens, prefix):
+    room = Room(be)
+    hkv, group = 2, 20 if prefix == 0 else 3
+    c = Cache(3, pages=sum(blocks_of(n) for n in lens), kv_heads=hkv, d=D, dt=N.F16, seqs=len(lens), blocks=100)
+    for i, n in enumerate(lens):
+        c.give(i, n)
+    if prefix:
+        c.table[:, :prefix // PAGE] = c.table[0, :prefix // PAGE]
+    dev = c.put(room)
+    cu = None if prefix is not None else np.concatenate([[0], np.cumsum(new)])
+    b = batch(room, range(len(lens)), cu, max_len=max(lens))
+    bits = to_bits(np.random.default_rng(1).standard_normal((sum(new), hkv * group * D)), N.F16)
+    q, x, out = room.put(bits), room.put(bits), room.put(np.zeros_like(bits))
+    for source, to in ((q, out), (x, x)):
+        if prefix is None:
+            be.attn_packed(dev, 0, b, source, hkv * group, to)
+        else:
+            be.attn_shared(dev, 0, b, prefix, source, hkv * group, to)
+    np.testing.assert_array_equal(room.get(x, bits), room.get(out, bits))
+    np.testing.assert_array_equal(room.get(q, bits), bits)
+    room.close()
 
 
 def test_kernels_are_timed(be):

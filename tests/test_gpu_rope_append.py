@@ -115,15 +115,18 @@ def held(seed, new, lens, **kw):
     return c, slots, [0] + np.cumsum(new).tolist()
 
 
+# rows behind the last entry's: few, and so many that the batch goes by blocks of positions
+PADS = [3, 1600]
 LENGTHS = [([1], [1]), ([5, 0, 1, 64], [5, 0, 1, 64]), ([33, 2, 63], [40, 66, 127]), ([130, 1, 31], [200, 65, 64]),
            ([200], [263])]
 
 
 @pytest.mark.parametrize("new,lens", LENGTHS)
 @pytest.mark.parametrize("d,hkv,group", [(128, 4, 4), (64, 3, 1), (128, 1, 7), (64, 2, 16)])
-def test_lengths_and_heads(be, new, lens, d, hkv, group):
+@pytest.mark.parametrize("pad", PADS)
+def test_lengths_and_heads(be, new, lens, d, hkv, group, pad):
     c, slots, cu = held(len(new) * 7 + d, new, lens, d=d, kv_heads=hkv, layers=2)
-    run(be, c, slots, cu, hkv * group, pad=3, layer=1)
+    run(be, c, slots, cu, hkv * group, pad=pad, layer=1)
 
 
 @pytest.mark.parametrize("n", [1, 3, 64, 65, 200])
@@ -138,23 +141,34 @@ def test_one_row_each(be, n, d, dt):
 @pytest.mark.parametrize("dt", [N.F16, N.BF16])
 @pytest.mark.parametrize("fused", [True, False])
 def test_types_and_strides(be, io, dt, fused):
-    c, slots, cu = held(3, [40, 70], [100, 70], dt=dt)
-    run(be, c, slots, cu, 6, io=io, fused=fused)
+    c, slots, cu = held(3, [40, 70], [100, 70], dt=dt, kv_heads=2)
+    for pad in PADS:
+        run(be, c, slots, cu, 6, io=io, fused=fused, pad=pad)
     run(be, c, slots, None, 6, io=io, fused=fused)
 
 
 @pytest.mark.parametrize("d,dim", [(128, x) for x in (0, 16, 32, 48, 64, 96, 112, 128)] + [(64, x) for x in (0, 16, 48, 64)])
 @pytest.mark.parametrize("interleaved", [0, 1])
-def test_rotated_part(be, d, dim, interleaved):
+@pytest.mark.parametrize("pad", PADS)
+def test_rotated_part(be, d, dim, interleaved, pad):
     c, slots, cu = held(dim, [50, 9], [77, 9], d=d, dt=N.F16)
-    run(be, c, slots, cu, 4, dim=dim, interleaved=interleaved)
+    run(be, c, slots, cu, 4, dim=dim, interleaved=interleaved, pad=pad)
 
 
 @pytest.mark.parametrize("scaling", [N.ROPE_LINEAR, N.ROPE_NTK, N.ROPE_YARN])
 @pytest.mark.parametrize("norm", [(True, False), (False, True), (False, False)])
-def test_scalings_and_norms(be, scaling, norm):
+@pytest.mark.parametrize("pad", PADS)
+def test_scalings_and_norms(be, scaling, norm, pad):
     c, slots, cu = held(9, [20, 3], [50, 300], dt=N.F16)
-    run(be, c, slots, cu, 4, scaling=scaling, norm=norm)
+    run(be, c, slots, cu, 4, scaling=scaling, norm=norm, pad=pad)
+
+
+@pytest.mark.parametrize("n,rows", [(1, 1535), (1, 1536), (3, 800), (120, 13), (120, 14), (120, 15)])
+def test_many_rows(be, n, rows):
+    """Both sides of where a batch goes by blocks, entries at every offset in a page."""
+    new = [max(rows + (i % 3 - 1) * (n > 2), 0) for i in range(n)]
+    c, slots, cu = held(n + rows, new, [x + 7 * i % 130 for i, x in enumerate(new)], kv_heads=1, d=64)
+    run(be, c, slots, cu, 2)
 
 
 def test_far_positions(be):
@@ -177,8 +191,10 @@ def test_rows_of_zeros_infinities_and_nan(be):
     x[6, 5] = np.nan
     x[9, 6, 3] = np.inf
     x[10, 7, 100] = -np.inf
-    run(be, c, slots, cu, 4, x=x, norm=(False, False), dim=0)
-    run(be, c, slots, cu, 4, x=np.where(np.isinf(x), np.nan, x))
+    for more in (0, 1600):
+        wide = np.concatenate([x, np.zeros((more, 8, 128), np.float32)])
+        run(be, c, slots, cu, 4, x=wide, norm=(False, False), dim=0, pad=more)
+        run(be, c, slots, cu, 4, x=np.where(np.isinf(wide), np.nan, wide), pad=more)
 
 
 def test_slots_and_pages_that_are_not_there(be):
@@ -188,13 +204,15 @@ def test_slots_and_pages_that_are_not_there(be):
     c.table[slots[1], 0] = -1
     c.table[slots[0], 1] = c.pages
     c.len[slots[2]] = 2  # two of its four rows stand before position 0
-    run(be, c, slots + [-1, 5, 1 << 30], cu + [cu[-1] + 2, cu[-1] + 3, cu[-1] + 3], 4, norm=(True, True))
+    for pad in PADS:
+        run(be, c, slots + [-1, 5, 1 << 30], cu + [cu[-1] + 2, cu[-1] + 3, cu[-1] + 3], 4, pad=pad)
 
 
 def test_nothing_to_do(be):
     c, slots, cu = held(6, [0, 0], [10, 0])
     run(be, c, slots, cu, 4)
     run(be, c, slots, cu, 4, pad=5)
+    run(be, c, slots, cu, 4, pad=1600)
 
 
 def test_a_row_has_the_same_bits_in_every_batch(be):
@@ -206,5 +224,10 @@ def test_a_row_has_the_same_bits_in_every_batch(be):
     np.testing.assert_array_equal(q0, q1)
     np.testing.assert_array_equal(k0, k1)
     np.testing.assert_array_equal(v0, v1)
+    wide = np.concatenate([x, np.zeros((1600, 12, 128), np.float32)])
+    q3, k3, v3 = run(be, c, slots, cu, 8, x=wide, pad=1600)
+    np.testing.assert_array_equal(q0, q3[:3])
+    np.testing.assert_array_equal(k0, k3)
+    np.testing.assert_array_equal(v0, v3)
     q2, _, _ = run(be, c, slots[1:2], None, 8, x=x[1:2])
     np.testing.assert_array_equal(q2[0], q0[1])

@@ -131,6 +131,12 @@ def test_batches(ctx, f):
     else:
         assert f(*ctx, b=batch(rows=(1 << 24) + 1)) == N.HYMT_E_UNSUPPORTED
         assert f(*ctx, b=batch(rows=0)) == N.HYMT_E_NO_DEVICE
+        assert f(*ctx, b=batch(rows=1 << 22)) == N.HYMT_E_NO_DEVICE
+        assert f(*ctx, b=batch(rows=(1 << 22) + 1)) == N.HYMT_E_UNSUPPORTED
+        wide = dict(q_ld=1 << 16) if f is append else {}
+        assert f(*ctx, b=batch(rows=1 << 22), heads=256, **wide) == N.HYMT_E_NO_DEVICE  # 2^30 rows of all heads
+        eight = dict(c=cache(kv_heads=8), **(dict(q_ld=1 << 16, kv_ld=1 << 12) if f is append else {}))
+        assert f(*ctx, b=batch(rows=1 << 22), heads=264, **eight) == N.HYMT_E_UNSUPPORTED
 
 
 @pytest.mark.parametrize("f", ROWS)
@@ -147,7 +153,8 @@ def test_append(ctx):
     for bad in (dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(r=None), dict(q=OK + 8), dict(k=OK + 8),
                 dict(v=OK + 4), dict(out=OK + 8), dict(qnw=OK + 4), dict(knw=OK + 8), dict(q_ld=2040), dict(q_ld=2052),
                 dict(kv_ld=504), dict(kv_ld=516), dict(eps=-1.0), dict(eps=float("nan")), dict(r=rope(freq=None)),
-                dict(r=rope(freq=OK + 4)), dict(r=rope(interleaved=2)), dict(r=rope(reserved=1))):
+                dict(r=rope(freq=OK + 4)), dict(r=rope(interleaved=2)), dict(r=rope(reserved=1)),
+                dict(r=rope(scale=float("nan"))), dict(r=rope(scale=float("inf")))):
         assert append(*ctx, **bad) == N.HYMT_E_ARG, bad
     for bad in (dict(io=3), dict(io=-1), dict(r=rope(dim=8)), dict(r=rope(dim=144)), dict(r=rope(dim=-16)),
                 dict(c=cache(head_dim=64), r=rope(dim=80))):
