@@ -522,6 +522,43 @@ struct Tile {
 template <bool SPLIT> __device__ __forceinline__ bool find_tile(const Plan &a, int w, Tile &out) {
     const int lane = threadIdx.x & 63;
     int before = 0;
+    if (!SPLIT && !a.b.cu) {  // a tile an entry
+        if (w >= a.b.n) return false;
+        const int slot = a.b.slots[w];
+        out = {0, slot, slot_len(a.p, slot), {w, 1}};
+        return true;
+    }
+    if (!SPLIT && a.b.n > 64) {
+        // 256 entries in a round trip, and the length after the search (256 prompts of 30
+        // rows 33.2 -> 30.0 us, 1024 of 8 rows 121 -> 85)
+        constexpr int C = 4;
+        for (int base = 0; base < a.b.n; base += 64 * C) {
+            Span sp[C];
+            int slot[C];
+#pragma unroll
+            for (int j = 0; j < C; j++) {
+                const int i = min(base + 64 * j + lane, a.b.n);  // past the end: no rows
+                const int lo = max(0, min(a.b.cu[i], a.b.rows)), hi = min(a.b.cu[min(i + 1, a.b.n)], a.b.rows);
+                sp[j] = {lo, max(lo, hi) - lo};
+                slot[j] = a.b.slots[min(i, a.b.n - 1)];
+            }
+#pragma unroll
+            for (int j = 0; j < C; j++) {
+                const int tiles = (sp[j].n * a.group + a.tile_rows - 1) / a.tile_rows, x = wave_sums(tiles);
+                const uint64_t hit = __ballot(w < before + x);
+                if (hit) {
+                    const int at = __ffsll((unsigned long long)hit) - 1;
+                    out.index = before + __builtin_amdgcn_readlane(x, at) - 1 - w;
+                    out.slot = __builtin_amdgcn_readlane(slot[j], at);
+                    out.len = slot_len(a.p, out.slot);
+                    out.span = {__builtin_amdgcn_readlane(sp[j].first, at), __builtin_amdgcn_readlane(sp[j].n, at)};
+                    return true;
+                }
+                before += __builtin_amdgcn_readlane(x, 63);
+            }
+        }
+        return false;
+    }
     for (int base = 0; base < a.b.n; base += 64) {
         const int i = base + lane;
         Span sp{0, 0};

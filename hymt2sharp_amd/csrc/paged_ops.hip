@@ -576,24 +576,27 @@ __device__ __forceinline__ int slot_length(const hymt_paged &p, int slot) {
     return (unsigned)slot < (unsigned)p.seqs ? max(0, min(p.len[slot], 1 << 30)) : 0;
 }
 
-// The entry of row r, its slot and its rows from r on.  Lanes look at 64 entries
-// at a time, end and slot in one round trip.
+// The entry of row r (the first that ends behind it), its slot and its rows from r on.
+// Lanes look at 64 runs of entries, then at the run's, in two round trips at most.
 struct RowEntry {
     int slot, behind;
 };
 __device__ __forceinline__ bool entry_of_row(const hymt_batch &b, int r, RowEntry &out) {
-    const int lane = threadIdx.x & 63;
-    for (int base = 0; base < b.n; base += 64) {
-        const int i = min(base + lane, b.n - 1);
-        const int end = b.cu[i + 1], slot = b.slots[i];
-        const uint64_t hit = __ballot(base + lane < b.n && end > r);
-        if (hit) {
-            const int k = __ffsll((unsigned long long)hit) - 1;
-            out = {__builtin_amdgcn_readlane(slot, k), __builtin_amdgcn_readlane(end, k) - r};
-            return true;
-        }
+    static_assert(HYMT_PAGED_BATCH <= 64 * 64, "two steps");
+    const int lane = threadIdx.x & 63, run = (b.n + 63) / 64;
+    int first = 0;
+    if (run > 1) {
+        const uint64_t hit = __ballot(lane * run < b.n && b.cu[min((lane + 1) * run, b.n)] > r);
+        if (!hit) return false;
+        first = (__ffsll((unsigned long long)hit) - 1) * run;
     }
-    return false;
+    const int i = min(first + lane, b.n - 1);
+    const int end = b.cu[i + 1], slot = b.slots[i];
+    const uint64_t hit = __ballot(first + lane < b.n && end > r);
+    if (!hit) return false;
+    const int k = __ffsll((unsigned long long)hit) - 1;
+    out = {__builtin_amdgcn_readlane(slot, k), __builtin_amdgcn_readlane(end, k) - r};
+    return true;
 }
 
 // A workgroup a row, for batches of few rows.  q, k and v do not wait for the

@@ -112,6 +112,24 @@ def test_packed_many_entries(be):
     run(be, c, slots, cu_of(new), 4, pad=2)
 
 
+@pytest.mark.parametrize("n", [1, 64, 65, 300])
+@pytest.mark.parametrize("group", [3, 64])
+def test_packed_single_rows_without_offsets(be, n, group):
+    lens = np.random.default_rng(n).integers(0, 200, n).tolist()
+    c, slots = held(n, lens, kv_heads=1, d=64, dt=N.F16)
+    run(be, c, slots, None, group)
+
+
+@pytest.mark.parametrize("n", [300, 1024])
+def test_packed_hundreds_of_prompts(be, n):
+    rng = np.random.default_rng(n)
+    new = rng.integers(0, 40, n) * (rng.random(n) < 0.3)
+    new[[0, n - 1]] = 0, 33
+    lens = (new + rng.integers(0, 70, n)).tolist()
+    c, slots = held(5, lens, kv_heads=2, d=64)
+    run(be, c, slots, cu_of(new), 10, pad=2)
+
+
 def test_rows_without_positions(be):
     """Unknown slots, rows before position 0 and empty slots: zeros."""
     c, slots = held(6, [40, 10], seqs=4)

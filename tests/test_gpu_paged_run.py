@@ -270,6 +270,47 @@ def test_out_may_be_q(be, new, lens, prefix):
     room.close()
 
 
+@pytest.mark.parametrize("n", [5, 64, 65, 300, 1024])
+def test_offsets_and_slots_that_mean_nothing(be, n):
+    """Whatever slots, cu, table and len hold, nothing outside the buffers is written
+    (Room.close checks their surroundings) and the calls end; the cache's lists are
+    read only."""
+    rng = np.random.default_rng(n)
+    rows, heads, hkv, d = 700, 4, 2, 64
+    for kind in ("random", "alternating", "near"):
+        c = Cache(n, pages=40, kv_heads=hkv, d=d, dt=N.F16, seqs=9, blocks=5)
+        c.table[:] = rng.integers(-3, 45, c.table.shape)
+        c.len[:] = rng.integers(-50, 400, c.len.shape)
+        c.table[0, 0], c.len[1], c.len[2] = 2 ** 31 - 1, 2 ** 31 - 1, -2 ** 31
+        cu = {"random": rng.integers(-2 ** 31, 2 ** 31, n + 1), "alternating": np.arange(n + 1) % 2 * rows,
+              "near": rng.integers(-5, rows + 5, n + 1)}[kind]
+        slots = rng.integers(-2, 12, n)
+        slots[0] = 2 ** 31 - 1
+        room = Room(be)
+        dev = c.put(room)
+        b = batch(room, slots, cu, rows=rows, max_len=300)
+        x = room.put(rng.standard_normal((rows, heads + 2 * hkv, d)).astype(np.float32))
+        freq, scale = rope_freqs(d)
+        rope = Rope(freq=room.put(freq), dim=d, interleaved=0, scale=scale)
+        q = room.put(to_bits(rng.standard_normal((max(rows, n), heads * d)), N.F16))
+        out = room.put(np.zeros((max(rows, n), heads * d), np.uint16))
+        wide = (heads + 2 * hkv) * d
+        be.attn_packed(dev, 0, b, q, heads, out)
+        for prefix in (0, 128):
+            be.attn_shared(dev, 0, batch(room, slots), prefix, q, heads, out)
+        for more in (0, 1):  # row by row and by blocks
+            if more:
+                x = room.put(rng.standard_normal((16 * max(n, 100), wide)).astype(np.float32))
+                q = room.put(np.zeros((16 * max(n, 100), heads * d), np.uint16))
+                b = batch(room, slots, cu, rows=16 * max(n, 100))
+            be.rope_append(dev, 0, b, x, wide, x + 4 * heads * d, x + 4 * (heads + hkv) * d, wide, N.F32, heads, rope, None,
+                           None, EPS, q)
+        be.sync()
+        for name, got in zip(("table", "len", "refs"), c.get(room, dev, "table", "len", "refs")):
+            np.testing.assert_array_equal(got, getattr(c, name), err_msg=name)
+        room.close()
+
+
 def test_kernels_are_timed(be):
     room = Room(be)
     c = Cache(1, pages=60, kv_heads=1, d=D, seqs=2, blocks=60)
