@@ -1563,7 +1563,8 @@ int check_heads(const hymt_paged *p, const hymt_batch *b, int layer, int heads) 
     if (layer < 0 || layer >= p->layers) return fail(HYMT_E_ARG, "layer outside the cache");
     if (heads < 1 || heads % p->kv_heads != 0) return fail(HYMT_E_ARG, "heads must be a multiple of kv_heads");
     if (heads / p->kv_heads > kPagedMaxGroup) return fail(HYMT_E_UNSUPPORTED, "more than 64 heads per kv head");
-    if ((int64_t)b->rows * heads > 1 << 30) return fail(HYMT_E_UNSUPPORTED, "more than 2^30 rows of all heads");
+    // the grids' threads stay below 2^32
+    if ((int64_t)b->rows * heads > 1 << 28) return fail(HYMT_E_UNSUPPORTED, "more than 2^28 rows of all heads");
     return HYMT_OK;
 }
 

@@ -512,7 +512,7 @@ typedef struct hymt_batch {
     const int32_t *cu;    /* device, [n + 1], rising from 0, or NULL                */
     int32_t n;            /* entries, up to HYMT_PAGED_BATCH                        */
     int32_t rows;         /* rows of the packed tensors, cu[n] at least (NULL: n); up to
-                             2^22, and 2^30 times the q heads                       */
+                             2^22, and 2^28 times the q heads                       */
     int32_t max_len;      /* about the longest len, 0 if unknown: how the work is split
                              goes by it, and no result but for its rounding         */
     int32_t reserved;     /* 0                                                      */

@@ -1,8 +1,6 @@
 """Inputs and plain references of the multi-sequence cache's operators
 (hymt_paged_*, hymt_rope_append, hymt_attn_packed, hymt_attn_shared): numpy, in 64
 bits, from the definitions in include/hymt_hip.h."""
-import ctypes
-
 import numpy as np
 
 from hymt2sharp_amd import _native as N
@@ -207,11 +205,3 @@ def rotated(x, pos, freq, scale, dim, interleaved, w, eps):
         y = y * root * w
         err = err * root * np.abs(w) + np.abs(y) * ((d + 16) * U32 + rel)
     return y, err + np.abs(y) * 2 * U32
-
-
-def make_room(be):
-    return Room(be)
-
-
-def pointer(s):
-    return ctypes.byref(s)

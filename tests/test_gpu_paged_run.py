@@ -311,6 +311,63 @@ def test_offsets_and_slots_that_mean_nothing(be, n):
         room.close()
 
 
+def test_the_most_rows(be):
+    """2^22 rows in 1024 sequences of 4096 through the append and the attention: byte
+    offsets past 2^31, rows looked at where blocks, tiles and sequences meet."""
+    n, length, heads, hkv, d = 1024, 4096, 4, 1, 64
+    rows, wide, some = n * length, (heads + 2 * hkv) * d, 4096 - 7
+    rng = np.random.default_rng(0)
+    x = to_bits(rng.standard_normal((some, wide)), N.F16)  # row r of the batch is x[r % some]
+    room = Room(be)
+    c = be.paged_create(1, n * length // PAGE, n, length // PAGE, kv_heads=hkv, head_dim=d, dtype=N.F16)
+    qkv, q = be.alloc(rows * wide * 2), be.alloc(rows * heads * d * 2)
+    try:
+        for r in range(0, rows, some):
+            part = x[:min(some, rows - r)]
+            be.upload(qkv + r * wide * 2, part)
+        slots = rng.permutation(n).astype(np.int32)
+        d_slots, cu = ints(room, slots), ints(room, np.arange(n + 1) * length)
+        b = N.SeqBatch(slots=d_slots, cu=cu, n=n, rows=rows, max_len=length)
+        freq, scale = rope_freqs(d)
+        rope = Rope(freq=room.put(freq), dim=d, interleaved=0, scale=scale)
+        be.paged_extend(c, d_slots, n, cu=cu)
+        be.rope_append(c, 0, b, qkv, wide, qkv + heads * d * 2, qkv + (heads + hkv) * d * 2, wide, N.F16, heads, rope, None,
+                       None, EPS, q)
+        got_q = {}
+        entries = {0: [0, 1, 4095], 1: [0, 31], 511: [2047, 2048], 1022: [4064], 1023: [4063, 4064, 4095]}
+        for e, some_rows in entries.items():
+            for i in some_rows:
+                r = e * length + i
+                got_q[r] = be.download(np.empty(heads * d, np.uint16), q + r * heads * d * 2)
+                y, err = rotated(from_bits(x[r % some], N.F16)[None, :heads * d].reshape(1, heads, d), np.array([i]), freq,
+                                 scale, d, 0, None, EPS)
+                near = np.abs(from_bits(got_q[r], N.F16) - y.reshape(-1))
+                assert (near <= U[N.F16] * np.abs(y.reshape(-1)) + err.reshape(-1) * 1.001 + TINY[N.F16]).all(), r
+        be.attn_packed(c, 0, b, q, heads, q)  # in place
+        assert be.paged_work(c)["first"] == 0
+        table = be.download(np.empty((n, length // PAGE), np.int32), c.table)
+        one = Cache(0, pages=length // PAGE, kv_heads=hkv, d=d, dt=N.F16, seqs=1, blocks=length // PAGE)
+        one.len[0], one.table[0] = length, np.arange(length // PAGE)
+        for e, some_rows in entries.items():
+            for k, page in enumerate(table[slots[e]]):
+                for pool, to in ((c.k, one.k), (c.v, one.v)):
+                    to[0, k, 0] = be.download(np.empty(PAGE * d, np.uint16), pool + int(page) * PAGE * d * 2)
+            v = one.rows(0, 0, length)[1][0]
+            np.testing.assert_array_equal(v, from_bits(x[(e * length + np.arange(length)) % some], N.F16)[:, -d:])
+            for i in some_rows:
+                r = e * length + i
+                one.len[0] = i + 1  # the row as a sequence's last
+                want, tol, done = attention(one, 0, [0], None, from_bits(got_q[r], N.F16)[None], heads)
+                got = be.download(np.empty((1, heads * d), np.uint16), q + r * heads * d * 2)
+                check_rows(got, want, tol, done, got, N.F16)
+            one.len[0] = length
+    finally:
+        be.free(qkv)
+        be.free(q)
+        be.paged_free(c)
+        room.close()
+
+
 def test_kernels_are_timed(be):
     room = Room(be)
     c = Cache(1, pages=60, kv_heads=1, d=D, seqs=2, blocks=60)

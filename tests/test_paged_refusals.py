@@ -134,9 +134,8 @@ def test_batches(ctx, f):
         assert f(*ctx, b=batch(rows=1 << 22)) == N.HYMT_E_NO_DEVICE
         assert f(*ctx, b=batch(rows=(1 << 22) + 1)) == N.HYMT_E_UNSUPPORTED
         wide = dict(q_ld=1 << 16) if f is append else {}
-        assert f(*ctx, b=batch(rows=1 << 22), heads=256, **wide) == N.HYMT_E_NO_DEVICE  # 2^30 rows of all heads
-        eight = dict(c=cache(kv_heads=8), **(dict(q_ld=1 << 16, kv_ld=1 << 12) if f is append else {}))
-        assert f(*ctx, b=batch(rows=1 << 22), heads=264, **eight) == N.HYMT_E_UNSUPPORTED
+        assert f(*ctx, b=batch(rows=1 << 22), heads=64, **wide) == N.HYMT_E_NO_DEVICE  # 2^28 rows of all heads
+        assert f(*ctx, b=batch(rows=1 << 22), heads=68, **wide) == N.HYMT_E_UNSUPPORTED
 
 
 @pytest.mark.parametrize("f", ROWS)
