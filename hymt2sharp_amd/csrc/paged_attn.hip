@@ -125,7 +125,7 @@ struct Plan {
     int own_parts, own_span;  // shared: the same of an entry's own range
     int tiles;        // tiles of one kv head, at most
     int tile_rows;    // 64 or 128
-    int direct;       // shared: no prefix and no split, the row part writes the output
+    int direct;       // shared: no tiles and no split, the row part writes the output
     float *o, *ml;    // partials: [part][rows * heads][D], [part][rows * heads][2]
 };
 
@@ -626,11 +626,18 @@ template <int D> struct RowLds {
     float m[4][16], l[4][16];
 };
 
+// Page t of an entry that reads the first `common` of them from another slot's table.
+struct RowPages {
+    Ids first, own;
+    int common;
+    __device__ __forceinline__ int page(const hymt_paged &p, int t) { return t < common ? first.page(p, t) : own.page(p, t); }
+};
+
 // Up to 16 rows (heads g0 ..) of one entry over pages [t0, t1) of its slot, a page to
 // a wave: K and V go from memory into operand registers, those of the wave's next
 // page as soon as the products have read these.
 template <typename T, int D>
-__device__ __forceinline__ void row_part(const Plan &a, RowLds<D> &s, int entry, int h, int g0, Ids ids, int len, int t0,
+__device__ __forceinline__ void row_part(const Plan &a, RowLds<D> &s, int entry, int h, int g0, RowPages ids, int len, int t0,
                                          int t1, int part, bool partial) {
     typedef typename Mma<T>::vec vec;
     constexpr int DS = D / 32, DB = D / 16;
@@ -769,7 +776,8 @@ __device__ __forceinline__ int common_of(const Plan &a) {
     return a.prefix ? min(a.prefix, slot_len(a.p, a.b.slots[0]) / kPage * kPage) : 0;
 }
 
-// Workgroups [0, tile_wgs) the prefix, the others the entries' own positions.
+// Workgroups [0, tile_wgs) the prefix, the others the entries' own positions (tile_wgs
+// 0: all of them).
 template <typename T, int D, int QB> __global__ __launch_bounds__(256, 2) void attn_shared_kernel(Plan a, int tile_wgs) {
     __shared__ __attribute__((aligned(256))) union {
         TileLds<D, 1> tile;
@@ -794,9 +802,11 @@ template <typename T, int D, int QB> __global__ __launch_bounds__(256, 2) void a
     const int g0 = w % blocks16 * 16;
     w /= blocks16;
     const int part = w % a.own_parts, entry = w / a.own_parts, slot = a.b.slots[entry];
-    const Ids ids = ids_of(a.p, slot, pages_expected);
+    RowPages ids{ids_of(a.p, slot0, 0), ids_of(a.p, slot, pages_expected), 0};
     const int common = common_of(a), len = slot_len(a.p, slot);
-    const int first = common / kPage, pages = max(0, pages_of(len) - first),
+    ids.common = common / kPage;
+    // without tiles the rows see to the prefix too
+    const int first = tile_wgs ? ids.common : 0, pages = max(0, pages_of(len) - first),
               parts = parts_of(pages, a.own_span, a.own_parts);
     if (part >= parts) return;
     row_part<T, D>(a, s.row, entry, h, g0, ids, len, first + (int)((long)part * pages / parts),
@@ -941,6 +951,15 @@ Shape shape_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, boo
         if ((long)ceil_div((long)b.n * group, 64) * p.kv_heads * common <= 8 * kCus) s.rows = 64;
         s.tiles = a.prefix ? ceil_div((long)b.n * group, s.rows) : 0;
         const long rows = (long)b.n * p.kv_heads * s.blocks16;
+        // Short sequences, and not too many rows: each row by itself through the prefix too, in one
+        // launch without a join.  With tiles and without, us: 8 rows behind 512 positions and 64
+        // of their own 8.7 and 6.8, 64 rows 12.8 and 8.1, 256 rows 21.2 and 19.0; behind 1024 8
+        // rows 10.6 and 9.2, 128 18.0 and 15.9, 256 21.6 and 27.3; behind 1536 8 rows 10.3 and 11.4.
+        if (s.tiles && pages <= 20 && rows * pages <= 40 * kCus) {
+            s.tiles = 0;
+            s.own_span = pages;
+            return s;
+        }
         // One tile a CU, beside it the rows: at 256 rows behind 16384 positions 75 us
         // (tiles in both places first, rows after them, 94).  Short parts, as
         // the join is launched anyway, yet not one page each of a longer prefix,

@@ -180,7 +180,7 @@ def test_large_and_lopsided_scores(be, dt):
     run(be, c, slots, [0, 500], 2, q=q)
 
 
-@pytest.mark.parametrize("form", ["packed", "few_rows", "single", "shared"])
+@pytest.mark.parametrize("form", ["packed", "few_rows", "single", "shared", "shared in tiles"])
 @pytest.mark.parametrize("dt,qv,kv", [(N.BF16, 2.0 ** 60, -2.0 ** 62), (N.BF16, 2.0 ** 60, 2.0 ** 61), (N.BF16, 3.0, 2.0 ** 20),
                                       (N.F16, 60000.0, 30000.0), (N.F16, 60000.0, -30000.0)])
 @pytest.mark.parametrize("scale", [None, 0.0])
@@ -189,7 +189,9 @@ def test_scores_far_from_zero(be, form, dt, qv, kv, scale):
     V, to the fp32 sums' (n + 8) 2^-24 of the mean of |v| and one rounding; and a position
     that stands out by half a score takes all."""
     lens = [300, 90] if form != "few_rows" else [3000, 90]
-    c, slots = held(11, lens, kv_heads=1, d=64, dt=dt)
+    blocks = 80 if form == "shared in tiles" else blocks_of(max(lens)) + 1
+    form = form.split()[0]
+    c, slots = held(11, lens, kv_heads=1, d=64, dt=dt, blocks=blocks)
     c.k[:] = to_bits(np.full(1, kv / 8), dt)[0]
     new = {"packed": lens, "few_rows": [20, 7], "single": [1, 1], "shared": [1, 1]}[form]
     prefix = 64 if form == "shared" else 0 if form == "single" else None
@@ -231,10 +233,22 @@ def test_rows_have_the_same_bits_twice(be):
 # ---- shared ------------------------------------------------------------------------
 
 
+ROOM = [0]
+
+
+@pytest.fixture(params=["by rows", "in tiles"])
+def way(request):
+    """Short sequences read their prefix row by row, unless the slots could be long (and
+    the batch does not say): then tiles of all rows do."""
+    ROOM[0] = 60 if request.param == "in tiles" else 0
+    yield
+    ROOM[0] = 0
+
+
 def behind(seed, n, prefix, own, **kw):
     """n slots that begin with the same `prefix` positions, own[i] after them."""
     kw.setdefault("seqs", n + 2)
-    kw.setdefault("blocks", blocks_of(prefix + max(own)) + 1)
+    kw.setdefault("blocks", blocks_of(prefix + max(own)) + 1 + ROOM[0])
     kw.setdefault("pages", prefix // PAGE + sum(blocks_of(x) for x in own) + 3)
     c = Cache(seed, **kw)
     slots = np.random.default_rng(seed).permutation(kw["seqs"])[:n].tolist()
@@ -257,14 +271,16 @@ def behind(seed, n, prefix, own, **kw):
                                           (2, 0, [1, 300]), (40, 128, [1 + 7 * i % 90 for i in range(40)]),
                                           (9, 1024, [2] * 9)])
 @pytest.mark.parametrize("d,hkv,group", HEADS)
+@pytest.mark.usefixtures("way")
 def test_shared(be, n, prefix, own, d, hkv, group):
     dt = N.F16 if (d + n) % 3 else N.BF16
     c, slots = behind(n + d, n, prefix, own, d=d, kv_heads=hkv, dt=dt, layers=2)
-    run(be, c, slots, None, hkv * group, prefix=prefix, layer=1, max_len=prefix + max(own))
+    run(be, c, slots, None, hkv * group, prefix=prefix, layer=1)
 
 
 @pytest.mark.parametrize("dt", [N.F16, N.BF16])
 @pytest.mark.parametrize("out_dt", [N.F16, N.BF16])
+@pytest.mark.usefixtures("way")
 def test_shared_types_and_scales(be, dt, out_dt):
     c, slots = behind(5, 4, 192, [1, 5, 64, 100], dt=dt)
     for scale in (None, 1.0, 0.0, -0.2):
@@ -280,12 +296,14 @@ def test_shared_long(be, max_len):
     run(be, c, slots, None, 4, prefix=0, max_len=max_len)
 
 
+@pytest.mark.usefixtures("way")
 def test_shared_many(be):
     own = [1 + (i * 37) % 130 for i in range(300)]
     c, slots = behind(4, 300, 256, own, kv_heads=1, d=64)
     run(be, c, slots, None, 3, prefix=256)
 
 
+@pytest.mark.usefixtures("way")
 def test_shorter_than_the_prefix(be):
     """Slots that end inside the prefix, empty ones, and one that begins otherwise:
     its first positions are read as slots[0]'s."""
@@ -295,6 +313,7 @@ def test_shorter_than_the_prefix(be):
     run(be, c, slots, None, 8, prefix=256)
 
 
+@pytest.mark.usefixtures("way")
 def test_first_slot_shorter_than_the_prefix(be):
     """Only its whole pages are shared; the others read their own from there on."""
     c, slots = behind(7, 4, 256, [1, 20, 64, 90])
@@ -304,6 +323,7 @@ def test_first_slot_shorter_than_the_prefix(be):
     run(be, c, slots, None, 8, prefix=256)
 
 
+@pytest.mark.usefixtures("way")
 def test_shared_unknown_slots_and_pages(be):
     c, slots = behind(8, 3, 128, [10, 70, 5])
     sl = [slots[0], -1, slots[1], 77, slots[2]]
@@ -316,6 +336,7 @@ def test_shared_unknown_slots_and_pages(be):
     np.testing.assert_array_equal(from_bits(got[0], c.dt), 0)
 
 
+@pytest.mark.usefixtures("way")
 def test_pages_outside_the_pool_are_absent(be):
     """A page entry outside the pool hides its positions, in either form."""
     c, slots = behind(9, 2, 128, [70, 70], kv_heads=1)
@@ -341,6 +362,7 @@ def test_pages_outside_the_pool_are_absent(be):
 
 
 @pytest.mark.parametrize("bad", ["v_nan", "v_inf", "k_nan"])
+@pytest.mark.usefixtures("way")
 def test_shared_and_values_that_some_rows_do_not_see(be, bad):
     """A slot that ends inside the prefix does not see what stands after it."""
     c, slots = behind(10, 5, 192, [5, 5, 5, 5, 5], kv_heads=1, dt=N.BF16)
@@ -355,6 +377,7 @@ def test_shared_and_values_that_some_rows_do_not_see(be, bad):
     assert np.isfinite(want[[1, 3]]).all() and not np.isfinite(want[0]).all()
 
 
+@pytest.mark.usefixtures("way")
 def test_shared_has_the_same_bits_twice(be):
     c, slots = behind(11, 20, 1024, [1 + 40 * i for i in range(20)], dt=N.F16, kv_heads=2)
     a = call(be, c, slots, None, 16, prefix=1024)[1]

@@ -128,8 +128,8 @@ def step_of(be, dev, slots, n, prefix, rope, x, q, out, max_len):
         be.attn_shared(dev, layer, b, prefix, q, HEADS, out + 2 * layer * n * HEADS * D)
 
 
-@pytest.mark.parametrize("prefix", [0, 192])
-def test_a_recorded_step_follows_the_lengths(be, prefix):
+@pytest.mark.parametrize("prefix,most", [(0, 600), (192, 600), (192, 2500)])
+def test_a_recorded_step_follows_the_lengths(be, prefix, most):
     """Two equal caches, one stepped by replays, one eagerly, compared bit by bit
     after every step, over a page's end and with other work between the replays."""
     rng = np.random.default_rng(1)
@@ -139,7 +139,7 @@ def test_a_recorded_step_follows_the_lengths(be, prefix):
     freq, scale = rope_freqs(D)
     rope = Rope(freq=room.put(freq), dim=D, interleaved=1, scale=scale)
     for _ in range(2):
-        c = Cache(4, layers=LAYERS, pages=70, kv_heads=HKV, d=D, dt=N.BF16, seqs=6, blocks=14)
+        c = Cache(4, layers=LAYERS, pages=70, kv_heads=HKV, d=D, dt=N.BF16, seqs=6, blocks=40)
         for i, s in enumerate(slots):
             pages = None if i == 0 or not prefix else c.table[slots[0], :prefix // PAGE].tolist() + [
                 int(p) for p in np.flatnonzero(c.refs == 0)]
@@ -150,7 +150,7 @@ def test_a_recorded_step_follows_the_lengths(be, prefix):
     d_slots = ints(room, slots)
     q = room.put(np.zeros((n, HEADS * D), np.uint16))
     outs = [room.put(np.zeros((LAYERS, n, HEADS * D), np.uint16)) for _ in range(2)]
-    args = lambda k: (be, sides[k][1], d_slots, n, prefix, rope, x, q, outs[k], 600)
+    args = lambda k: (be, sides[k][1], d_slots, n, prefix, rope, x, q, outs[k], most)
     step_of(*args(0))  # workspaces grow outside the recording
     step_of(*args(1))
     be.graph_begin()
@@ -246,7 +246,7 @@ def test_a_recording_whose_workspace_was_replaced(be):
 
 @pytest.mark.parametrize("new,lens,prefix", [([70, 3], [300, 900], None), ([2000], [2000], None), ([5] * 3, [4000] * 3, None),
                                              ([1] * 5, [100, 1, 64, 700, 9], 0), ([1] * 2, [3000, 5000], 0),
-                                             ([1] * 40, [700] * 40, 640)])
+                                             ([1] * 40, [700] * 40, 640), ([1] * 5, [1500] * 5, 640)])
 def test_out_may_be_q(be, new, lens, prefix):
     room = Room(be)
     hkv, group = 2, 20 if prefix == 0 else 3

@@ -67,12 +67,15 @@ def test_packed_with_values_that_are_not_finite(be, bad, rows, length):
 
 SHARED = {
     # name: (slots, prefix, own positions of each, head dim, kv heads, group)
-    "64 rows, a page a part": (5, 512, [1, 9, 64, 65, 200], 128, 2, 4),
+    "by rows": (5, 512, [1, 9, 64, 65, 200], 128, 2, 4),
+    "by rows, 20 pages": (5, 1216, [1, 9, 64, 63, 2], 64, 2, 4),
+    "64 rows, a page a part": (5, 512, [1, 9, 64, 65, 1500], 128, 2, 4),
     "64 rows, many parts": (3, 4096, [700, 1, 64], 64, 1, 4),
     "128 rows": (66, 8256, [1 + i for i in range(66)], 64, 1, 16),
     "no prefix, cut": (2, 0, [3000, 10], 128, 1, 4),
     "no prefix, whole": (40, 0, [1 + 7 * i for i in range(40)], 64, 8, 3),
     "groups of more than 16 heads": (3, 256, [5, 70, 1], 64, 1, 40),
+    "groups of more than 16 heads, in tiles": (3, 256, [5, 70, 1400], 64, 1, 40),
     "groups of more than 16 heads, no prefix": (3, 0, [5, 700, 1], 128, 2, 17),
     "many parts of many rows": (24, 2048, [30] * 24, 64, 4, 16),
 }
@@ -103,7 +106,8 @@ def test_shared_tiles_with_values_that_are_not_finite(be):
 
 def test_a_thousand_slots(be):
     own = [1 + i % 70 for i in range(1024)]
-    c, slots = behind(6, 1024, 128, own, d=64, kv_heads=1, dt=N.F16)
+    c, slots = behind(6, 1024, 128, own, d=64, kv_heads=1, dt=N.F16, blocks=30)
     run(be, c, slots, None, 2, prefix=128, max_len=longest(c))
+    run(be, c, slots, None, 2, prefix=128)  # in tiles
     new = [min(x, 1 + i % 3) for i, x in enumerate(own)]
     run(be, c, slots, cu_of(new), 2, max_len=longest(c))
