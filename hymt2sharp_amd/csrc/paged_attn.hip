@@ -966,7 +966,14 @@ Shape shape_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, boo
         // which moves more partials than it saves (64 rows behind 1024: one page 15.6 us,
         // three 13.9; 16 behind 8192: two 16.8, three 15.5; 8 behind 512: one 9.4, two 10.1).
         if (s.tiles) cut((long)s.tiles * p.kv_heads, common, common, kCus, common <= 8 ? 1 : 3, 0, s.parts, s.span);
-        cut(rows, pages - common, pages - common, kCus, 4, s.tiles ? 0 : 4, s.own, s.own_span);
+        cut(rows, pages - common, pages - common, kCus, 4, 0, s.own, s.own_span);
+        // Without tiles whole ranges need no join: cut in two or three they gain less (cut and whole:
+        // 8 rows over 576 positions 8.5 and 7.1 us, over 832 8.9 and 9.1, over 2048 12.3 and 14.6; 32
+        // over 832 15.2 and 11.9, over 2048 29.5 and 28.0).
+        if (!s.tiles && pages <= 2 * s.own_span + 4) {
+            s.own = 1;
+            s.own_span = std::max(pages, 1);
+        }
     } else {
         auto tiles = [&](int rows) {
             return (int)(b.cu ? (long)b.rows * group / rows + b.n : (long)b.n * ceil_div(group, rows));
