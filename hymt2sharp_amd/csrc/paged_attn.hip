@@ -24,10 +24,11 @@
 //             8192: 235 us, 1.17 PFLOP/s; four of 4096 to 8192: 495, 1.10.  Not
 //             kept: the next page's S beside this one's weights (48 -> 49-56 us at
 //             2048), tiles of 192 rows, one to a CU (495 -> 840).
-// row part    (row_part) one entry's G rows over its own pages: pages go
-//             from memory straight into operand registers, a page to a wave, the next
-//             page's as soon as the products have read these.  Bound by memory:
-//             512 single rows behind 500 positions each 105 us, 5.0 TB/s.
+// row part    (row_part) one entry's G rows over its own pages, and those of the prefix
+//             where sequences are short: pages go from memory straight into operand
+//             registers, a page to a wave, the next page's as soon as the products have
+//             read these.  Bound by memory:
+//             64 rows over 2048 positions each 48 us, 5.6 TB/s.
 // joining     where rows are few, a kv range is cut into parts whose (O, m, l) meet
 //             in a second launch, in fp32: 4 to 7 us, most of it the launch (64 rows behind 4096
 //             10 MB of partials in 5.1 us).
