@@ -120,6 +120,15 @@ def test_packed_single_rows_without_offsets(be, n, group):
     run(be, c, slots, None, group)
 
 
+@pytest.mark.parametrize("lens", [[3000], [5000, 1, 0, 2600, 64], [2900] * 30])
+def test_packed_single_rows_over_many_positions(be, lens):
+    """Cut and joined, with offsets and without: the same bits."""
+    c, slots = held(len(lens), lens, kv_heads=1, d=64, dt=N.F16)
+    a = run(be, c, slots, None, 5)
+    b = run(be, c, slots, list(range(len(lens) + 1)), 5)
+    np.testing.assert_array_equal(a, b)
+
+
 @pytest.mark.parametrize("n", [300, 1024])
 def test_packed_hundreds_of_prompts(be, n):
     rng = np.random.default_rng(n)
