@@ -183,8 +183,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_fork_plan_kernel(hymt_page
                                                                        const int32_t *child, int n) {
     __shared__ PlanShared sh;
     const int i = threadIdx.x, free0 = is_free(p, i);
-    int from = 0, to = 0, len = 0, need = 0, src = 0;
-    bool known = false;
+    int from = 0, to = 0, len = 0, need = 0, src = 0, held = 1;
+    bool known = false, gone = false;
     if (i < n) {
         from = parent[i];
         to = child[i];
@@ -203,19 +203,27 @@ __global__ __launch_bounds__(kPlanThreads) void paged_fork_plan_kernel(hymt_page
             need = 1;
             src = p.table[(size_t)from * p.blocks + len / kPage];
             if ((unsigned)src >= (unsigned)p.pages) plan_fail(sh, HYMT_E_STATE);
+            else held = p.refs[src];
         }
         sh.slot[i] = from;
         sh.count[i] = len / kPage;
     }
     __syncthreads();
     if (known && (sh.bits[from >> 5] >> (from & 31) & 1)) plan_fail(sh, HYMT_E_ARG);
-    // whole pages have to be in the pool before one of them is counted again
+    // whole pages have to be in the pool, and in use (a free one may be handed out
+    // here), before one of them is counted again
     for (int e = threadIdx.x >> 6; e < n; e += kPlanWaves)
-        for (int j = threadIdx.x & 63; j < sh.count[e]; j += 64)
-            if ((unsigned)p.table[(size_t)sh.slot[e] * p.blocks + j] >= (unsigned)p.pages) plan_fail(sh, HYMT_E_STATE);
+        for (int j = threadIdx.x & 63; j < sh.count[e]; j += 64) {
+            const int page = p.table[(size_t)sh.slot[e] * p.blocks + j];
+            if ((unsigned)page >= (unsigned)p.pages) plan_fail(sh, HYMT_E_STATE);
+            else gone |= p.refs[page] <= 0;
+        }
     int32_t *list = work_dst(p);
     int rank, total;
     if (!hand_out(p, sh, need, free0, list, rank, total) && i == 0) plan_fail(sh, HYMT_E_CAPACITY);
+    // the counts, loaded while the free pages were looked up; a page that is copied is
+    // its sequence's alone
+    if (gone || held != 1) plan_fail(sh, HYMT_E_STATE);
     __syncthreads();
     if (sh.status != HYMT_OK) {
         if (i == 0) finish(p, sh.status, 0);
@@ -238,6 +246,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_set_len_plan_kernel(hymt_p
     __shared__ PlanShared sh;
     const int i = threadIdx.x, free0 = is_free(p, i);
     int slot = 0, len = 0, want = 0, need = 0, src = 0;
+    bool gone = false;
     if (i < n) {
         slot = slots[i];
         want = lens ? lens[i] : 0;
@@ -264,13 +273,17 @@ __global__ __launch_bounds__(kPlanThreads) void paged_set_len_plan_kernel(hymt_p
         }
     }
     __syncthreads();
+    // pages that are given up have to be in the pool and in use
     for (int e = threadIdx.x >> 6; e < n; e += kPlanWaves)
-        for (int j = threadIdx.x & 63; j < sh.count[e]; j += 64)
-            if ((unsigned)p.table[(size_t)sh.slot[e] * p.blocks + sh.first[e] + j] >= (unsigned)p.pages)
-                plan_fail(sh, HYMT_E_STATE);
+        for (int j = threadIdx.x & 63; j < sh.count[e]; j += 64) {
+            const int page = p.table[(size_t)sh.slot[e] * p.blocks + sh.first[e] + j];
+            if ((unsigned)page >= (unsigned)p.pages) plan_fail(sh, HYMT_E_STATE);
+            else gone |= p.refs[page] <= 0;
+        }
     int32_t *list = work_dst(p);
     int rank, total;
     if (!hand_out(p, sh, need, free0, list, rank, total) && i == 0) plan_fail(sh, HYMT_E_CAPACITY);
+    if (gone) plan_fail(sh, HYMT_E_STATE);
     __syncthreads();
     if (sh.status != HYMT_OK) {
         if (i == 0) finish(p, sh.status, 0);

@@ -477,11 +477,14 @@ int hymt_gemm_i8_swiglu(hymt_ctx *ctx, const int8_t *gate, const float *gate_sca
  * work[0] keeps the status (hymt_status) of the first call that found something
  * wrong on the device, until the caller clears it: HYMT_E_ARG a slot outside the
  * cache, a slot twice, a falling cu; HYMT_E_CAPACITY too few free pages or more
- * than blocks * 64 positions; HYMT_E_STATE a fork into a slot that is not empty, or a table
- * entry, length or count that the rules above exclude.  Such a call changes
- * nothing else.  work[1] is the number of pages that the last such call copied,
- * work[2] the number of pages in use at the last compact, work[3] the last call's own
- * status.
+ * than blocks * 64 positions; HYMT_E_STATE a fork into a slot that is not empty, a length
+ * outside [0, blocks * 64], or an entry outside the pool or a count that cannot be
+ * among those that the call goes by: other than 1 for the page that extend writes on or
+ * fork copies, below 1 for a page that fork shares or set_len cuts inside or gives up.  Such
+ * a call changes nothing else.  (Whether the counts are the numbers of entries is not
+ * looked into any further, and compact goes by them alone.)  work[1] is the number of
+ * pages that the last such call copied, work[2] the number of pages in use at the last
+ * compact, work[3] the last call's own status.
  * The other calls' reads and writes stay inside the buffers whatever these hold:
  * slots outside the cache count as empty, positions in pages outside the pool as
  * absent. */
