@@ -43,6 +43,7 @@
 #include "device_common.hpp"
 #include "ktimer.hpp"
 #include "paged.hpp"
+#include "paged_split.hpp"
 
 namespace hymt {
 
@@ -102,7 +103,6 @@ __device__ __forceinline__ float rows_sum(float v) {
     r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-constexpr int kMaxParts = 64;      // parts of a split range
 constexpr float kLazyMax = 8.0f;   // weights stay below 2^8 of the running maximum's
 constexpr float kNoMax = -3.4028234e38f;  // the maximum before any score: finite, so that -inf - m is -inf
 // c s - m in one fma has the rounding of m = c max s left over, |m| 2^-25 of a power of
@@ -921,91 +921,7 @@ template <typename T, int D, bool WHOLE> __global__ __launch_bounds__(256) void 
 
 // ---- host --------------------------------------------------------------------------
 
-constexpr int kCus = 256;
-
-struct Shape {
-    int tiles, parts, span, own, own_span, blocks16;
-    int groups;  // of waves in a tile workgroup
-    int rows;    // of a tile
-};
-int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
-
-// Cut ranges of up to `longest` pages, `average` on average, of `wgs` workgroups so
-// that every one of `slots` gets its share, `least` pages at least, unless that saves
-// less than `worth` pages' time on the longest.
-void cut(long wgs, int longest, long average, int slots, int least, int worth, int &parts, int &span) {
-    span = std::max({least, ceil_div(wgs * average, slots), ceil_div(longest, kMaxParts), 1});
-    if (longest <= span + worth) span = std::max(longest, 1);
-    parts = std::max(1, ceil_div(longest, span));
-}
-
-Shape shape_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, bool shared) {
-    const int group = a.heads / p.kv_heads;
-    const long longest = b.max_len > 0 ? std::min<long>(b.max_len, (long)p.blocks * kPage) : (long)p.blocks * kPage;
-    const int pages = ceil_div(longest, kPage);
-    Shape s{0, 1, 1, 1, 1, (group + 15) / 16, 1, 128};
-    if (shared) {
-        const int common = (int)std::min<long>(a.prefix, longest) / kPage;
-        // tiles of 64 rows until a CU has more than 8 pages of them (128 rows and 64: 8
-        // rows behind 512 positions 9.4 and 8.6 us, 64 behind 4096 20.3 and 18.3, 128 22.1 and
-        // 21.3; 256 behind 16384 73 and 88)
-        if ((long)ceil_div((long)b.n * group, 64) * p.kv_heads * common <= 8 * kCus) s.rows = 64;
-        s.tiles = a.prefix ? ceil_div((long)b.n * group, s.rows) : 0;
-        const long rows = (long)b.n * p.kv_heads * s.blocks16;
-        // Short sequences, and not too many rows: each row by itself through the prefix too, in one
-        // launch without a join.  With tiles and without, us: 8 rows behind 512 positions and 64
-        // of their own 8.7 and 6.8, 64 rows 12.8 and 8.1, 256 rows 21.2 and 19.0; behind 1024 8
-        // rows 10.6 and 9.2, 128 18.0 and 15.9, 256 21.6 and 27.3; behind 1536 8 rows 10.3 and 11.4.
-        if (s.tiles && pages <= 20 && rows * pages <= 40 * kCus) {
-            s.tiles = 0;
-            s.own_span = pages;
-            return s;
-        }
-        // One tile a CU, beside it the rows: at 256 rows behind 16384 positions 75 us
-        // (tiles in both places first, rows after them, 94).  Short parts, as
-        // the join is launched anyway, yet not one page each of a longer prefix,
-        // which moves more partials than it saves (64 rows behind 1024: one page 15.6 us,
-        // three 13.9; 16 behind 8192: two 16.8, three 15.5; 8 behind 512: one 9.4, two 10.1).
-        if (s.tiles) cut((long)s.tiles * p.kv_heads, common, common, kCus, common <= 8 ? 1 : 3, 0, s.parts, s.span);
-        cut(rows, pages - common, pages - common, kCus, 4, 0, s.own, s.own_span);
-        // Without tiles whole ranges need no join: cut in two or three they gain less (cut and whole:
-        // 8 rows over 576 positions 8.5 and 7.1 us, over 832 8.9 and 9.1, over 2048 12.3 and 14.6; 32
-        // over 832 15.2 and 11.9, over 2048 29.5 and 28.0).
-        if (!s.tiles && pages <= 2 * s.own_span + 4) {
-            s.own = 1;
-            s.own_span = std::max(pages, 1);
-        }
-    } else {
-        auto tiles = [&](int rows) {
-            return (int)(b.cu ? (long)b.rows * group / rows + b.n : (long)b.n * ceil_div(group, rows));
-        };
-        s.tiles = tiles(s.rows);
-        // the rows are an entry's last ones: the first of them attend to less
-        const int average = pages - (int)(std::min<long>(b.rows, longest) / kPage / 2);
-        const long wgs = (long)s.tiles * p.kv_heads;
-        // Two groups of waves, which halve a tile's own time, where the longest
-        // tile takes about as long as the chip needs for all: one prompt of 2048
-        // 48 -> 38 us, of 4096 93 -> 80; three of 2048 would go from 73 to 84, one of
-        // 8192 from 262 to 277.
-        if (pages >= 8 && 5L * pages * kCus >= 4 * wgs * average) s.groups = 2;
-        // Few tiles of long ranges are cut besides (two chunks of 256 over 8192: 68
-        // us with two parts, 50 with four).  Shorter ranges or more tiles are not: one
-        // prompt of 1000 cut in four 34 us, whole 17; of 2048 47 and 38.
-        if (wgs <= kCus / 2) cut(wgs, pages, average, 2 * kCus / s.groups, 4, 24, s.parts, s.span);
-        else s.span = pages;
-        // Tiles of half the rows, as a tile's time is mostly its own chain of reads
-        // and products, as long as they do not queue for the CUs (128 rows and 64: one
-        // sentence 8.6 and 6.6 us, 32 of them 11.0 and 10.0, one prompt of 700 18.8 and
-        // 13.5, of 2048 37.6 and 34.2; but 12 of 200 16.0 and 17.1, 64 of 61 16.1 and 18.2).
-        if (s.parts == 1 && 8 * wgs <= 9 * kCus) {
-            s.rows = 64;
-            s.tiles = tiles(s.rows);
-        }
-    }
-    return s;
-}
-
-Plan plan_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, const Shape &s, float *ws) {
+Plan plan_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, const PagedSplit &s, float *ws) {
     Plan r{};
     r.p = p;
     r.b = b;
@@ -1030,7 +946,7 @@ Plan plan_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, const
     return r;
 }
 
-template <typename T, int D> void packed(const Plan &a, const Shape &s, hipStream_t st) {
+template <typename T, int D> void packed(const Plan &a, const PagedSplit &s, hipStream_t st) {
     {
         KernelSpan span("attn_packed", st, true);
         const dim3 grid(s.tiles * s.parts * a.p.kv_heads);
@@ -1047,7 +963,7 @@ template <typename T, int D> void packed(const Plan &a, const Shape &s, hipStrea
     launch(span, attn_join_tiles_kernel<T, D>, dim3(std::min<long>((long)s.tiles * (s.rows * D / 1024) * a.p.kv_heads, kJoinGrid)), dim3(256), 0, st, a);
 }
 
-template <typename T, int D> void shared(Plan a, const Shape &s, hipStream_t st) {
+template <typename T, int D> void shared(Plan a, const PagedSplit &s, hipStream_t st) {
     const int tile_wgs = s.tiles * s.parts * a.p.kv_heads, row_wgs = a.b.n * a.p.kv_heads * s.blocks16 * s.own;
     a.direct = s.tiles == 0 && s.own == 1;
     if (s.tiles == 0) a.parts = 0;
@@ -1064,21 +980,21 @@ template <typename T, int D> void shared(Plan a, const Shape &s, hipStream_t st)
     if (a.parts + a.own_parts > L || (rows < 2048 && a.parts + a.own_parts >= G))
         launch(span, attn_join_rows_kernel<T, D, true>, dim3((unsigned)rows), dim3(256), 0, st, a);
     else
-        launch(span, attn_join_rows_kernel<T, D, false>, dim3(ceil_div(rows, G)), dim3(256), 0, st, a);
+        launch(span, attn_join_rows_kernel<T, D, false>, dim3((unsigned)ceil_div(rows, G)), dim3(256), 0, st, a);
 }
 
 }  // namespace
 
 size_t paged_attn_workspace(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, bool shared) {
     if (b.n == 0 || b.rows == 0) return 0;
-    const Shape s = shape_of(p, b, a, shared);
+    const PagedSplit s = paged_split(p, b, a.heads, a.prefix, shared);
     if (shared ? s.tiles == 0 && s.own == 1 : s.parts == 1) return 0;
     return (size_t)(s.parts + s.own) * b.rows * a.heads * (p.head_dim + 2);
 }
 
 hipError_t launch_attn_packed(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, float *ws, hipStream_t st) {
     if (b.n == 0 || b.rows == 0) return hipSuccess;
-    const Shape s = shape_of(p, b, a, false);
+    const PagedSplit s = paged_split(p, b, a.heads, 0, false);
     const Plan r = plan_of(p, b, a, s, ws);
     if (p.dtype == HYMT_F16) p.head_dim == 64 ? packed<F16, 64>(r, s, st) : packed<F16, 128>(r, s, st);
     else p.head_dim == 64 ? packed<BF16, 64>(r, s, st) : packed<BF16, 128>(r, s, st);
@@ -1087,7 +1003,7 @@ hipError_t launch_attn_packed(const hymt_paged &p, const hymt_batch &b, const Pa
 
 hipError_t launch_attn_shared(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, float *ws, hipStream_t st) {
     if (b.n == 0) return hipSuccess;
-    const Shape s = shape_of(p, b, a, true);
+    const PagedSplit s = paged_split(p, b, a.heads, a.prefix, true);
     const Plan r = plan_of(p, b, a, s, ws);
     if (p.dtype == HYMT_F16) p.head_dim == 64 ? shared<F16, 64>(r, s, st) : shared<F16, 128>(r, s, st);
     else p.head_dim == 64 ? shared<BF16, 64>(r, s, st) : shared<BF16, 128>(r, s, st);
