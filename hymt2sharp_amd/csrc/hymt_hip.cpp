@@ -1591,7 +1591,7 @@ int paged_attention(hymt_ctx *c, const hymt_paged *p, int layer, const hymt_batc
     if (prefix < 0 || prefix % kPage != 0) return fail(HYMT_E_ARG, "prefix must be a multiple of 64");
     if (!q || !out) return fail(HYMT_E_ARG, "null q or out");
     if (out_dtype != HYMT_F16 && out_dtype != HYMT_BF16) return fail(HYMT_E_UNSUPPORTED, "out must be fp16 or bf16");
-    if (!std::isfinite(scale)) return fail(HYMT_E_ARG, "scale must be finite");
+    if (!std::isfinite(paged_log2_scale(scale))) return fail(HYMT_E_ARG, "scale must be finite, and times log2 e too");
     if (misaligned16(q) || misaligned16(out)) return fail(HYMT_E_ARG, "q and out must be 16-byte aligned");
     const PagedAttn a{q, heads, layer, prefix, scale, out, out_dtype};
     if (!c->has_device()) return fail(HYMT_E_NO_DEVICE, "context has no device");

@@ -56,6 +56,10 @@ struct RopeAppend {
     void *q_out;
 };
 
+// Scores are multiplied by this before the powers of 2; the entry points see to it
+// that it is finite (the product with a score of 0 would not be one otherwise).
+inline float paged_log2_scale(float scale) { return scale * 1.4426950408889634f; }
+
 struct PagedAttn {
     const void *q;
     int heads, layer, prefix;

@@ -932,7 +932,7 @@ Plan plan_of(const hymt_paged &p, const hymt_batch &b, const PagedAttn &a, const
     r.layer = a.layer;
     r.prefix = a.prefix;
     r.out_f16 = a.out_dtype == HYMT_F16;
-    r.c = std::max(std::abs(a.scale) * 1.4426950408889634f, std::numeric_limits<float>::denorm_min());
+    r.c = std::max(std::abs(paged_log2_scale(a.scale)), std::numeric_limits<float>::denorm_min());
     r.flip = a.scale < 0 ? 0x80008000u : 0u;
     r.parts = s.parts;
     r.span = s.span;

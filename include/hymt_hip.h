@@ -584,7 +584,8 @@ int hymt_rope_append(hymt_ctx *ctx, const hymt_paged *cache, int layer, const hy
  * pages where a row does not attend, infinities and NaN too, does not reach it (where
  * it does attend they make its result infinite or NaN).
  * Softmax and sums in fp32, its weights rounded to the cache's type for the
- * products with V.  q and out 16-byte aligned; out may be q, else they do not overlap. */
+ * products with V.  |scale| up to 2^127.  q and out 16-byte aligned; out may be q, else they
+ * do not overlap. */
 int hymt_attn_packed(hymt_ctx *ctx, const hymt_paged *cache, int layer, const hymt_batch *batch, const void *q,
                      int heads, float scale, void *out, int out_dtype);
 

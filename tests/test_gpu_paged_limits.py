@@ -1,11 +1,12 @@
 """The attention over the multi-sequence cache at the ends of what its entry points
 accept."""
+import numpy as np
 import pytest
 
 from hymt2sharp_amd import HipBackend
 from hymt2sharp_amd import _native as N
 from tests.paged_cases import Cache
-from tests.test_gpu_paged_attn import run
+from tests.test_gpu_paged_attn import run, cu_of
 
 pytestmark = pytest.mark.gpu
 
@@ -32,3 +33,17 @@ def test_rows_of_sequences_that_could_have_2_24_pages(be):
         pass
     be.timing_enable(0)
     assert calls == 1 and merges == 0
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 127, -2.0 ** 127])
+@pytest.mark.parametrize("new,lens,prefix", [([70, 9], [70, 200], None), ([20], [3000], None), ([1, 1], [70, 200], 0),
+                                             ([1, 1], [70, 2000], 64)])
+def test_the_largest_scale(be, scale, new, lens, prefix):
+    """Scores of 0 times the largest scale are 0: the mean of V."""
+    c = Cache(2, pages=60, kv_heads=1, d=64, dt=N.BF16, seqs=2, blocks=50)
+    for i, n in enumerate(lens):
+        c.give(i, n)
+    if prefix:
+        c.table[1, 0] = c.table[0, 0]
+    run(be, c, [0, 1][:len(new)], None if prefix is not None else cu_of(new), 4, scale=scale, prefix=prefix,
+        q=np.zeros((sum(new), 4 * 64)))
