@@ -65,10 +65,14 @@ inline PagedSplit paged_split(const hymt_paged &p, const hymt_batch &b, int head
         // three 13.9; 16 behind 8192: two 16.8, three 15.5; 8 behind 512: one 9.4, two 10.1).
         if (s.tiles) cut((long)s.tiles * p.kv_heads, common, common, kCus, common <= 8 ? 1 : 3, 0, s.parts, s.span);
         cut(rows, pages - common, pages - common, kCus, 4, 0, s.own, s.own_span);
-        // Without tiles whole ranges need no join: cut in two or three they gain less (cut and whole:
-        // 8 rows over 576 positions 8.5 and 7.1 us, over 832 8.9 and 9.1, over 2048 12.3 and 14.6; 32
-        // over 832 15.2 and 11.9, over 2048 29.5 and 28.0).
-        if (!s.tiles && pages <= 2 * s.own_span + 4) {
+        // Without tiles whole ranges need no join: cut in two or three they gain less (cut and whole,
+        // us: 8 rows of 4 kv heads over 576 positions 9.3 and 7.9, over 2048 13.1 and 15.5; 32 over
+        // 832 16.0 and 12.6, over 2048 30.3 and 28.8; 48 over 8192 146 and 134, over 32768 549 and
+        // 518; 60 over 32768 663 and 657), except that a workgroup for every other CU is too
+        // few for long ranges (32 rows over 4096 52.3 and 51.8, over 8192 97.7 and 98.2, over
+        // 32768 360 and 375).
+        const bool few = rows <= kCus / 2 && pages > 128;
+        if (!s.tiles && !few && pages <= 2 * s.own_span + 4) {
             s.own = 1;
             s.own_span = std::max(pages, 1);
         }

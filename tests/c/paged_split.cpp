@@ -87,6 +87,14 @@ int main() {
     where = "the largest";
     const PagedSplit s = split(1024, 32, 1, 1 << 24, 0, 0, true, 1024);
     CHECK(s.own == 1 && s.own_span == 1 << 24);
+    // long ranges of half as many rows as CUs are cut in two, short ones and those of more
+    // rows stay whole
+    where = "single rows";
+    CHECK(split(32, 4, 4, 1 << 14, 32768, 0, true, 32).own == 2);
+    CHECK(split(16, 8, 4, 1 << 14, 8256, 0, true, 16).own == 2);
+    CHECK(split(32, 4, 4, 1 << 14, 8192, 0, true, 32).own == 1);
+    CHECK(split(33, 4, 4, 1 << 14, 32768, 0, true, 33).own == 1);
+    CHECK(split(48, 4, 4, 1 << 14, 32768, 0, true, 48).own == 1);
     if (failures) std::printf("%d failures\n", failures);
     return failures != 0;
 }
