@@ -593,6 +593,11 @@ __device__ __forceinline__ int slot_length(const hymt_paged &p, int slot) {
     return (unsigned)slot < (unsigned)p.seqs ? max(0, min(p.len[slot], 1 << 30)) : 0;
 }
 
+// Whether the last upkeep call went through.  If not, the lengths are those before it and
+// a batch's rows would fall on positions that stand already, of other sequences too
+// where the last page is whole.  Loaded beside what a row needs anyway.
+__device__ __forceinline__ bool has_grown(const hymt_paged &p) { return p.work[kWorkStatus] == HYMT_OK; }
+
 // The entry of row r (the first that ends behind it), its slot and its rows from r on.
 // Lanes look at 64 runs of entries, then at the run's, in two round trips at most.
 struct RowEntry {
@@ -635,12 +640,13 @@ __global__ __launch_bounds__(256) void rope_row_kernel(hymt_paged p, hymt_batch 
     const int u0 = threadIdx.x / L;
     Raw8<IO> next = load(u0), after = load(u0 + U);
     const double freq = (int)threadIdx.x < a.dim / 2 ? a.freq[threadIdx.x] : 0.0;
+    const bool grown = has_grown(p);
     RowEntry e{0, 1};
     if (!b.cu) e.slot = b.slots[row];
     else if (!entry_of_row(b, row, e)) return;
     const int slot = e.slot, pos = slot_length(p, slot) - e.behind;
     if ((int)threadIdx.x < a.dim / 2) s_cs[threadIdx.x] = turn_of(pos, freq, a.scale);
-    const bool stored = pos >= 0 && pos < (long)p.blocks * kPage;
+    const bool stored = grown && pos >= 0 && pos < (long)p.blocks * kPage;
     const int page = stored ? p.table[(size_t)slot * p.blocks + pos / kPage] : -1;
     const bool in_pool = (unsigned)page < (unsigned)p.pages;
     const int t = pos & (kPage - 1);
@@ -700,6 +706,7 @@ __global__ __launch_bounds__(256) void rope_block_kernel(hymt_paged p, hymt_batc
     __shared__ __attribute__((aligned(16))) uint16_t s_v[kRopeRows][D + 8];
     const int tid = threadIdx.x, lane = tid & 63;
     const int h = blockIdx.x % p.kv_heads, w = blockIdx.x / p.kv_heads;
+    const bool grown = has_grown(p);
     // ---- the block's entry: 64 entries at a time, one a lane
     int slot = -1, row0 = 0, n = 0, p0 = 0, index = -1;  // first row, rows, their first position, block of it
     for (int base = 0, before = 0; base < b.n; base += 64) {
@@ -728,7 +735,7 @@ __global__ __launch_bounds__(256) void rope_block_kernel(hymt_paged p, hymt_batc
     if (index < 0) return;
     const int pb = ((p0 >> 5) + index) * 32;  // position of the block's first row
     const int r_lo = max(0, p0 - pb), r_hi = min(kRopeRows, p0 + n - pb);
-    const bool stored = slot >= 0 && slot < p.seqs && pb >= 0 && pb < (long)p.blocks * kPage;
+    const bool stored = grown && slot >= 0 && slot < p.seqs && pb >= 0 && pb < (long)p.blocks * kPage;
     const int page = stored ? p.table[(size_t)slot * p.blocks + pb / kPage] : -1;
     const bool in_pool = (unsigned)page < (unsigned)p.pages;
     const int c = tid & (L - 1), d0 = 8 * c, r0 = tid / L;

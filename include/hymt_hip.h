@@ -572,7 +572,11 @@ int hymt_rope_freqs(int dim, double base, int scaling, double factor, int traine
  * [D] (fp32, NULL for none) 16-byte aligned.  heads is a multiple of kv_heads, up to 64
  * times.  A slot stands once in the batch (else which of its rows is stored is
  * open), and q_out overlaps none of the others.  Pages for the positions are there
- * already (hymt_paged_extend).  The counterpart of what hymt_attn_prefill does before its products. */
+ * already (hymt_paged_extend).  While work[3] is not 0, the last upkeep call having changed
+ * nothing, no row is stored (q_out is written all the same): after an extend that found too few
+ * pages the rows would take the place of the last positions.  So a step that is enqueued as a whole has
+ * its appends behind its own extend, and after one that failed the lengths say which slots have grown.
+ * The counterpart of what hymt_attn_prefill does before its products. */
 int hymt_rope_append(hymt_ctx *ctx, const hymt_paged *cache, int layer, const hymt_batch *batch, const void *q,
                      int q_ld, const void *k, const void *v, int kv_ld, int io_dtype, int heads,
                      const hymt_rope *rope, const float *qnw, const float *knw, float eps, void *q_out);
