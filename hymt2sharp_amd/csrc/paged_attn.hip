@@ -21,14 +21,14 @@
 //             much of exponentials and other vector work, which hardly run beside the
 //             products (a wave of 4 fmas to a product took 10.1 ns a product, products
 //             alone 6.8, fmas alone 4.4), and LDS reads of 32 KB a wave.  One prompt of
-//             8192: 235 us, 1.17 PFLOP/s; four of 4096 to 8192: 495, 1.10.  Not
+//             8192: 235-243 us, 1.13-1.17 PFLOP/s; four of 4096 to 8192: 495, 1.10.  Not
 //             kept: the next page's S beside this one's weights (48 -> 49-56 us at
 //             2048), tiles of 192 rows, one to a CU (495 -> 840).
 // row part    (row_part) one entry's G rows over its own pages, and those of the prefix
 //             where sequences are short: pages go from memory straight into operand
 //             registers, a page to a wave, the next page's as soon as the products have
 //             read these.  Bound by memory:
-//             64 rows over 2048 positions each 48 us, 5.6 TB/s.
+//             64 rows over 2048 positions each 48-49 us, 5.5 TB/s.
 // joining     where rows are few, a kv range is cut into parts whose (O, m, l) meet
 //             in a second launch, in fp32: 4 to 7 us, most of it the launch (64 rows behind 4096
 //             10 MB of partials in 5.1 us).
@@ -542,7 +542,7 @@ template <bool SPLIT> __device__ __forceinline__ bool find_tile(const Plan &a, i
     }
     if (!SPLIT && a.b.n > 64) {
         // 256 entries in a round trip, and the length after the search (256 prompts of 30
-        // rows 33.2 -> 30.0 us, 1024 of 8 rows 121 -> 85)
+        // rows 33.2 -> 30-32 us, 1024 of 8 rows 121 -> 85-88)
         constexpr int C = 4;
         for (int base = 0; base < a.b.n; base += 64 * C) {
             Span sp[C];

@@ -7,8 +7,10 @@
 // launch over the whole chip moves the bytes.  extend moves none and is the plan
 // alone.  A plan first looks at everything it would rely on and only then writes, so a
 // call that finds something wrong changes nothing but `work`.  A plan is a chain of
-// round trips (entries, lengths, table, counts) and two scans: 64 slots extended in 4.3 us,
-// 16 forked in 4.9, a pool of 512 compacted in 3.4.
+// round trips (entries, lengths, table, counts) and two scans: 64 slots extended in 4.2 us,
+// 16 forked in 5.0, 64 of 1000 positions released in 7.4, a pool of 512 compacted in 3.5.  Free
+// pages are looked for from the first on, 1024 at a time, 0.9 us each: behind 10000 pages in use 64
+// slots get one in 12.7 us, behind 60000 in 59.
 #include <algorithm>
 
 #include "attn_kernels.hpp"
@@ -687,7 +689,7 @@ __global__ __launch_bounds__(256) void rope_row_kernel(hymt_paged p, hymt_batch 
 // Packed rows: a workgroup takes the rows of one entry that lie in one block of 32
 // positions, for one kv head with its q heads.  A V chunk holds 8 of the block's
 // positions, so the block writes its chunks whole, 16 bytes a thread, after a
-// turn through LDS; row by row each chunk was written in 8 pieces, by
+// turn through LDS; row by row each chunk is written in 8 pieces, by
 // workgroups on 8 XCDs.  19 k rows of 24 heads in 58 us, 4.0 TB/s over 118 MB read and
 // 118 written, no more than it must (row by row 94 us; a plain copy would take 50).
 constexpr int kRopeRows = 32;
@@ -696,7 +698,10 @@ constexpr int kRopeRows = 32;
 // in turn; blocks win once the chip has several rows a CU.  bf16 cache, 16 q heads,
 // fp32 rows, by rows and by blocks, us: one entry of 64 rows 4.9 and 11.7, of 1024 10.8
 // and 12.8, of 1536 15.0 and 13.5, of 2048 17.1 and 13.7; 256 entries of 12 25.5 and 26.3, of 16
-// 34.5 and 31.7; 128 of 12 15.8 and 15.4.
+// 34.5 and 31.7; 128 of 12 15.8 and 15.4; one of 8192 and 700 of 1 71 and 89, one of 2048 and 200 of 1
+// 20.9 and 24.4.  The numbers are those of 4 kv heads: a block of a kv head with more q heads
+// is a longer chain, with fewer a shorter one (8 q heads of one kv head, 1536 rows 9.3 and
+// 18.1, 8192 28.5 and 19.9; 8 kv heads of one q head, bf16 rows, 1024 14.2 and 10.1, 1536 19.7 and 12.0).
 constexpr int kRopeFew = 1536, kRopeFewEach = 14;
 
 template <typename T, typename IO, int D>

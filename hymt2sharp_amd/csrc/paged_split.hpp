@@ -38,7 +38,7 @@ inline void cut(long wgs, int longest, long average, int slots, int least, int w
 
 inline PagedSplit paged_split(const hymt_paged &p, const hymt_batch &b, int heads, int prefix, bool shared) {
     const int group = heads / p.kv_heads;
-    const long longest = b.max_len > 0 ? std::min<long>(b.max_len, (long)p.blocks * HYMT_PAGE_TOKENS) : (long)p.blocks * HYMT_PAGE_TOKENS;
+    const long room = (long)p.blocks * HYMT_PAGE_TOKENS, longest = b.max_len > 0 ? std::min<long>(b.max_len, room) : room;
     const int pages = (int)ceil_div(longest, HYMT_PAGE_TOKENS);
     PagedSplit s{0, 1, 1, 1, 1, (group + 15) / 16, 1, 128};
     if (shared) {

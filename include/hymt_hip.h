@@ -509,15 +509,20 @@ typedef struct hymt_paged {
 /* A batch of rows: entry i is slot slots[i] and has the rows [cu[i], cu[i+1]) of
  * the packed tensors, or with cu NULL row i alone.  They are its last positions:
  * row j of n stands at len - n + j.  Rows from cu[n] on belong to no entry and are
- * left as they are. */
+ * left as they are.
+ * How the attention's work is split goes by max_len, as if every sequence were that
+ * long, and no result but for its rounding.  What a loose value costs: a bound several times
+ * too large, as a recording has to set one, leaves long ranges whole (two chunks of 256
+ * rows over 8192 positions 55 us with 8448, 125 with four times that; 8 single rows over 2048 13
+ * us, 14.5, and 19 with 16 times), and so do many short sequences beside a long one (256 single rows
+ * over 100 positions each 16 us, with one of 16384 among them 148). */
 typedef struct hymt_batch {
     const int32_t *slots; /* device, [n]                                            */
     const int32_t *cu;    /* device, [n + 1], rising from 0, or NULL                */
     int32_t n;            /* entries, up to HYMT_PAGED_BATCH                        */
     int32_t rows;         /* rows of the packed tensors, cu[n] at least (NULL: n); up to
                              2^22, and 2^28 times the q heads                       */
-    int32_t max_len;      /* about the longest len, 0 if unknown: how the work is split
-                             goes by it, and no result but for its rounding         */
+    int32_t max_len;      /* about the longest len, 0 if unknown (blocks * 64 then)  */
     int32_t reserved;     /* 0                                                      */
 } hymt_batch;
 
@@ -532,8 +537,8 @@ int hymt_paged_fork(hymt_ctx *ctx, const hymt_paged *cache, const int32_t *paren
 
 /* Slot slots[i] keeps its first min(len, lens[i]) positions (lens NULL: none, the
  * slot is free again): pages past them are given up, and one that the rest ends
- * inside is copied if another sequence holds it too.  The counterpart of
- * hymt_kv_set_len. */
+ * inside is copied if another sequence holds it too, into pages that were free before the
+ * call.  The counterpart of hymt_kv_set_len. */
 int hymt_paged_set_len(hymt_ctx *ctx, const hymt_paged *cache, const int32_t *slots, const int32_t *lens, int n);
 
 /* The pages in use become the first ones of the pool: the k-th page in use past
