@@ -376,7 +376,7 @@ class HipBackend:
     def rope_append(self, cache, layer: int, batch, q_dev, q_ld: int, k_dev, v_dev, kv_ld: int, io_dtype: int,
                     heads: int, rope, qnw, knw, eps: float, q_out_dev):
         """q_out = the batch's q rows rotated and normed; k (likewise) and v into
-        the pages of `layer`."""
+        the pages of `layer`, unless the last upkeep call was refused."""
         N.check(self._lib.hymt_rope_append(self._h, ctypes.byref(cache), layer, ctypes.byref(batch), q_dev, q_ld, k_dev,
                                            v_dev, kv_ld, io_dtype, heads, ctypes.byref(rope), qnw, knw, eps, q_out_dev))
 
